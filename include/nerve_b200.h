@@ -275,6 +275,56 @@ int32_t nerve_b200_op_rms_norm(const void *x_device, const void *weight_device, 
 int32_t nerve_b200_op_linear_fp8(const void *x_device, const void *w_device, const void *wscale_device,
                                  void *y_device, const void *residual_device, void *xq_scratch_device,
                                  void *xscale_scratch_device, int32_t lanes, int32_t n, int32_t k, void *stream);
+/* ---- 8-bit integers: linears with one scale per token and output channel, and sparse experts ----
+ * No counterpart in the reference (its 8-bit weights are FP8 and Q8_0).  x bf16 [lanes][k] is quantised per lane within the
+ * call: a = amax / 127, q = x / a to the nearest whole number, ties to even.  w int8 [n][k] (all 256 values), one f32 scale
+ * per output channel.  The products are added up exactly in 32-bit integers, so a lane's outputs do not depend on the other
+ * lanes of the call, bit for bit; what is rounded is q, (sum * channel scale) * a in f32, and the output, once.  A lane that
+ * holds an infinity or a NaN is NaN throughout; a lane of zeros gives zeros (+ residual).
+ * k: a multiple of 16, up to 131072.  w and scratch start on 16-byte boundaries, everything else on its type's.  The calls
+ * are asynchronous, capturable and allocate nothing but, the first on a device, what the INT4 linears' first call sets up;
+ * their waits are bounded as described above.  scratch holds ..._scratch_bytes(...) device bytes (0 for sizes that the call
+ * refuses); calls that may overlap in time, captured graphs among them, need one each.  0 lanes or tokens: nothing is done.
+ */
+uint64_t nerve_b200_op_linear_int8_scratch_bytes(int32_t lanes, int32_t k);
+/* y[lane][n] = x . W^T (+ residual bf16 [lanes][n], which may be y itself), bf16, or f32 where to_f32 != 0. */
+int32_t nerve_b200_op_linear_int8(const void *x_device, const void *w_device, const void *wscale_device, void *y_device,
+                                  const void *residual_device, void *scratch_device, int32_t lanes, int32_t n, int32_t k,
+                                  int32_t to_f32, void *stream);
+/* gate/up pair: y = bf16(silu(x . Wg^T) * (x . Wu^T)), the factors in f32. */
+int32_t nerve_b200_op_linear_int8_silu_pair(const void *x_device, const void *gate_w_device, const void *gate_scale_device,
+                                            const void *up_w_device, const void *up_scale_device, void *y_device,
+                                            void *scratch_device, int32_t lanes, int32_t n, int32_t k, void *stream);
+/* The choice of experts.  Scores: softmax over the open experts, or sigmoid, of logits [tokens][experts] (f32, or bf16 where
+ * logits_f32 is 0); an expert is closed to a token where its logit is NaN or -inf (+inf takes softmax's limit).
+ * Choices: score + bias (f32 [experts] or NULL; NaN and -inf close an expert).  groups > 1 cuts the experts into that many
+ * runs of equal length, ranks a run by the sum of its group_scores (1 or 2) largest choices, as many as it has, and
+ * leaves the chosen_groups best.  ids int32 [tokens][top_k]: the largest choices, the lower number first among equals, -1
+ * where open experts run out; weights f32 [tokens][top_k]: the scores without the bias (0 for -1), over the sum of the
+ * chosen ones' where renormalise != 0 (0 where that sum is 0), times scale.  Scores and choices are held in 64 bits.
+ * experts 1..1024, top_k 1..64 and no more than chosen_groups' experts, groups 1..32 that divide the experts into runs of
+ * at least group_scores. */
+typedef struct nerve_b200_routing {
+    int32_t experts, top_k;
+    int32_t sigmoid; /* 0 = softmax, 1 = sigmoid */
+    int32_t groups, chosen_groups, group_scores;
+    int32_t renormalise;
+    float scale;
+} nerve_b200_routing;
+int32_t nerve_b200_op_route_experts(const void *logits_device, const void *bias_device, void *ids_device, void *weights_device,
+                                    int32_t tokens, int32_t logits_f32, const nerve_b200_routing *routing, void *stream);
+/* Sparse experts: y[token] = bf16(sum over its routes of weight * down_e(silu(gate_e(x)) * up_e(x)) (+ residual)), both
+ * products as above, the intermediate rows quantised from f32 per route.  ids int32 and weights f32 [tokens][top_k] as
+ * nerve_b200_op_route_experts writes them: a route to none of the experts (-1, or any id outside 0..experts-1) adds nothing,
+ * an expert may be named twice.  gate_up_w int8 [experts][2 * inter][hidden], gate's rows first, gate_up_scale f32
+ * [experts][2 * inter]; down_w int8 [experts][hidden][inter], down_scale f32 [experts][hidden].  y may be x or residual.
+ * The result of a token does not depend on the other tokens of the call.  hidden and inter: multiples of 16 up to 131072;
+ * experts 1..1024, top_k 1..64, at most 2^24 routes. */
+uint64_t nerve_b200_op_experts_int8_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t hidden, int32_t inter);
+int32_t nerve_b200_op_experts_int8(const void *x_device, const void *ids_device, const void *weights_device, const void *gate_up_w_device,
+                                   const void *gate_up_scale_device, const void *down_w_device, const void *down_scale_device,
+                                   void *y_device, const void *residual_device, void *scratch_device, int32_t tokens, int32_t top_k,
+                                   int32_t experts, int32_t hidden, int32_t inter, void *stream);
 /* greedy_sampler_f32.comp.template:52-109: records u32[lanes][4] = {token, logit bits, 0, 0}.  Two-stage
  * reduction: scratch_device must hold nerve_b200_op_greedy_scratch_bytes(lanes) bytes. */
 int32_t nerve_b200_op_greedy(const void *logits_device, void *records_device, void *scratch_device, int32_t lanes,

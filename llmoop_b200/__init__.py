@@ -9,6 +9,7 @@ from .runtime import (  # noqa: F401
     Engine,
     NerveError,
     Package,
+    Routing,
     RunReport,
     library,
     nccl_library_path,

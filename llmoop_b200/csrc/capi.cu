@@ -1,4 +1,5 @@
 // extern "C" surface declared in include/nerve_b200.h: exception -> status + thread-local message.
+#include <algorithm>
 #include <cstring>
 #include <mutex>
 #include <exception>
@@ -187,6 +188,40 @@ int32_t linear_call(const char *name, bool bounded_waits, Body body) {
         verify(body(device));
     });
 }
+
+// ---- argument checks of the 8-bit integer operators
+
+bool on_boundary(const void *pointer, size_t bytes) { return reinterpret_cast<uintptr_t>(pointer) % bytes == 0; }
+void check_pointer(const char *name, const char *what, const void *pointer, size_t bytes, bool optional = false) {
+    if (pointer == nullptr && !optional) throw std::runtime_error(std::string(name) + ": " + what + " is NULL");
+    if (!on_boundary(pointer, bytes)) throw std::runtime_error(std::string(name) + ": " + what + " must start on a " + std::to_string(bytes) + "-byte boundary");
+}
+void check_size(const char *name, const char *what, int64_t value, int64_t least, int64_t most, int64_t multiple = 1) {
+    if (value < least || value > most || value % multiple != 0)
+        throw std::runtime_error(std::string(name) + ": " + what + " is " + std::to_string(value) + ", must be " + std::to_string(least) + " to " + std::to_string(most) +
+                                 (multiple > 1 ? " and a multiple of " + std::to_string(multiple) : ""));
+}
+constexpr int64_t INT8_MAX_LANES = 1 << 20, INT8_MAX_CHANNELS = 1 << 24, EXPERTS_MAX_ROUTES = 1 << 24;
+void check_int8_sizes(const char *name, int32_t lanes, int32_t n, int32_t k) {
+    check_size(name, "lanes", lanes, 0, INT8_MAX_LANES);
+    check_size(name, "n", n, 1, INT8_MAX_CHANNELS);
+    check_size(name, "k", k, 16, INT8_MAX_COLUMNS, 16);
+}
+void check_experts_sizes(const char *name, int32_t tokens, int32_t top_k, int32_t experts, int32_t hidden, int32_t inter) {
+    check_size(name, "experts", experts, 1, EXPERTS_INT8_MAX);
+    check_size(name, "top_k", top_k, 1, ROUTING_MAX_TOP_K);
+    check_size(name, "tokens", tokens, 0, EXPERTS_MAX_ROUTES / top_k);
+    check_size(name, "hidden", hidden, 16, INT8_MAX_COLUMNS, 16);
+    check_size(name, "inter", inter, 16, INT8_MAX_COLUMNS, 16);
+}
+// The activations of an 8-bit integer linear in the caller's scratch buffer: whole numbers, then one scale per lane.
+size_t int8_row_bytes(int32_t lanes, int32_t k) { return (static_cast<size_t>(lanes) * k + 255) / 256 * 256; }
+struct Int8Rows {
+    int8_t *values;
+    float *scales;
+    Int8Rows(void *scratch, int32_t lanes, int32_t k)
+        : values(static_cast<int8_t *>(scratch)), scales(reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + int8_row_bytes(lanes, k))) {}
+};
 
 // One reference less; the last one takes the model and the operator-level linears' unused memory with it.
 void release(nerve_b200_package *package) {
@@ -643,6 +678,127 @@ int32_t nerve_b200_op_linear_fp8(const void *x, const void *w, const void *wscal
                                          static_cast<const uint16_t *>(residual), lanes, n, k,
                                          residual ? EPILOGUE_RESIDUAL_F32 : EPILOGUE_BF16, st),
                        "nerve_b200_op_linear_fp8");
+}
+
+uint64_t nerve_b200_op_linear_int8_scratch_bytes(int32_t lanes, int32_t k) {
+    uint64_t bytes = 0;
+    guarded([&] {
+        check_int8_sizes("nerve_b200_op_linear_int8_scratch_bytes", lanes, 1, k);
+        bytes = int8_row_bytes(lanes, k) + static_cast<uint64_t>(lanes) * sizeof(float);
+    });
+    return bytes;
+}
+
+int32_t nerve_b200_op_linear_int8(const void *x, const void *w, const void *wscale, void *y, const void *residual, void *scratch, int32_t lanes, int32_t n, int32_t k,
+                                  int32_t to_f32, void *stream) {
+    constexpr const char *name = "nerve_b200_op_linear_int8";
+    const int32_t checked = guarded([&] {
+        check_int8_sizes(name, lanes, n, k);
+        if (lanes == 0) return;
+        check_pointer(name, "x", x, 2);
+        check_pointer(name, "w", w, 16);
+        check_pointer(name, "wscale", wscale, 4);
+        check_pointer(name, "y", y, to_f32 ? 4 : 2);
+        check_pointer(name, "residual", residual, 2, true);
+        check_pointer(name, "scratch", scratch, 16);
+    });
+    if (checked != NERVE_B200_OK || lanes == 0) return checked;
+    return linear_call(name, true, [&](const OperatorDevice *device) {
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const Int8Rows rows(scratch, lanes, k);
+        const cudaError_t status = launch_quantise_int8(static_cast<const uint16_t *>(x), rows.values, rows.scales, lanes, k, st);
+        if (status != cudaSuccess) return status;
+        return launch_linear_int8(rows.values, rows.scales, static_cast<const int8_t *>(w), static_cast<const float *>(wscale), y, static_cast<const uint16_t *>(residual),
+                                  lanes, n, k, to_f32, device->error_word(), st);
+    });
+}
+
+int32_t nerve_b200_op_linear_int8_silu_pair(const void *x, const void *gate_w, const void *gate_scale, const void *up_w, const void *up_scale, void *y, void *scratch,
+                                            int32_t lanes, int32_t n, int32_t k, void *stream) {
+    constexpr const char *name = "nerve_b200_op_linear_int8_silu_pair";
+    const int32_t checked = guarded([&] {
+        check_int8_sizes(name, lanes, n, k);
+        if (lanes == 0) return;
+        check_pointer(name, "x", x, 2);
+        check_pointer(name, "gate_w", gate_w, 16);
+        check_pointer(name, "gate_scale", gate_scale, 4);
+        check_pointer(name, "up_w", up_w, 16);
+        check_pointer(name, "up_scale", up_scale, 4);
+        check_pointer(name, "y", y, 2);
+        check_pointer(name, "scratch", scratch, 16);
+    });
+    if (checked != NERVE_B200_OK || lanes == 0) return checked;
+    return linear_call(name, true, [&](const OperatorDevice *device) {
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const Int8Rows rows(scratch, lanes, k);
+        const cudaError_t status = launch_quantise_int8(static_cast<const uint16_t *>(x), rows.values, rows.scales, lanes, k, st);
+        if (status != cudaSuccess) return status;
+        return launch_linear_int8_silu_pair(rows.values, rows.scales, static_cast<const int8_t *>(gate_w), static_cast<const float *>(gate_scale),
+                                            static_cast<const int8_t *>(up_w), static_cast<const float *>(up_scale), static_cast<uint16_t *>(y), lanes, n, k,
+                                            device->error_word(), st);
+    });
+}
+
+int32_t nerve_b200_op_route_experts(const void *logits, const void *bias, void *ids, void *weights, int32_t tokens, int32_t logits_f32, const nerve_b200_routing *routing,
+                                    void *stream) {
+    constexpr const char *name = "nerve_b200_op_route_experts";
+    const int32_t checked = guarded([&] {
+        require(routing != nullptr, "nerve_b200_op_route_experts: routing is NULL");
+        check_size(name, "tokens", tokens, 0, EXPERTS_MAX_ROUTES);
+        check_size(name, "experts", routing->experts, 1, ROUTING_MAX_EXPERTS);
+        check_size(name, "groups", routing->groups, 1, std::min(ROUTING_MAX_GROUPS, routing->experts));
+        check_size(name, "experts", routing->experts, 1, ROUTING_MAX_EXPERTS, routing->groups);
+        check_size(name, "chosen_groups", routing->chosen_groups, 1, routing->groups);
+        check_size(name, "group_scores", routing->group_scores, 1, routing->groups > 1 ? std::min(2, routing->experts / routing->groups) : 2);
+        check_size(name, "top_k", routing->top_k, 1, std::min(ROUTING_MAX_TOP_K, routing->chosen_groups * (routing->experts / routing->groups)));
+        if (tokens == 0) return;
+        check_pointer(name, "logits", logits, logits_f32 ? 4 : 2);
+        check_pointer(name, "bias", bias, 4, true);
+        check_pointer(name, "ids", ids, 4);
+        check_pointer(name, "weights", weights, 4);
+    });
+    if (checked != NERVE_B200_OK || tokens == 0) return checked;
+    const Routing how{routing->experts,      routing->top_k,      routing->sigmoid, routing->groups, routing->chosen_groups, routing->group_scores,
+                      routing->renormalise, routing->scale};
+    return cuda_status(launch_route_experts(logits, logits_f32 != 0, static_cast<const float *>(bias), static_cast<int *>(ids), static_cast<float *>(weights), tokens, how,
+                                            static_cast<cudaStream_t>(stream)),
+                       name);
+}
+
+uint64_t nerve_b200_op_experts_int8_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t hidden, int32_t inter) {
+    uint64_t bytes = 0;
+    guarded([&] {
+        check_experts_sizes("nerve_b200_op_experts_int8_scratch_bytes", tokens, top_k, experts, hidden, inter);
+        bytes = experts_int8_scratch_bytes(tokens, top_k, experts, hidden, inter);
+    });
+    return bytes;
+}
+
+int32_t nerve_b200_op_experts_int8(const void *x, const void *ids, const void *weights, const void *gate_up_w, const void *gate_up_scale, const void *down_w,
+                                   const void *down_scale, void *y, const void *residual, void *scratch, int32_t tokens, int32_t top_k, int32_t experts, int32_t hidden,
+                                   int32_t inter, void *stream) {
+    constexpr const char *name = "nerve_b200_op_experts_int8";
+    const int32_t checked = guarded([&] {
+        check_experts_sizes(name, tokens, top_k, experts, hidden, inter);
+        if (tokens == 0) return;
+        check_pointer(name, "x", x, 2);
+        check_pointer(name, "ids", ids, 4);
+        check_pointer(name, "weights", weights, 4);
+        check_pointer(name, "gate_up_w", gate_up_w, 16);
+        check_pointer(name, "gate_up_scale", gate_up_scale, 4);
+        check_pointer(name, "down_w", down_w, 16);
+        check_pointer(name, "down_scale", down_scale, 4);
+        check_pointer(name, "y", y, 2);
+        check_pointer(name, "residual", residual, 2, true);
+        check_pointer(name, "scratch", scratch, 16);
+    });
+    if (checked != NERVE_B200_OK || tokens == 0) return checked;
+    return linear_call(name, true, [&](const OperatorDevice *device) {
+        return launch_experts_int8(static_cast<const uint16_t *>(x), static_cast<const int *>(ids), static_cast<const float *>(weights),
+                                   static_cast<const int8_t *>(gate_up_w), static_cast<const float *>(gate_up_scale), static_cast<const int8_t *>(down_w),
+                                   static_cast<const float *>(down_scale), static_cast<uint16_t *>(y), static_cast<const uint16_t *>(residual), scratch, tokens, top_k,
+                                   experts, hidden, inter, device->error_word(), static_cast<cudaStream_t>(stream));
+    });
 }
 
 int32_t nerve_b200_op_greedy(const void *logits, void *records, void *scratch, int32_t lanes, int32_t vocab, void *stream) {

@@ -132,6 +132,30 @@ cudaError_t launch_moe_down_fp8(const uint8_t *xq, const float *xscale, const Mo
 cudaError_t launch_moe_reduce(const uint16_t *outputs, uint16_t *y, int lanes, int hidden_size, int top_k,
                               float routed_scale, cudaStream_t stream);
 
+// 8-bit integer linears: x is quantised per lane into q int8 [lanes][k] and scales f32 [lanes]; w int8 [n][k] with scales f32
+// [n].  k: a multiple of 16, up to INT8_MAX_COLUMNS (32-bit sums hold as many products); w and q on 16-byte boundaries.
+constexpr int INT8_MAX_COLUMNS = 131072;
+cudaError_t launch_quantise_int8(const uint16_t *x, int8_t *q, float *scales, int lanes, int k, cudaStream_t stream);
+cudaError_t launch_linear_int8(const int8_t *q, const float *lane_scales, const int8_t *w, const float *scales, void *y, const uint16_t *residual, int lanes, int n,
+                               int k, int to_f32, int *error_flag, cudaStream_t stream);
+cudaError_t launch_linear_int8_silu_pair(const int8_t *q, const float *lane_scales, const int8_t *gate, const float *gate_scales, const int8_t *up,
+                                         const float *up_scales, uint16_t *y, int lanes, int n, int k, int *error_flag, cudaStream_t stream);
+// Sparse experts in 8-bit integers: ids, weights [tokens][top_k]; gate_up int8 [experts][2 inter][hidden] (gate's rows first),
+// down int8 [experts][hidden][inter], scales f32 per row of both.  hidden and inter: multiples of 16; up to EXPERTS_INT8_MAX
+// experts.
+constexpr int EXPERTS_INT8_MAX = 1024;
+size_t experts_int8_scratch_bytes(int tokens, int top_k, int experts, int hidden, int inter);
+cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *weights, const int8_t *gate_up, const float *gate_up_scales, const int8_t *down,
+                                const float *down_scales, uint16_t *y, const uint16_t *residual, void *scratch, int tokens, int top_k, int experts, int hidden, int inter,
+                                int *error_flag, cudaStream_t stream);
+// The choice of experts (kernels_routing.cu holds the definition).
+struct Routing {
+    int experts, top_k, sigmoid, groups, chosen_groups, group_scores, renormalise;
+    float scale;
+};
+constexpr int ROUTING_MAX_EXPERTS = 1024, ROUTING_MAX_TOP_K = 64, ROUTING_MAX_GROUPS = 32;
+cudaError_t launch_route_experts(const void *logits, bool logits_f32, const float *bias, int *ids, float *weights, int tokens, const Routing &routing, cudaStream_t stream);
+
 // Rotary embedding of q and k (with a per-head RMSNorm in front where norm weights are given) and the append of K and V
 // at every lane's position, in one launch.
 struct RopeForm {

@@ -44,6 +44,16 @@ class _SamplerConfig(ctypes.Structure):
                 ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32)]
 
 
+class Routing(ctypes.Structure):
+    """How nerve_b200_op_route_experts chooses experts (see the header)."""
+
+    _fields_ = [(name, ctypes.c_int32) for name in ("experts", "top_k", "sigmoid", "groups", "chosen_groups", "group_scores", "renormalise")] + [
+        ("scale", ctypes.c_float)]
+
+    def __init__(self, experts, top_k, sigmoid=False, groups=1, chosen_groups=1, group_scores=1, renormalise=True, scale=1.0):
+        super().__init__(experts, top_k, sigmoid, groups, chosen_groups, group_scores, renormalise, scale)
+
+
 _REPORT_U64 = (
     "prefill_ns", "decode_ns", "prefill_tokens", "generated_tokens", "activation_count", "batch_count",
     "max_batch_width", "cycle_count", "proposed_draft_token_count", "accepted_draft_token_count",
@@ -81,6 +91,8 @@ EXPORTED_SYMBOLS = (
     "nerve_b200_engine_set_cycle_logging", "nerve_b200_engine_cycle_log", "nerve_b200_debug_target_logits",
     "nerve_b200_op_linear_int4", "nerve_b200_op_linear_int4_silu_pair",
     "nerve_b200_op_linear_bf16", "nerve_b200_op_rms_norm", "nerve_b200_op_linear_fp8",
+    "nerve_b200_op_linear_int8", "nerve_b200_op_linear_int8_scratch_bytes", "nerve_b200_op_linear_int8_silu_pair",
+    "nerve_b200_op_route_experts", "nerve_b200_op_experts_int8", "nerve_b200_op_experts_int8_scratch_bytes",
     "nerve_b200_op_greedy", "nerve_b200_op_greedy_scratch_bytes", "nerve_b200_op_greedy_static", "nerve_b200_op_sample_top_k_top_p", "nerve_b200_op_sample_scratch_bytes", "nerve_b200_verify_prefix",
     "nerve_b200_stream_control_bytes", "nerve_b200_state_page_table_bytes",
     "nerve_b200_scheduler_create", "nerve_b200_scheduler_destroy", "nerve_b200_scheduler_add_stream",
@@ -109,6 +121,8 @@ def library() -> ctypes.CDLL:
                 getattr(lib, name).restype = ctypes.c_int32
         lib.nerve_b200_op_greedy_scratch_bytes.restype = ctypes.c_uint64
         lib.nerve_b200_op_sample_scratch_bytes.restype = ctypes.c_uint64
+        lib.nerve_b200_op_linear_int8_scratch_bytes.restype = ctypes.c_uint64
+        lib.nerve_b200_op_experts_int8_scratch_bytes.restype = ctypes.c_uint64
         _library = lib
     return _library
 
