@@ -214,15 +214,6 @@ void check_experts_sizes(const char *name, int32_t tokens, int32_t top_k, int32_
     check_size(name, "hidden", hidden, 16, INT8_MAX_COLUMNS, 16);
     check_size(name, "inter", inter, 16, INT8_MAX_COLUMNS, 16);
 }
-// The activations of an 8-bit integer linear in the caller's scratch buffer: whole numbers, then one scale per lane.
-size_t int8_row_bytes(int32_t lanes, int32_t k) { return (static_cast<size_t>(lanes) * k + 255) / 256 * 256; }
-struct Int8Rows {
-    int8_t *values;
-    float *scales;
-    Int8Rows(void *scratch, int32_t lanes, int32_t k)
-        : values(static_cast<int8_t *>(scratch)), scales(reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + int8_row_bytes(lanes, k))) {}
-};
-
 // One reference less; the last one takes the model and the operator-level linears' unused memory with it.
 void release(nerve_b200_package *package) {
     if (--package->references != 0) return;
@@ -684,7 +675,7 @@ uint64_t nerve_b200_op_linear_int8_scratch_bytes(int32_t lanes, int32_t k) {
     uint64_t bytes = 0;
     guarded([&] {
         check_int8_sizes("nerve_b200_op_linear_int8_scratch_bytes", lanes, 1, k);
-        bytes = int8_row_bytes(lanes, k) + static_cast<uint64_t>(lanes) * sizeof(float);
+        bytes = linear_int8_scratch_bytes(lanes, k);
     });
     return bytes;
 }
@@ -704,12 +695,8 @@ int32_t nerve_b200_op_linear_int8(const void *x, const void *w, const void *wsca
     });
     if (checked != NERVE_B200_OK || lanes == 0) return checked;
     return linear_call(name, true, [&](const OperatorDevice *device) {
-        const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const Int8Rows rows(scratch, lanes, k);
-        const cudaError_t status = launch_quantise_int8(static_cast<const uint16_t *>(x), rows.values, rows.scales, lanes, k, st);
-        if (status != cudaSuccess) return status;
-        return launch_linear_int8(rows.values, rows.scales, static_cast<const int8_t *>(w), static_cast<const float *>(wscale), y, static_cast<const uint16_t *>(residual),
-                                  lanes, n, k, to_f32, device->error_word(), st);
+        return launch_linear_int8(static_cast<const uint16_t *>(x), static_cast<const int8_t *>(w), static_cast<const float *>(wscale), y,
+                                  static_cast<const uint16_t *>(residual), scratch, lanes, n, k, to_f32, device->error_word(), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -729,13 +716,9 @@ int32_t nerve_b200_op_linear_int8_silu_pair(const void *x, const void *gate_w, c
     });
     if (checked != NERVE_B200_OK || lanes == 0) return checked;
     return linear_call(name, true, [&](const OperatorDevice *device) {
-        const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const Int8Rows rows(scratch, lanes, k);
-        const cudaError_t status = launch_quantise_int8(static_cast<const uint16_t *>(x), rows.values, rows.scales, lanes, k, st);
-        if (status != cudaSuccess) return status;
-        return launch_linear_int8_silu_pair(rows.values, rows.scales, static_cast<const int8_t *>(gate_w), static_cast<const float *>(gate_scale),
-                                            static_cast<const int8_t *>(up_w), static_cast<const float *>(up_scale), static_cast<uint16_t *>(y), lanes, n, k,
-                                            device->error_word(), st);
+        return launch_linear_int8_silu_pair(static_cast<const uint16_t *>(x), static_cast<const int8_t *>(gate_w), static_cast<const float *>(gate_scale),
+                                            static_cast<const int8_t *>(up_w), static_cast<const float *>(up_scale), static_cast<uint16_t *>(y), scratch, lanes, n, k,
+                                            device->error_word(), static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -132,14 +132,14 @@ cudaError_t launch_moe_down_fp8(const uint8_t *xq, const float *xscale, const Mo
 cudaError_t launch_moe_reduce(const uint16_t *outputs, uint16_t *y, int lanes, int hidden_size, int top_k,
                               float routed_scale, cudaStream_t stream);
 
-// 8-bit integer linears: x is quantised per lane into q int8 [lanes][k] and scales f32 [lanes]; w int8 [n][k] with scales f32
-// [n].  k: a multiple of 16, up to INT8_MAX_COLUMNS (32-bit sums hold as many products); w and q on 16-byte boundaries.
+// 8-bit integer linears: x bf16 is quantised per lane within the call; w int8 [n][k] with scales f32 [n].  k: a multiple of 16,
+// up to INT8_MAX_COLUMNS (32-bit sums hold as many products); w and scratch on 16-byte boundaries.
 constexpr int INT8_MAX_COLUMNS = 131072;
-cudaError_t launch_quantise_int8(const uint16_t *x, int8_t *q, float *scales, int lanes, int k, cudaStream_t stream);
-cudaError_t launch_linear_int8(const int8_t *q, const float *lane_scales, const int8_t *w, const float *scales, void *y, const uint16_t *residual, int lanes, int n,
-                               int k, int to_f32, int *error_flag, cudaStream_t stream);
-cudaError_t launch_linear_int8_silu_pair(const int8_t *q, const float *lane_scales, const int8_t *gate, const float *gate_scales, const int8_t *up,
-                                         const float *up_scales, uint16_t *y, int lanes, int n, int k, int *error_flag, cudaStream_t stream);
+size_t linear_int8_scratch_bytes(int lanes, int k);
+cudaError_t launch_linear_int8(const uint16_t *x, const int8_t *w, const float *scales, void *y, const uint16_t *residual, void *scratch, int lanes, int n, int k, int to_f32,
+                               int *error_flag, cudaStream_t stream);
+cudaError_t launch_linear_int8_silu_pair(const uint16_t *x, const int8_t *gate, const float *gate_scales, const int8_t *up, const float *up_scales, uint16_t *y, void *scratch,
+                                         int lanes, int n, int k, int *error_flag, cudaStream_t stream);
 // Sparse experts in 8-bit integers: ids, weights [tokens][top_k]; gate_up int8 [experts][2 inter][hidden] (gate's rows first),
 // down int8 [experts][hidden][inter], scales f32 per row of both.  hidden and inter: multiples of 16; up to EXPERTS_INT8_MAX
 // experts.

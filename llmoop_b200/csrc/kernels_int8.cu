@@ -34,7 +34,7 @@ constexpr int BLOCK_K = 128;  // columns per stage: one swizzled row of 128 byte
 constexpr int ROWS = 128;     // the MMA's M
 constexpr int MAX_LANES = 256, MAX_STAGES = 32;
 constexpr int OUTPUT_WARPS = 8, THREADS = 128 + 32 * OUTPUT_WARPS;
-constexpr size_t SMEM_LIMIT = 226 * 1024, CONTROL_BYTES = 1024;
+constexpr size_t SMEM_LIMIT = 226 * 1024, SMEM_HALF = 112 * 1024, CONTROL_BYTES = 1024;
 constexpr unsigned int SPIN_LIMIT = 1u << 22;  // tries of 1.5 us
 
 enum Mode { LINEAR, PAIR, EXPERTS_PAIR, EXPERTS_DOWN };
@@ -85,113 +85,165 @@ __device__ __forceinline__ void copy_tile(uint32_t target, const CUtensorMap *ma
                  : "memory");
 }
 
+// Into L2, which later writes to the tile reach: safe ahead of the wait for the kernel in front, whatever that writes.
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap *map, int column, int row) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(column), "r"(row) : "memory");
+}
+
 // NaN stays NaN.
 __device__ __forceinline__ uint16_t to_bf16(float value) { return __bfloat16_as_ushort(__float2bfloat16_rn(value)); }
 
 // ---- quantisation of activation rows
 
-// Largest magnitude of a block's values; NaN (as an infinity or a NaN among them makes it) spreads.
-__device__ __forceinline__ float block_amax(float mine, float *warps) {
-    // magnitudes compare as their bits do, and those of NaN and infinity are the largest
-    const uint32_t best = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = __uint_as_float(best);
-    __syncthreads();
-    uint32_t all = 0;
-    for (int warp = 0; warp < static_cast<int>(blockDim.x >> 5); warp++) all = max(all, __float_as_uint(warps[warp]));
-    return __uint_as_float(all);
-}
+// Sixteen values of a row, as they are read.
+struct HeldBf16 {
+    uint4 words[2];
+    __device__ __forceinline__ void load(const uint16_t *row, int at, bool wide) {
+        if (wide) {
+            words[0] = reinterpret_cast<const uint4 *>(row + at)[0];
+            words[1] = reinterpret_cast<const uint4 *>(row + at)[1];
+        } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = row[at + 2 * i] | (static_cast<uint32_t>(row[at + 2 * i + 1]) << 16);
+            words[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            words[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+    }
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4 &four = words[i >> 2];
+        return (i & 3) == 0 ? four.x : (i & 3) == 1 ? four.y : (i & 3) == 2 ? four.z : four.w;
+    }
+    // the largest magnitude, as the bits of an f32
+    __device__ __forceinline__ uint32_t amax() const {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) most = __vmaxu2(most, word(i) & 0x7fff7fffu);
+        return max(most & 0xffff0000u, most << 16);
+    }
+    __device__ __forceinline__ float value(int i) const { return i & 1 ? bf16_hi(word(i >> 1)) : bf16_lo(word(i >> 1)); }
+};
+struct HeldF32 {
+    float4 words[4];
+    __device__ __forceinline__ void load(const float *row, int at, bool) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) words[i] = reinterpret_cast<const float4 *>(row + at)[i];
+    }
+    __device__ __forceinline__ float value(int i) const {
+        const float4 &four = words[i >> 2];
+        return (i & 3) == 0 ? four.x : (i & 3) == 1 ? four.y : (i & 3) == 2 ? four.z : four.w;
+    }
+    __device__ __forceinline__ uint32_t amax() const {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(fabsf(value(i))));
+        return most;
+    }
+};
 
 struct RowScale {
-    float pre, multiplier, scale;
+    float multiplier, scale;
+    bool tiny;
 };
-// q = rint((x pre) multiplier).  pre lifts rows of tiny values to where 127 / amax is finite.
-__device__ __forceinline__ RowScale row_scale(float amax) {
-    RowScale row;
+// q = rint(x multiplier), or of x 2^90 for rows of tiny values, whose 127 / amax is not finite.  The multiplier is rounded up:
+// a bf16 quotient 127 x / amax is 2^-16 of itself away from the nearest tie (both significands are whole numbers below 256)
+// unless it is one; ties are x = amax / 2, whose 63.5 a multiplier too large sends to the even 64 as an exact one does, and
+// those of an amax of 254 powers of two, whose multiplier is exact.
+__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {  // magnitudes compare as their bits do; infinities and NaN are the largest
+    const float amax = __uint_as_float(amax_bits);
     const bool finite = amax <= 3.4028234e38f;
-    row.pre = amax < 0x1p-90f ? 0x1p+90f : 1.0f;
-    row.multiplier = finite && amax > 0.0f ? 127.0f / (amax * row.pre) : 0.0f;
+    RowScale row;
+    row.tiny = amax < 0x1p-90f;
+    row.multiplier = finite && amax > 0.0f ? __fdiv_ru(127.0f, row.tiny ? amax * 0x1p+90f : amax) : 0.0f;
     row.scale = finite ? amax / 127.0f : __uint_as_float(0x7fffffffu);  // a row with an infinity or a NaN is NaN throughout
     return row;
 }
-// The whole number as the low byte.  x multiplier carries a relative error below 2^-22, which matters at ties alone: a bf16
-// quotient 127 x / amax is either a tie, with at most eight significant bits, or 2^-16 of itself away from one (both
-// significands are whole numbers below 256), so that rounding the product to nineteen bits first puts ties, and nothing
-// else, back onto themselves.  f32 inputs go without.
-template <bool TIES>
-__device__ __forceinline__ uint32_t quantise(float x, const RowScale &row) {
-    float t = (x * row.pre) * row.multiplier;
-    if (TIES) t = __uint_as_float((__float_as_uint(t) + 0x10u) & ~0x1Fu);
-    return __float_as_uint(t + 12582912.0f);  // 1.5 * 2^23: rounds to even, leaves two's complement in the low bits
-}
-__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-
-// Eight values of a row from `at` on.
-struct Eight {
-    float v[8];
-};
-__device__ __forceinline__ Eight load_eight(const uint16_t *row, int at, bool wide) {
-    Eight out;
-    if (wide) {
-        const uint4 words = *reinterpret_cast<const uint4 *>(row + at);
-        const uint32_t w[4] = {words.x, words.y, words.z, words.w};
+// Sixteen whole numbers as bytes.
+template <typename Held>
+__device__ __forceinline__ uint4 quantise(const Held &held, const RowScale &row) {
+    uint32_t out[4];
+#pragma unroll
+    for (int word = 0; word < 4; word++) {
+        uint32_t b[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            out.v[2 * i] = bf16_lo(w[i]);
-            out.v[2 * i + 1] = bf16_hi(w[i]);
+            float x = held.value(4 * word + i);
+            if (row.tiny) x *= 0x1p+90f;
+            b[i] = __float_as_uint(__fmaf_rn(x, row.multiplier, 12582912.0f));  // 1.5 * 2^23: one rounding, to even; two's complement in the low bits
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) out.v[i] = bf16_bits_to_f32(row[at + i]);
+        out[word] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
-    return out;
-}
-__device__ __forceinline__ Eight load_eight(const float *row, int at, bool) {
-    Eight out;
-    const float4 low = *reinterpret_cast<const float4 *>(row + at), high = *reinterpret_cast<const float4 *>(row + at + 4);
-    out.v[0] = low.x, out.v[1] = low.y, out.v[2] = low.z, out.v[3] = low.w;
-    out.v[4] = high.x, out.v[5] = high.y, out.v[6] = high.z, out.v[7] = high.w;
-    return out;
+    return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// One CTA per row of x.  Without places the row goes to its own number; with them (the experts' inputs) once to the place of
-// each of its top_k routes, where it has one.  The second reading of the row comes from the caches.
+// One CTA per row of x, which its threads hold in registers, HELD times sixteen values each; what is wider is read again,
+// from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once to the place of each
+// of its top_k routes, where it has one.  Bound by DRAM for large batches, by the chain of loads, barrier and stores for small
+// ones.
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.
-template <typename T>
-__global__ void quantise_rows_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__restrict__ scales, const int *__restrict__ places,
-                                     const int *__restrict__ row_count, int top_k, int k, int wide) {
-    __shared__ float warps[32];
+template <typename T, typename Held, int HELD>
+__global__ void __launch_bounds__(512) quantise_rows_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__restrict__ scales, const int *__restrict__ places,
+                                                            const int *__restrict__ row_count, int top_k, int k, int wide) {
+    __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
     if (row_count != nullptr && static_cast<int>(blockIdx.x) >= *row_count) return;
     const T *row = x + static_cast<size_t>(blockIdx.x) * k;
-    float amax = 0.0f;
-    for (int at = threadIdx.x * 8; at < k; at += blockDim.x * 8) {
-        const Eight eight = load_eight(row, at, wide);
+    const int step = blockDim.x * 16;
+    Held held[HELD];
 #pragma unroll
-        for (int i = 0; i < 8; i++) amax = __uint_as_float(max(__float_as_uint(amax), __float_as_uint(fabsf(eight.v[i]))));
+    for (int i = 0; i < HELD; i++)
+        if (static_cast<int>(threadIdx.x) * 16 + i * step < k) held[i].load(row, threadIdx.x * 16 + i * step, wide);
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+        if (static_cast<int>(threadIdx.x) * 16 + i * step < k) amax = max(amax, held[i].amax());
+    for (int at = threadIdx.x * 16 + HELD * step; at < k; at += step) {
+        Held more;
+        more.load(row, at, wide);
+        amax = max(amax, more.amax());
     }
-    const RowScale scale = row_scale(block_amax(amax, warps));
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    for (int warp = 0; warp < static_cast<int>(blockDim.x >> 5); warp++) amax = max(amax, warps[warp]);
+    const RowScale scale = row_scale(amax);
     const int copies = places != nullptr ? top_k : 1;
-    for (int at = threadIdx.x * 8; at < k; at += blockDim.x * 8) {
-        const Eight eight = load_eight(row, at, wide);
-        uint32_t b[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) b[i] = quantise<sizeof(T) == 2>(eight.v[i], scale);
-        const uint2 packed = make_uint2(pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7]));
+    const int *own_places = places + (places != nullptr ? static_cast<size_t>(blockIdx.x) * top_k : 0);
+    auto store = [&](int at, const Held &values) {
+        const uint4 packed = quantise(values, scale);
         for (int copy = 0; copy < copies; copy++) {
-            const int place = places != nullptr ? places[static_cast<size_t>(blockIdx.x) * top_k + copy] : static_cast<int>(blockIdx.x);
-            if (place >= 0) *reinterpret_cast<uint2 *>(q + static_cast<size_t>(place) * k + at) = packed;
+            const int place = places != nullptr ? own_places[copy] : static_cast<int>(blockIdx.x);
+            if (place >= 0) *reinterpret_cast<uint4 *>(q + static_cast<size_t>(place) * k + at) = packed;
         }
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+        if (static_cast<int>(threadIdx.x) * 16 + i * step < k) store(threadIdx.x * 16 + i * step, held[i]);
+    for (int at = threadIdx.x * 16 + HELD * step; at < k; at += step) {
+        Held more;
+        more.load(row, at, wide);
+        store(at, more);
     }
-    if (static_cast<int>(threadIdx.x) < copies) {
-        const int place = places != nullptr ? places[static_cast<size_t>(blockIdx.x) * top_k + threadIdx.x] : static_cast<int>(blockIdx.x);
+    for (int copy = threadIdx.x; copy < copies; copy += blockDim.x) {
+        const int place = places != nullptr ? own_places[copy] : static_cast<int>(blockIdx.x);
         if (place >= 0) scales[place] = scale.scale;
     }
 }
 
-int quantise_threads(int k) { return std::min(512, std::max(64, (k / 8 + 31) / 32 * 32)); }
+// The rows are cut so that a thread holds its part of up to 32768 columns (bf16) or 16384 (f32), with as many threads as
+// sixteen columns each ask for up to 256, then more columns each.
+template <typename T, typename Held, int MOST>
+cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int rows, int top_k, int k, cudaStream_t stream) {
+    const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    auto with = [&](auto kernel, int held) {
+        const int threads = std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
+        return launch_dependent(kernel, dim3(rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, top_k, k, wide);
+    };
+    if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1>, 1);
+    if (parts <= 1024 || MOST == 2) return with(quantise_rows_kernel<T, Held, 2>, 2);
+    return with(quantise_rows_kernel<T, Held, MOST>, MOST);
+}
 
 // ---- the product
 
@@ -231,20 +283,22 @@ __device__ __forceinline__ Tile tile_at(const Int8Args &a, int index) {
     }
     return tile;
 }
-// The weight copies of one stage: box `which` of `boxes`.
-template <Mode MODE>
-__device__ __forceinline__ void copy_weights(const Int8Args &a, const Tile &tile, int which, int column, uint32_t target, uint32_t barrier) {
+// Box `which` of a stage's weights: visit(map, row of the matrix, row of the stage).
+template <Mode MODE, typename Visit>
+__device__ __forceinline__ void visit_weights(const Int8Args &a, const Tile &tile, int which, Visit visit) {
     if (MODE == LINEAR || MODE == EXPERTS_DOWN) {
-        copy_tile(target, &a.weights, column, tile.expert * a.n + tile.row0, barrier);
+        visit(&a.weights, tile.expert * a.n + tile.row0, 0);
     } else {  // sixteen rows each, by turns of gate and of up
         const bool up = which & 1;
         const int row = tile.row0 + (which >> 1) * 16;
-        if (MODE == PAIR) copy_tile(target + which * 16 * BLOCK_K, up ? &a.up : &a.weights, column, row, barrier);
-        else copy_tile(target + which * 16 * BLOCK_K, &a.weights, column, tile.expert * 2 * a.n + (up ? a.n : 0) + row, barrier);
+        if (MODE == PAIR) visit(up ? &a.up : &a.weights, row, which * 16);
+        else visit(&a.weights, tile.expert * 2 * a.n + (up ? a.n : 0) + row, which * 16);
     }
 }
 
-__device__ __forceinline__ float silu_product(float gate, float up) { return __fdividef(gate, 1.0f + __expf(-gate)) * up; }
+// The outputs' arithmetic, the same to the bit in every kernel (no contraction).
+__device__ __forceinline__ float scaled(int sum, float factor, float lane_scale) { return __fmul_rn(__fmul_rn(static_cast<float>(sum), factor), lane_scale); }
+__device__ __forceinline__ float silu_product(float gate, float up) { return __fmul_rn(__fdividef(gate, __fadd_rn(1.0f, __expf(-gate))), up); }
 
 template <Mode MODE>
 __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
@@ -284,18 +338,12 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
 
     if (warp == 0) {  // ---- copies
         const int weight_boxes = TWO ? a.tile_rows / 16 : 1;
-        int stage = 0, issued = 0, ahead = 0;
+        int stage = 0, issued = 0;
         uint32_t parity = 1;  // the first round waits for no release
-        if (!GROUPED && static_cast<int>(blockIdx.x) < a.row_tiles * a.lane_tiles) {
-            // the weights of the first stages do not wait for the kernel in front, which is the quantisation
+        if (!GROUPED) {
             const Tile tile = tile_at<MODE>(a, blockIdx.x);
-            const uint32_t bytes = a_bytes + static_cast<uint32_t>((tile.count + a.box_lanes - 1) / a.box_lanes * a.box_lanes) * BLOCK_K;
-            ahead = min(a.stages, blocks);
-            for (int block = 0; block < ahead; block++) {
-                if (elect_one()) expect_bytes(full + block * 8, bytes);
-                __syncwarp();
-                if (lane < weight_boxes) copy_weights<MODE>(a, tile, lane, block * BLOCK_K, base + static_cast<uint32_t>(block) * stage_bytes, full + block * 8);
-            }
+            for (int block = 0; block < min(a.stages, blocks); block++)
+                if (lane < weight_boxes) visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int) { prefetch_tile(map, block * BLOCK_K, row); });
         }
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
@@ -314,11 +362,10 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                     alive = false;
                     break;
                 }
-                if (issued >= ahead) {
-                    if (elect_one()) expect_bytes(barrier, bytes);
-                    __syncwarp();
-                    if (lane < weight_boxes) copy_weights<MODE>(a, tile, lane, block * BLOCK_K, target, barrier);
-                }
+                if (elect_one()) expect_bytes(barrier, bytes);
+                __syncwarp();
+                if (lane < weight_boxes)
+                    visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int at) { copy_tile(target + at * BLOCK_K, map, block * BLOCK_K, row, barrier); });
                 if (lane < lane_boxes)
                     copy_tile(target + a_bytes + static_cast<uint32_t>(lane * a.box_lanes) * BLOCK_K, &a.activations, block * BLOCK_K, tile.lane0 + lane * a.box_lanes, barrier);
                 __syncwarp();
@@ -411,15 +458,15 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                         lane_scale = a.lane_scales[first_lane + lane];
                         if (MODE == EXPERTS_DOWN) {
                             pair = a.pair_of[first_lane + lane];
-                            lane_scale *= a.weights_of[pair];
+                            lane_scale = __fmul_rn(lane_scale, a.weights_of[pair]);
                         }
                     }
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (TWO) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {  // the warp's lower half finishes lane i, its upper half lane i + 1
-                            const float low = static_cast<float>(static_cast<int>(d[i])) * factor * __shfl_sync(0xffffffffu, lane_scale, i);
-                            const float high = static_cast<float>(static_cast<int>(d[i + 1])) * factor * __shfl_sync(0xffffffffu, lane_scale, i + 1);
+                            const float low = scaled(static_cast<int>(d[i]), factor, __shfl_sync(0xffffffffu, lane_scale, i));
+                            const float high = scaled(static_cast<int>(d[i + 1]), factor, __shfl_sync(0xffffffffu, lane_scale, i + 1));
                             const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? high : low, 16);
                             const float product = lane < 16 ? silu_product(low, other) : silu_product(other, high);
                             const int at = i + (lane >> 4);
@@ -437,14 +484,14 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                                 if (in_range && i < count) residual[i] = bf16_bits_to_f32(a.residual[static_cast<size_t>(first_lane + i) * a.n + channel]);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            float value = static_cast<float>(static_cast<int>(d[i])) * factor * __shfl_sync(0xffffffffu, lane_scale, i);
+                            float value = scaled(static_cast<int>(d[i]), factor, __shfl_sync(0xffffffffu, lane_scale, i));
                             const int to = MODE == EXPERTS_DOWN ? __shfl_sync(0xffffffffu, pair, i) : first_lane + i;
                             if (!in_range || i >= count) continue;
                             const size_t out = static_cast<size_t>(to) * a.n + channel;
                             if (MODE == EXPERTS_DOWN) {
                                 reinterpret_cast<float *>(a.y)[out] = value;
                             } else {
-                                if (a.residual != nullptr) value += residual[i];
+                                if (a.residual != nullptr) value = __fadd_rn(value, residual[i]);
                                 if (a.to_f32) reinterpret_cast<float *>(a.y)[out] = value;
                                 else reinterpret_cast<uint16_t *>(a.y)[out] = to_bf16(value);
                             }
@@ -459,6 +506,409 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+
+// ---- few lanes: the weights stream by, the activations stay
+
+// Up to eight lanes: one launch that is bound by the weights' bytes, or for small matrices by the chain of its steps.  Every
+// CTA quantises all lanes itself while its first weights are on their way: eight rows of 128 columns make one swizzled
+// atom of 1 KB, the K-th 128 columns the K-th atom.  A stage of the ring is the MMA's 128 rows; a tile with fewer
+// weight rows puts `groups` successive blocks of 128 columns on top of one another there, 128 / groups rows to each, and
+// multiplies them by as many successive atoms side by side (N = 8 groups): of the products only those of a block with its
+// own atom count, the outputs add them up.  So a tile of 28 rows costs the tensor pipe, which reads all 128 rows at 128
+// bytes per cycle whatever N, a fourth of what one block after the other would.
+// Warps: 0 copies weights, 1 issues MMAs, 4-7 write outputs, 4-11 (the experts' down product: 8-11) quantise.
+constexpr int FEW = 8, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
+constexpr uint32_t ATOM = 1024, STREAM_STAGE = ROWS * BLOCK_K;
+constexpr int FEW_ROUTES = 128;          // of the experts' form
+constexpr int STREAM_SMALL_SHARE = 16;   // stages
+
+struct StreamArgs {
+    CUtensorMap weights, up;  // boxes of 128 columns x rows weight rows
+    const void *x;            // bf16 rows; the down product: f32
+    const float *scales, *up_scales;
+    void *y;
+    const uint16_t *residual;
+    int lanes, n, k, to_f32, wide;
+    int *error_flag;
+    int rows, groups, row_tiles, stages;  // output channels of a tile
+    // experts
+    const int *ids;
+    const float *weights_of;
+    int top_k, experts;
+};
+
+struct StreamControl {
+    uint64_t full[STREAM_MAX_STAGES], empty[STREAM_MAX_STAGES], acc_full[2], acc_empty[2], b_full[2], b_empty[2];
+    uint32_t tmem;
+    int used;                                // experts with a route
+    uint32_t amax[2][FEW];
+    float lane_scales[2][FEW];
+    int sums[FEW][ROWS];                     // of a finished tile, per lane and row of the accumulator
+};
+// Routes by expert, for tables of up to FEW_ROUTES routes of FEW tokens.
+struct StreamRoutes {
+    int slot[EXPERTS_INT8_MAX];              // first route of an expert, then its number among the used ones
+    int expert[FEW_ROUTES];
+    int lead[FEW_ROUTES][FEW];               // a token's first route to the used expert; past all routes: none
+    int ids[FEW_ROUTES];
+    int before[FEW_ROUTES / 32];
+};
+constexpr int NO_ROUTE = 1 << 30;
+
+// All threads.  The used experts are numbered in the order of their first routes, the same in every CTA.
+__device__ __forceinline__ void find_routes(const StreamArgs &a, StreamControl &control, StreamRoutes &routes) {
+    const int thread = threadIdx.x, count = a.lanes * a.top_k;
+    for (int e = thread; e < a.experts; e += STREAM_THREADS) routes.slot[e] = NO_ROUTE;
+    for (int i = thread; i < FEW_ROUTES * FEW; i += STREAM_THREADS) (&routes.lead[0][0])[i] = NO_ROUTE;
+    __syncthreads();
+    int expert = -1;
+    if (thread < count) {
+        expert = a.ids[thread];
+        if (expert < 0 || expert >= a.experts) expert = -1;
+        routes.ids[thread] = expert;
+        if (expert >= 0) atomicMin(&routes.slot[expert], thread);
+    }
+    __syncthreads();
+    const bool first = expert >= 0 && routes.slot[expert] == thread;
+    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+    if (thread < FEW_ROUTES && (thread & 31) == 0) routes.before[thread >> 5] = __popc(firsts);
+    __syncthreads();
+    int number = __popc(firsts & ((1u << (thread & 31)) - 1u)), used = 0;
+    for (int warp = 0; warp < FEW_ROUTES / 32; warp++) {
+        if (warp < thread >> 5) number += routes.before[warp];
+        used += routes.before[warp];
+    }
+    if (first) {
+        routes.slot[expert] = number;
+        routes.expert[number] = expert;
+    }
+    if (thread == 0) control.used = used;
+    __syncthreads();
+    if (expert >= 0) atomicMin(&routes.lead[routes.slot[expert]][thread / a.top_k], thread);
+    __syncthreads();
+}
+
+// Quantises rows into atoms at `atoms`, by THREADS_ threads of which this is number `thread`.  row_of(lane): where lane's
+// row starts, NULL for a lane without one.  sync(): among those threads.  The first two parts of a thread stay in registers.
+template <int COUNT, typename T, typename Held, typename RowOf, typename Sync>
+__device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms, uint32_t *amax, float *scales, int thread, RowOf row_of, Sync sync) {
+    const int parts = a.k / 16, all = a.lanes * parts;
+    constexpr int KEPT = sizeof(T) == 2 ? 2 : 1;
+    if (thread < FEW) amax[thread] = 0;
+    sync();
+    Held kept[KEPT];
+    const bool even = parts % 32 == 0;  // a warp's thirty-two parts are of one row
+    for (int i = 0, part = thread; part < all; i++, part += COUNT) {
+        const int lane = part / parts;
+        const T *row = row_of(lane);
+        if (row == nullptr) continue;
+        Held values;
+        values.load(row, (part - lane * parts) * 16, a.wide);
+#pragma unroll
+        for (int j = 0; j < KEPT; j++)
+            if (i == j) kept[j] = values;
+        uint32_t most = values.amax();
+        if (even) {
+            most = __reduce_max_sync(0xffffffffu, most);
+            if ((thread & 31) == 0) atomicMax(&amax[lane], most);
+        } else {
+            atomicMax(&amax[lane], most);
+        }
+    }
+    sync();
+    if (thread < FEW) scales[thread] = row_scale(amax[thread]).scale;
+    RowScale scale = {};
+    int scaled = -1;
+    for (int i = 0, part = thread; part < all; i++, part += COUNT) {
+        const int lane = part / parts, at = part - lane * parts;
+        const T *row = row_of(lane);
+        if (row == nullptr) continue;
+        if (lane != scaled) {
+            scale = row_scale(amax[lane]);
+            scaled = lane;
+        }
+        Held values;
+        if (i >= KEPT) values.load(row, at * 16, a.wide);
+#pragma unroll
+        for (int j = 0; j < KEPT; j++)
+            if (i == j) values = kept[j];
+        *reinterpret_cast<uint4 *>(atoms + (at >> 3) * ATOM + lane * BLOCK_K + (((at & 7) ^ lane) << 4)) = quantise(values, scale);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Whether it holds for all 128 threads of named barrier ID: they go on together or not at all.
+template <int ID>
+__device__ __forceinline__ bool all_of(bool mine) {
+    uint32_t all;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 p, %1, 0;\n"
+        "bar.red.and.pred q, %2, 128, p;\n"
+        "selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(mine)), "n"(ID)
+        : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ uint32_t shared_address(const void *pointer) { return static_cast<uint32_t>(__cvta_generic_to_shared(pointer)); }
+__device__ __forceinline__ void arrive(uint32_t barrier) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory"); }
+__device__ __forceinline__ void init_barrier(uint32_t barrier, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory"); }
+
+constexpr size_t STREAM_CONTROL = (sizeof(StreamControl) + 1023) / 1024 * 1024, STREAM_ROUTES = (sizeof(StreamRoutes) + 1023) / 1024 * 1024;
+
+template <Mode MODE>
+__global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __grid_constant__ StreamArgs a) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr bool GROUPED = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN, TWO = MODE == PAIR || MODE == EXPERTS_PAIR, DOWN = MODE == EXPERTS_DOWN;
+    StreamControl &control = *reinterpret_cast<StreamControl *>(smem);
+    StreamRoutes &routes = *reinterpret_cast<StreamRoutes *>(smem + STREAM_CONTROL);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
+    const int blocks = (a.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + a.groups - 1) / a.groups, slot_rows = ROWS / a.groups;
+    const uint32_t atom_bytes = static_cast<uint32_t>(steps * a.groups) * ATOM;
+    uint8_t *const atoms = smem + STREAM_CONTROL + (GROUPED ? STREAM_ROUTES : 0);
+    const uint32_t ring = shared_address(atoms) + (DOWN ? 2 : 1) * atom_bytes;
+    const uint32_t full = shared_address(control.full), empty = shared_address(control.empty), acc_full = shared_address(control.acc_full),
+                   acc_empty = shared_address(control.acc_empty), b_full = shared_address(control.b_full), b_empty = shared_address(control.b_empty);
+    constexpr int QUANTISING = DOWN ? 4 : 8;  // warps
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STREAM_MAX_STAGES; s++) {
+            init_barrier(full + s * 8, 1);
+            init_barrier(empty + s * 8, 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            init_barrier(acc_full + s * 8, 1);
+            init_barrier(acc_empty + s * 8, 4);
+            init_barrier(b_full + s * 8, QUANTISING);
+            init_barrier(b_empty + s * 8, 2);  // the MMAs' commit and the outputs
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    constexpr uint32_t COLUMNS = 64, ACCUMULATOR = 32;
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tmem)), "r"(COLUMNS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // not before the tensor memory is this CTA's: one of the next kernel's that took it first would wait for this one
+    grid_launch_dependents();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(shared_address(&control.tmem)) : "memory");
+    tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
+    if (GROUPED) {
+        grid_dependency_wait();
+        find_routes(a, control, routes);
+    }
+    const int tiles = (GROUPED ? control.used : 1) * a.row_tiles;
+    const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.x / gridDim.x), last_tile = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.x + 1) / gridDim.x);
+
+    if (warp == 0) {  // ---- weights
+        const int copies = TWO ? 2 * a.groups : a.groups, group = TWO ? lane >> 1 : lane, up = TWO ? lane & 1 : 0;
+        const CUtensorMap *const map = MODE == PAIR && up ? &a.up : &a.weights;
+        if (!GROUPED) {
+            if (first_tile < last_tile && lane < copies)
+                for (int step = 0; step < min(steps, a.stages); step++) prefetch_tile(map, (step * a.groups + group) * BLOCK_K, first_tile * a.rows);
+            grid_dependency_wait();
+        }
+        const uint32_t bytes = static_cast<uint32_t>(copies * a.rows) * BLOCK_K;
+        int stage = 0, issued = 0;
+        uint32_t parity = 1;  // the first round waits for no release
+        bool alive = true;
+        for (int tile = first_tile; tile < last_tile && alive; tile++) {
+            const int row0 = tile % a.row_tiles * a.rows, expert = GROUPED ? routes.expert[tile / a.row_tiles] : 0;
+            for (int step = 0; step < steps; step++) {
+                if (!wait_barrier(empty + stage * 8, parity, a.error_flag)) {
+                    for (int s = 0; s < a.stages && s < issued; s++) {  // the copies in flight land before the CTA gives its memory up
+                        const int which = (issued - 1 - s) % a.stages;
+                        wait_barrier(full + which * 8, static_cast<uint32_t>(((issued - 1 - s) / a.stages) & 1), a.error_flag);
+                    }
+                    alive = false;
+                    break;
+                }
+                if (elect_one()) expect_bytes(full + stage * 8, bytes);
+                __syncwarp();
+                if (lane < copies) {
+                    const uint32_t target = ring + static_cast<uint32_t>(stage) * STREAM_STAGE + static_cast<uint32_t>(group * slot_rows + up * (slot_rows / 2)) * BLOCK_K;
+                    const int row = MODE == EXPERTS_PAIR ? (expert * 2 + up) * a.n + row0 : expert * a.n + row0;
+                    copy_tile(target, map, (step * a.groups + group) * BLOCK_K, row, full + stage * 8);
+                }
+                __syncwarp();
+                issued++;
+                if (++stage == a.stages) {
+                    stage = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {  // ---- MMAs
+        if (!GROUPED) grid_dependency_wait();
+        // instruction descriptor as in int8_gemm_kernel
+        const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(max(2, a.groups)) << 17) | (8u << 24));
+        const uint64_t a_first = swizzled_descriptor(ring), b_first = swizzled_descriptor(shared_address(atoms));
+        int stage = 0, round = 0, builds = 0, expert = -1;
+        uint32_t parity = 0;
+        bool alive = true;
+        for (int tile = first_tile; tile < last_tile && alive; tile++, round++) {
+            const int which = DOWN ? tile / a.row_tiles : 0;
+            if (which != expert) {
+                if (!wait_barrier(b_full + (builds & 1) * 8, static_cast<uint32_t>((builds >> 1) & 1), a.error_flag)) break;
+                expert = which;
+                builds++;
+            }
+            const bool last_of_build = DOWN && (tile + 1 == last_tile || (tile + 1) / a.row_tiles != which);
+            const uint64_t b_base = b_first + static_cast<uint64_t>((builds - 1) & 1) * (DOWN ? atom_bytes >> 4 : 0);
+            if (!wait_barrier(acc_empty + (round & 1) * 8, static_cast<uint32_t>((round / 2 + 1) & 1), a.error_flag)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t accumulator = tmem + (round & 1) * ACCUMULATOR;
+            for (int step = 0; step < steps; step++) {
+                if (!wait_barrier(full + stage * 8, parity, a.error_flag)) {
+                    alive = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+                    const uint64_t a_stage = a_first + static_cast<uint64_t>(stage) * (STREAM_STAGE >> 4), b_stage = b_base + static_cast<uint64_t>(step * a.groups) * (ATOM >> 4);
+#pragma unroll
+                    for (int part = 0; part < 4; part++) {  // K = 32 per instruction
+                        const uint32_t accumulate = (step > 0 || part > 0) ? 1u : 0u;
+                        asm volatile(
+                            "{\n"
+                            ".reg .pred p;\n"
+                            "setp.ne.b32 p, %4, 0;\n"
+                            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+                            "}\n" ::"r"(accumulator),
+                            "l"(a_stage + part * 2), "l"(b_stage + part * 2), "r"(instruction), "r"(accumulate)
+                            : "memory");
+                    }
+                    commit_to(empty + stage * 8);
+                    if (step == steps - 1) {
+                        commit_to(acc_full + (round & 1) * 8);
+                        if (last_of_build) commit_to(b_empty + ((builds - 1) & 1) * 8);
+                    }
+                }
+                __syncwarp();
+                if (++stage == a.stages) {
+                    stage = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        const int thread = threadIdx.x - 128;
+        if (!GROUPED) grid_dependency_wait();
+        if (!DOWN) {  // ---- quantisation, once
+            auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+            quantise_few<256, uint16_t, HeldBf16>(a, atoms, control.amax[0], control.lane_scales[0], thread,
+                                                  [&](int row) { return static_cast<const uint16_t *>(a.x) + static_cast<size_t>(row) * a.k; }, sync);
+            __syncwarp();
+            if (lane == 0) arrive(b_full);
+            sync();  // the outputs read the scales
+        } else if (warp >= 8) {  // ---- for every expert of this CTA's tiles, two at a time
+            auto sync = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
+            int builds = 0, expert = -1;
+            for (int tile = first_tile; tile < last_tile; tile++) {
+                const int which = tile / a.row_tiles;
+                if (which == expert) continue;
+                expert = which;
+                const int buffer = builds & 1;
+                if (!all_of<2>(wait_barrier(b_empty + buffer * 8, static_cast<uint32_t>((builds / 2 + 1) & 1), a.error_flag))) break;
+                quantise_few<128, float, HeldF32>(a, atoms + buffer * atom_bytes, control.amax[buffer], control.lane_scales[buffer], thread - 128,
+                                                  [&](int token) -> const float * {
+                                                      const int route = routes.lead[which][token];
+                                                      return route == NO_ROUTE ? nullptr : static_cast<const float *>(a.x) + static_cast<size_t>(route) * a.k;
+                                                  },
+                                                  sync);
+                __syncwarp();
+                if (lane == 0) arrive(b_full + buffer * 8);
+                builds++;
+            }
+        }
+        if (warp < 8) {  // ---- outputs
+            const int quarter = warp & 3, group = quarter * a.groups / 4;
+            int round = 0, builds = 0, expert = -1;
+            for (int tile = first_tile; tile < last_tile; tile++, round++) {
+                const int row0 = tile % a.row_tiles * a.rows, which = GROUPED ? tile / a.row_tiles : 0, outputs = min(a.rows, a.n - row0);
+                bool alive = true;
+                if (DOWN && which != expert) {
+                    expert = which;
+                    alive = wait_barrier(b_full + (builds & 1) * 8, static_cast<uint32_t>((builds >> 1) & 1), a.error_flag);
+                    builds++;
+                }
+                const float *scales = control.lane_scales[DOWN ? (builds - 1) & 1 : 0];
+                const size_t expert_row = GROUPED ? static_cast<size_t>(routes.expert[which]) * (TWO ? 2 : 1) * a.n : 0;
+                // what the first output of this thread needs, ahead of its sum
+                auto factors = [&](int at) {
+                    const int channel = row0 + at % a.rows;
+                    float2 factor = make_float2(0.0f, 0.0f);
+                    if (channel < a.n) {
+                        factor.x = a.scales[expert_row + channel];
+                        if (TWO) factor.y = MODE == PAIR ? a.up_scales[channel] : a.scales[expert_row + a.n + channel];
+                        else if (MODE == LINEAR && a.residual != nullptr) factor.y = bf16_bits_to_f32(a.residual[static_cast<size_t>(at / a.rows) * a.n + channel]);
+                    }
+                    return factor;
+                };
+                const int all = a.lanes * a.rows;
+                float2 factor = make_float2(0.0f, 0.0f);
+                if (thread < all) factor = factors(thread);
+                alive = alive && wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag);
+                if (!all_of<3>(alive)) break;  // and: the sums of the tile before have been read
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t d[8];
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7])
+                             : "r"(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (round & 1) * ACCUMULATOR + static_cast<uint32_t>(group * FEW))
+                             : "memory");
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < FEW; i++) control.sums[i][quarter * 32 + lane] = static_cast<int>(d[i]);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive(acc_empty + (round & 1) * 8);
+                asm volatile("bar.sync 3, 128;" ::: "memory");
+                for (int at = thread; at < all; at += 128) {
+                    const int row = at % a.rows, token = at / a.rows, channel = row0 + row;
+                    if (at != thread) factor = factors(at);
+                    if (row >= outputs) continue;
+                    int sum = 0, up_sum = 0;
+                    for (int g = 0; g < a.groups; g++) {
+                        sum += control.sums[token][g * slot_rows + row];
+                        if (TWO) up_sum += control.sums[token][g * slot_rows + slot_rows / 2 + row];
+                    }
+                    if (DOWN) {
+                        if (routes.lead[which][token] == NO_ROUTE) continue;
+                        const int id = routes.expert[which];
+                        for (int route = token * a.top_k; route < (token + 1) * a.top_k; route++)
+                            if (routes.ids[route] == id)
+                                reinterpret_cast<float *>(a.y)[static_cast<size_t>(route) * a.n + channel] = scaled(sum, factor.x, __fmul_rn(scales[token], a.weights_of[route]));
+                        continue;
+                    }
+                    float value = scaled(sum, factor.x, scales[token]);
+                    if (TWO) value = silu_product(value, scaled(up_sum, factor.y, scales[token]));
+                    if (MODE == EXPERTS_PAIR) {
+                        const int route = routes.lead[which][token];
+                        if (route != NO_ROUTE) reinterpret_cast<float *>(a.y)[static_cast<size_t>(route) * a.n + channel] = value;
+                        continue;
+                    }
+                    if (MODE == LINEAR && a.residual != nullptr) value = __fadd_rn(value, factor.y);
+                    const size_t out = static_cast<size_t>(token) * a.n + channel;
+                    if (MODE == LINEAR && a.to_f32) reinterpret_cast<float *>(a.y)[out] = value;
+                    else reinterpret_cast<uint16_t *>(a.y)[out] = to_bf16(value);
+                }
+                if (DOWN && (tile + 1 == last_tile || (tile + 1) / a.row_tiles != which)) {  // the scales may go
+                    asm volatile("bar.sync 3, 128;" ::: "memory");
+                    if (thread == 0) arrive(b_empty + ((builds - 1) & 1) * 8);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLUMNS) : "memory");
 }
 
 // ---- experts: routes grouped by expert
@@ -507,7 +957,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int 
 }
 
 // y[token] = the sum of its routes' weighted rows, in their order (+ residual), rounded once.  Four columns to a thread.
-__global__ void experts_sum_kernel(const float *__restrict__ parts, const int *__restrict__ place_of, const uint16_t *residual, uint16_t *y, int top_k, int hidden,
+__global__ void experts_sum_kernel(const float *__restrict__ parts, const int *__restrict__ ids, const uint16_t *residual, uint16_t *y, int top_k, int experts, int hidden,
                                    int wide) {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -521,8 +971,9 @@ __global__ void experts_sum_kernel(const float *__restrict__ parts, const int *_
         float4 values[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; i++)
-            if (first + i < top_k && place_of[token * top_k + first + i] >= 0) values[i] = *reinterpret_cast<const float4 *>(part + static_cast<size_t>(first + i) * hidden);
-            else values[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            values[i] = first + i < top_k && static_cast<uint32_t>(ids[token * top_k + first + i]) < static_cast<uint32_t>(experts)
+                            ? *reinterpret_cast<const float4 *>(part + static_cast<size_t>(first + i) * hidden)
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < BATCH; i++) sum.x += values[i].x, sum.y += values[i].y, sum.z += values[i].z, sum.w += values[i].w;
     }
@@ -593,49 +1044,101 @@ void plan_dense(Int8Args &args, bool pair) {
 
 }  // namespace
 
-cudaError_t launch_quantise_int8(const uint16_t *x, int8_t *q, float *scales, int lanes, int k, cudaStream_t stream) {
-    const int wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    return launch_dependent(quantise_rows_kernel<uint16_t>, dim3(lanes), dim3(quantise_threads(k)), 0, 1, stream, x, q, scales, nullptr, nullptr, 1, k, wide);
+namespace {
+
+size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// Tiles of `matrices` matrices of n output channels for the few-lane kernel: as few rows for the busiest CTA as possible, a
+// tile counted as the bytes of four rows more.
+void plan_stream(StreamArgs &args, int matrices, bool pair) {
+    const int count = multiprocessors(), most = pair ? 64 : 128;
+    int64_t best = 0;
+    for (int rows = std::min(most, args.n); rows >= 1; rows--) {
+        const int64_t tiles = static_cast<int64_t>(matrices) * ((args.n + rows - 1) / rows), cost = (tiles + count - 1) / count * (rows + 4);
+        if (best == 0 || cost < best) best = cost, args.rows = rows;
+    }
+    args.row_tiles = (args.n + args.rows - 1) / args.rows;
+    args.groups = args.rows * 4 <= most ? 4 : args.rows * 2 <= most ? 2 : 1;
+}
+size_t stream_bytes(const StreamArgs &args, bool two_buffers, size_t tables) {
+    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups;
+    return STREAM_CONTROL + tables + static_cast<size_t>(steps * args.groups) * ATOM * (two_buffers ? 2 : 1);
+}
+// Where a CTA's share of the weights is small, two CTAs of successive calls fit on a multiprocessor if three stages leave room
+// for that: the next one quantises while this one writes its outputs.  Larger shares take all the stages there is room for.
+// False where the activations' atoms leave no room for three.
+bool plan_stages(StreamArgs &args, int tiles, bool two_buffers, size_t tables, size_t *bytes) {
+    const size_t fixed = stream_bytes(args, two_buffers, tables);
+    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, count = multiprocessors();
+    const int64_t steps = static_cast<int64_t>((tiles + count - 1) / count) * ((blocks + args.groups - 1) / args.groups);
+    size_t room = SMEM_HALF;
+    if (fixed + 3 * STREAM_STAGE > room || steps > STREAM_SMALL_SHARE) room = SMEM_LIMIT;
+    if (fixed + 3 * STREAM_STAGE > room) return false;
+    args.stages = static_cast<int>(std::min<size_t>(STREAM_MAX_STAGES, (room - fixed) / STREAM_STAGE));
+    *bytes = fixed + static_cast<size_t>(args.stages) * STREAM_STAGE;
+    return true;
+}
+template <Mode MODE>
+cudaError_t launch_stream(const StreamArgs &args, int tiles, size_t bytes, cudaStream_t stream) {
+    const cudaError_t status = cudaFuncSetAttribute(int8_stream_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM_LIMIT));
+    if (status != cudaSuccess) return status;
+    return launch_dependent(int8_stream_kernel<MODE>, dim3(std::min(tiles, multiprocessors())), dim3(STREAM_THREADS), bytes, 1, stream, args);
 }
 
-cudaError_t launch_linear_int8(const int8_t *q, const float *lane_scales, const int8_t *w, const float *scales, void *y, const uint16_t *residual, int lanes, int n,
-                               int k, int to_f32, int *error_flag, cudaStream_t stream) {
+// The activations of a linear in the caller's scratch buffer: whole numbers, then one scale per lane.
+struct Int8Rows {
+    int8_t *values;
+    float *scales;
+    Int8Rows(void *scratch, int lanes, int k)
+        : values(static_cast<int8_t *>(scratch)), scales(reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + padded(static_cast<size_t>(lanes) * k))) {}
+};
+
+// gate alone (up == nullptr) or the pair.
+template <Mode MODE>
+cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales, const int8_t *up, const float *up_scales, void *y, const uint16_t *residual, void *scratch,
+                         int lanes, int n, int k, int to_f32, int *error_flag, cudaStream_t stream) {
+    constexpr bool TWO = MODE == PAIR;
+    if (lanes <= FEW) {
+        StreamArgs args = {};
+        args.x = x, args.scales = scales, args.up_scales = up_scales, args.y = y, args.residual = residual;
+        args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
+        args.wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+        plan_stream(args, 1, TWO);
+        size_t bytes;
+        if (plan_stages(args, args.row_tiles, false, 0, &bytes)) {
+            if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows))) return cudaErrorInvalidValue;
+            return launch_stream<MODE>(args, args.row_tiles, bytes, stream);
+        }
+    }
+    const Int8Rows rows(scratch, lanes, k);
+    const cudaError_t status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, lanes, 1, k, stream);
+    if (status != cudaSuccess) return status;
     Int8Args args = {};
-    args.lanes = lanes;
-    args.n = n;
-    args.k = k;
-    plan_dense(args, false);
-    if (!encode(&args.weights, w, n, k, args.tile_rows) || !encode(&args.activations, q, lanes, k, args.box_lanes)) return cudaErrorInvalidValue;
-    args.scales = scales;
-    args.lane_scales = lane_scales;
-    args.y = y;
-    args.residual = residual;
-    args.to_f32 = to_f32;
-    args.error_flag = error_flag;
-    return launch_gemm<LINEAR>(args, args.row_tiles * args.lane_tiles, stream);
+    args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
+    plan_dense(args, TWO);
+    if (!encode(&args.weights, w, n, k, TWO ? 16 : args.tile_rows) || (TWO && !encode(&args.up, up, n, k, 16)) || !encode(&args.activations, rows.values, lanes, k, args.box_lanes))
+        return cudaErrorInvalidValue;
+    args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
+    return launch_gemm<MODE>(args, args.row_tiles * args.lane_tiles, stream);
 }
 
-cudaError_t launch_linear_int8_silu_pair(const int8_t *q, const float *lane_scales, const int8_t *gate, const float *gate_scales, const int8_t *up,
-                                         const float *up_scales, uint16_t *y, int lanes, int n, int k, int *error_flag, cudaStream_t stream) {
-    Int8Args args = {};
-    args.lanes = lanes;
-    args.n = n;
-    args.k = k;
-    plan_dense(args, true);
-    if (!encode(&args.weights, gate, n, k, 16) || !encode(&args.up, up, n, k, 16) || !encode(&args.activations, q, lanes, k, args.box_lanes)) return cudaErrorInvalidValue;
-    args.scales = gate_scales;
-    args.up_scales = up_scales;
-    args.lane_scales = lane_scales;
-    args.y = y;
-    args.error_flag = error_flag;
-    return launch_gemm<PAIR>(args, args.row_tiles * args.lane_tiles, stream);
+}  // namespace
+
+size_t linear_int8_scratch_bytes(int lanes, int k) { return padded(static_cast<size_t>(lanes) * k) + static_cast<size_t>(lanes) * sizeof(float); }
+
+cudaError_t launch_linear_int8(const uint16_t *x, const int8_t *w, const float *scales, void *y, const uint16_t *residual, void *scratch, int lanes, int n, int k, int to_f32,
+                               int *error_flag, cudaStream_t stream) {
+    return launch_dense<LINEAR>(x, w, scales, nullptr, nullptr, y, residual, scratch, lanes, n, k, to_f32, error_flag, stream);
+}
+
+cudaError_t launch_linear_int8_silu_pair(const uint16_t *x, const int8_t *gate, const float *gate_scales, const int8_t *up, const float *up_scales, uint16_t *y, void *scratch,
+                                         int lanes, int n, int k, int *error_flag, cudaStream_t stream) {
+    return launch_dense<PAIR>(x, gate, gate_scales, up, up_scales, y, nullptr, scratch, lanes, n, k, 0, error_flag, stream);
 }
 
 // ---- the experts
 
 namespace {
-
-size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // The scratch buffer of one call, in parts on 256-byte boundaries; the weighted rows of the down product take the place of
 // what the gate/up product read and wrote.
@@ -693,6 +1196,31 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
                                 int *error_flag, cudaStream_t stream) {
     const ExpertsScratch part(scratch, tokens, top_k, experts, hidden, inter);
     const int pairs = tokens * top_k;
+    auto sum = [&] {
+        const int wide = (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) % 8 == 0;
+        return launch_dependent(experts_sum_kernel, dim3(tokens, (hidden / 4 + 255) / 256), dim3(std::min(256, (hidden / 4 + 31) / 32 * 32)), 0, 1, stream, part.parts, ids,
+                                residual, y, top_k, experts, hidden, wide);
+    };
+    if (tokens <= FEW && pairs <= FEW_ROUTES) {
+        StreamArgs first = {}, second = {};
+        first.n = inter, first.k = hidden, first.x = x, first.scales = gate_up_scales, first.y = part.h;
+        second.n = hidden, second.k = inter, second.x = part.h, second.scales = down_scales, second.y = part.parts;
+        for (StreamArgs *args : {&first, &second}) {
+            args->lanes = tokens, args->ids = ids, args->weights_of = weights, args->top_k = top_k, args->experts = experts, args->error_flag = error_flag;
+            args->wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+            plan_stream(*args, std::min(experts, pairs), args == &first);
+        }
+        size_t first_bytes, second_bytes;
+        if (plan_stages(first, std::min(experts, pairs) * first.row_tiles, false, STREAM_ROUTES, &first_bytes) && plan_stages(second, std::min(experts, pairs) * second.row_tiles, true, STREAM_ROUTES, &second_bytes)) {
+            if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) ||
+                !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows))
+                return cudaErrorInvalidValue;
+            cudaError_t status = launch_stream<EXPERTS_PAIR>(first, std::min(experts, pairs) * first.row_tiles, first_bytes, stream);
+            if (status != cudaSuccess) return status;
+            status = launch_stream<EXPERTS_DOWN>(second, std::min(experts, pairs) * second.row_tiles, second_bytes, stream);
+            return status != cudaSuccess ? status : sum();
+        }
+    }
     Int8Args first = {}, second = {};
     first.n = inter, first.k = hidden;
     second.n = hidden, second.k = inter;
@@ -714,20 +1242,14 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     cudaError_t status = launch_dependent(expert_groups_kernel, dim3(1), dim3(GROUP_THREADS), 0, 1, stream, ids, pairs, experts, first.tile_lanes, part.tiles, part.counts,
                                           part.place_of, part.pair_of);
     if (status != cudaSuccess) return status;
-    const int wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    status = launch_dependent(quantise_rows_kernel<uint16_t>, dim3(tokens), dim3(quantise_threads(hidden)), 0, 1, stream, x, part.xq, part.x_scales, part.place_of, nullptr,
-                              top_k, hidden, wide);
+    status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, tokens, top_k, hidden, stream);
     if (status != cudaSuccess) return status;
     status = launch_gemm<EXPERTS_PAIR>(first, most_tiles * first.row_tiles, stream);
     if (status != cudaSuccess) return status;
-    status = launch_dependent(quantise_rows_kernel<float>, dim3(pairs), dim3(quantise_threads(inter)), 0, 1, stream, part.h, part.hq, part.h_scales, nullptr, part.counts + 1, 1,
-                              inter, 1);
+    status = launch_quantise_rows<float, HeldF32, 2>(part.h, part.hq, part.h_scales, nullptr, part.counts + 1, pairs, 1, inter, stream);
     if (status != cudaSuccess) return status;
     status = launch_gemm<EXPERTS_DOWN>(second, most_tiles * second.row_tiles, stream);
-    if (status != cudaSuccess) return status;
-    const int narrow = (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) % 8 == 0;
-    return launch_dependent(experts_sum_kernel, dim3(tokens, (hidden / 4 + 255) / 256), dim3(std::min(256, (hidden / 4 + 31) / 32 * 32)), 0, 1, stream, part.parts,
-                            part.place_of, residual, y, top_k, hidden, narrow);
+    return status != cudaSuccess ? status : sum();
 }
 
 }  // namespace nerve
