@@ -34,7 +34,7 @@ constexpr int BLOCK_K = 128;  // columns per stage: one swizzled row of 128 byte
 constexpr int ROWS = 128;     // the MMA's M
 constexpr int MAX_LANES = 256, MAX_STAGES = 32;
 constexpr int OUTPUT_WARPS = 8, THREADS = 128 + 32 * OUTPUT_WARPS;
-constexpr size_t SMEM_LIMIT = 226 * 1024, SMEM_HALF = 112 * 1024, CONTROL_BYTES = 1024;
+constexpr size_t SMEM_LIMIT = 226 * 1024, SMEM_HALF = 112 * 1024;
 constexpr unsigned int SPIN_LIMIT = 1u << 22;  // tries of 1.5 us
 
 enum Mode { LINEAR, PAIR, EXPERTS_PAIR, EXPERTS_DOWN };
@@ -85,10 +85,50 @@ __device__ __forceinline__ void copy_tile(uint32_t target, const CUtensorMap *ma
                  : "memory");
 }
 
+// ---- of a pair of CTAs (cta_group::2)
+__device__ __forceinline__ uint32_t of_rank(uint32_t address, int rank) {  // the same place in that CTA's shared memory
+    uint32_t out;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(address), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ void copy_tile_of_pair(uint32_t target, const CUtensorMap *map, int column, int row, uint32_t barrier) {  // barrier: either CTA's
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(target), "l"(map), "r"(column),
+                 "r"(row), "r"(barrier)
+                 : "memory");
+}
+__device__ __forceinline__ void commit_to_pair(uint32_t barrier) {  // that barrier of both CTAs
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t barrier) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier) : "memory"); }
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Into L2, which later writes to the tile reach: safe ahead of the wait for the kernel in front, whatever that writes.
 __device__ __forceinline__ void prefetch_tile(const CUtensorMap *map, int column, int row) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(column), "r"(row) : "memory");
 }
+
+// Whether it holds for all COUNT threads of named barrier ID: they go on together or not at all.
+template <int ID, int COUNT>
+__device__ __forceinline__ bool all_of(bool mine) {
+    uint32_t all;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 p, %1, 0;\n"
+        "bar.red.and.pred q, %2, %3, p;\n"
+        "selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(mine)), "n"(ID), "n"(COUNT)
+        : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ uint32_t shared_address(const void *pointer) { return static_cast<uint32_t>(__cvta_generic_to_shared(pointer)); }
+__device__ __forceinline__ void arrive(uint32_t barrier) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory"); }
+__device__ __forceinline__ void init_barrier(uint32_t barrier, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory"); }
+
 
 // NaN stays NaN.
 __device__ __forceinline__ uint16_t to_bf16(float value) { return __bfloat16_as_ushort(__float2bfloat16_rn(value)); }
@@ -248,13 +288,14 @@ cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int
 // ---- the product
 
 struct Int8Args {
-    CUtensorMap weights, up, activations;  // boxes of 128 columns x box_rows weight rows, and x box_lanes lanes
+    CUtensorMap weights, up, activations;  // boxes of 128 columns x rows (a pair: quarter_rows) weight rows, and x box_lanes lanes
     const float *scales, *up_scales, *lane_scales;
     void *y;
     const uint16_t *residual;
     int lanes, n, k, to_f32;
     int *error_flag;
-    int tile_rows, tile_lanes, box_lanes, lane_tiles, row_tiles, stages;
+    int rows;  // weight rows of a CTA (linear), or output channels of every quarter of it (pair)
+    int tile_lanes, box_lanes, lane_tiles, row_tiles, stages;
     // experts
     const int4 *tiles;
     const int *tile_count, *pair_of;
@@ -262,21 +303,22 @@ struct Int8Args {
 };
 
 struct Tile {
-    int row0;   // first output channel
+    int row0;  // first output channel of this CTA
     int lane0, count, expert;
 };
 template <Mode MODE>
-__device__ __forceinline__ Tile tile_at(const Int8Args &a, int index) {
+__device__ __forceinline__ Tile tile_at(const Int8Args &a, int index, int rank) {
+    constexpr bool TWO = MODE == PAIR || MODE == EXPERTS_PAIR;
     Tile tile;
-    const int outputs = MODE == PAIR || MODE == EXPERTS_PAIR ? a.tile_rows / 2 : a.tile_rows;
+    const int outputs = TWO ? 4 * a.rows : a.rows;
     if (MODE == LINEAR || MODE == PAIR) {
-        tile.row0 = index / a.lane_tiles * outputs;
+        tile.row0 = (index / a.lane_tiles * 2 + rank) * outputs;
         tile.lane0 = index % a.lane_tiles * a.tile_lanes;
         tile.count = min(a.tile_lanes, a.lanes - tile.lane0);
         tile.expert = 0;
     } else {
         const int4 group = a.tiles[index / a.row_tiles];
-        tile.row0 = index % a.row_tiles * outputs;
+        tile.row0 = (index % a.row_tiles * 2 + rank) * outputs;
         tile.expert = group.x;
         tile.lane0 = group.y;
         tile.count = group.z;
@@ -288,9 +330,9 @@ template <Mode MODE, typename Visit>
 __device__ __forceinline__ void visit_weights(const Int8Args &a, const Tile &tile, int which, Visit visit) {
     if (MODE == LINEAR || MODE == EXPERTS_DOWN) {
         visit(&a.weights, tile.expert * a.n + tile.row0, 0);
-    } else {  // sixteen rows each, by turns of gate and of up
+    } else {  // for every quarter of the accumulator's rows, sixteen of gate and the same sixteen of up
         const bool up = which & 1;
-        const int row = tile.row0 + (which >> 1) * 16;
+        const int row = tile.row0 + (which >> 1) * a.rows;
         if (MODE == PAIR) visit(up ? &a.up : &a.weights, row, which * 16);
         else visit(&a.weights, tile.expert * 2 * a.n + (up ? a.n : 0) + row, which * 16);
     }
@@ -300,23 +342,40 @@ __device__ __forceinline__ void visit_weights(const Int8Args &a, const Tile &til
 __device__ __forceinline__ float scaled(int sum, float factor, float lane_scale) { return __fmul_rn(__fmul_rn(static_cast<float>(sum), factor), lane_scale); }
 __device__ __forceinline__ float silu_product(float gate, float up) { return __fmul_rn(__fdividef(gate, __fadd_rn(1.0f, __expf(-gate))), up); }
 
+// What belongs to the lanes of a tile: its scale (the down product: times the route's weight) and where its row goes.
+struct LaneInfo {
+    float scale[MAX_LANES];
+    int to[MAX_LANES];
+};
+struct GemmControl {
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    LaneInfo lanes[2];
+};
+constexpr size_t GEMM_CONTROL = (sizeof(GemmControl) + 1023) / 1024 * 1024;
+
 template <Mode MODE>
-__global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr bool GROUPED = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN, TWO = MODE == PAIR || MODE == EXPERTS_PAIR;
+    GemmControl &control = *reinterpret_cast<GemmControl *>(smem);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
-    const uint32_t a_bytes = static_cast<uint32_t>(a.tile_rows) * BLOCK_K, stage_bytes = a_bytes + static_cast<uint32_t>(a.tile_lanes) * BLOCK_K;
-    const uint32_t control = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), base = control + static_cast<uint32_t>(CONTROL_BYTES);
-    const uint32_t full = control, empty = full + 8 * MAX_STAGES, acc_full = empty + 8 * MAX_STAGES, acc_empty = acc_full + 16, tmem_slot = acc_empty + 16;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;         // rank: of the CTA in its pair
+    const uint32_t a_bytes = TWO ? ROWS * BLOCK_K : static_cast<uint32_t>((a.rows + 7) / 8 * 8) * BLOCK_K, stage_bytes = a_bytes + static_cast<uint32_t>(a.tile_lanes / 2) * BLOCK_K;
+    const uint32_t base = shared_address(smem) + static_cast<uint32_t>(GEMM_CONTROL);
+    const uint32_t full = shared_address(control.full), empty = shared_address(control.empty), acc_full = shared_address(control.acc_full),
+                   acc_empty = shared_address(control.acc_empty);
+    // the first CTA's barriers, which both CTAs' copies and outputs report to
+    const uint32_t leader_full = of_rank(full, 0), leader_acc_empty = of_rank(acc_empty, 0);
     const int blocks = (a.k + BLOCK_K - 1) / BLOCK_K;
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + s * 8) : "memory");
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty + s * 8) : "memory");
+            init_barrier(full + s * 8, 1);
+            init_barrier(empty + s * 8, 1);
         }
         for (int s = 0; s < 2; s++) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(acc_full + s * 8) : "memory");
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty + s * 8), "r"(OUTPUT_WARPS) : "memory");
+            init_barrier(acc_full + s * 8, 1);
+            init_barrier(acc_empty + s * 8, 2 * OUTPUT_WARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -324,50 +383,52 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
     uint32_t columns = 32;
     while (columns < 2 * acc_columns) columns *= 2;
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tmem)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    pair_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    // not before the tensor memory is this CTA's: one of the next kernel's that took it first would wait for this one
+    // not before the tensor memory is this pair's: one of the next kernel's that took it first would wait for this one
     grid_launch_dependents();
     uint32_t tmem;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(shared_address(&control.tmem)) : "memory");
     tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
 
-    if (warp == 0) {  // ---- copies
-        const int weight_boxes = TWO ? a.tile_rows / 16 : 1;
+    if (warp == 0) {  // ---- copies: this CTA's weight rows and its half of the lanes
+        const int weight_boxes = TWO ? 8 : 1;
         int stage = 0, issued = 0;
         uint32_t parity = 1;  // the first round waits for no release
         if (!GROUPED) {
-            const Tile tile = tile_at<MODE>(a, blockIdx.x);
+            const Tile tile = tile_at<MODE>(a, pair, rank);
             for (int block = 0; block < min(a.stages, blocks); block++)
                 if (lane < weight_boxes) visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int) { prefetch_tile(map, block * BLOCK_K, row); });
         }
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
         bool alive = true;
-        for (int index = blockIdx.x; index < tiles && alive; index += gridDim.x) {
-            const Tile tile = tile_at<MODE>(a, index);
-            const int lane_boxes = (tile.count + a.box_lanes - 1) / a.box_lanes;
-            const uint32_t bytes = a_bytes + static_cast<uint32_t>(lane_boxes * a.box_lanes) * BLOCK_K;
+        Tile tile = pair < tiles ? tile_at<MODE>(a, pair, rank) : Tile{};
+        for (int index = pair; index < tiles && alive; index += pairs) {
+            const Tile next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, rank) : tile;
+            const int half = (tile.count + 31) / 32 * 16, lane_boxes = (half + a.box_lanes - 1) / a.box_lanes;
+            const uint32_t bytes = 2 * static_cast<uint32_t>((TWO ? 8 : 1) * a.rows + lane_boxes * a.box_lanes) * BLOCK_K;  // of both CTAs
             for (int block = 0; block < blocks; block++) {
-                const uint32_t target = base + static_cast<uint32_t>(stage) * stage_bytes, barrier = full + stage * 8;
+                const uint32_t target = base + static_cast<uint32_t>(stage) * stage_bytes, barrier = leader_full + stage * 8;
                 if (!wait_barrier(empty + stage * 8, parity, a.error_flag)) {
-                    for (int s = 0; s < a.stages && s < issued; s++) {  // the copies in flight land before the CTA gives its memory up
+                    for (int s = 0; rank == 0 && s < a.stages && s < issued; s++) {  // the copies in flight land before the CTAs give their memory up
                         const int which = (issued - 1 - s) % a.stages;
                         wait_barrier(full + which * 8, static_cast<uint32_t>(((issued - 1 - s) / a.stages) & 1), a.error_flag);
                     }
                     alive = false;
                     break;
                 }
-                if (elect_one()) expect_bytes(barrier, bytes);
+                if (rank == 0 && elect_one()) expect_bytes(full + stage * 8, bytes);
                 __syncwarp();
                 if (lane < weight_boxes)
-                    visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int at) { copy_tile(target + at * BLOCK_K, map, block * BLOCK_K, row, barrier); });
+                    visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int at) { copy_tile_of_pair(target + at * BLOCK_K, map, block * BLOCK_K, row, barrier); });
                 if (lane < lane_boxes)
-                    copy_tile(target + a_bytes + static_cast<uint32_t>(lane * a.box_lanes) * BLOCK_K, &a.activations, block * BLOCK_K, tile.lane0 + lane * a.box_lanes, barrier);
+                    copy_tile_of_pair(target + a_bytes + static_cast<uint32_t>(lane * a.box_lanes) * BLOCK_K, &a.activations, block * BLOCK_K,
+                                      tile.lane0 + rank * half + lane * a.box_lanes, barrier);
                 __syncwarp();
                 issued++;
                 if (++stage == a.stages) {
@@ -375,19 +436,21 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                     parity ^= 1;
                 }
             }
+            tile = next;
         }
-    } else if (warp == 1) {  // ---- MMAs
+    } else if (warp == 1) {  // ---- MMAs, by the first CTA for both
         const uint64_t first = swizzled_descriptor(base);
         int stage = 0, round = 0;
         uint32_t parity = 0;
-        bool alive = true;
+        bool alive = rank == 0;
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
-        for (int index = blockIdx.x; index < tiles && alive; index += gridDim.x, round++) {
-            const Tile tile = tile_at<MODE>(a, index);
+        int count = alive && pair < tiles ? tile_at<MODE>(a, pair, 0).count : 0;
+        for (int index = pair; index < tiles && alive; index += pairs, round++) {
+            const int next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, 0).count : 0;
             // instruction descriptor: s32 accumulator, A and B signed bytes, both K-major, N / 8 in bits 17-22, M / 16 in bits 24-28
-            const uint32_t instruction =
-                __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>((tile.count + 15) / 16 * 2) << 17) | (8u << 24));
+            // (M = 256 with bytes: N in steps of 32)
+            const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>((count + 31) / 32 * 4) << 17) | (16u << 24));
             const uint32_t accumulator = tmem + (round & 1) * acc_columns;
             if (!wait_barrier(acc_empty + (round & 1) * 8, static_cast<uint32_t>((round / 2 + 1) & 1), a.error_flag)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -406,13 +469,13 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                             "{\n"
                             ".reg .pred p;\n"
                             "setp.ne.b32 p, %4, 0;\n"
-                            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+                            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
                             "}\n" ::"r"(accumulator),
                             "l"(a_stage + step * 2), "l"(b_stage + step * 2), "r"(instruction), "r"(accumulate)
                             : "memory");
                     }
-                    commit_to(empty + stage * 8);
-                    if (block == blocks - 1) commit_to(acc_full + (round & 1) * 8);
+                    commit_to_pair(empty + stage * 8);
+                    if (block == blocks - 1) commit_to_pair(acc_full + (round & 1) * 8);
                 }
                 __syncwarp();
                 if (++stage == a.stages) {
@@ -420,26 +483,39 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                     parity ^= 1;
                 }
             }
+            count = next;
         }
     } else if (warp >= 4) {  // ---- outputs: thread = row of the accumulator
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
-        const int quarter = warp & 3, part = (warp - 4) >> 2;
+        const int quarter = warp & 3, part = (warp - 4) >> 2, thread = threadIdx.x - 128;
         int round = 0;
-        for (int index = blockIdx.x; index < tiles; index += gridDim.x, round++) {
-            const Tile tile = tile_at<MODE>(a, index);
-            const bool mine = quarter * 32 < a.tile_rows;
+        Tile tile = pair < tiles ? tile_at<MODE>(a, pair, rank) : Tile{};
+        for (int index = pair; index < tiles; index += pairs, round++) {
+            const Tile next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, rank) : tile;
+            const bool mine = TWO || quarter * 32 < a.rows;
             // the output channel of this thread, and its factor: a lane of a pair's upper half holds up's row of the same channel
-            const int channel = TWO ? tile.row0 + quarter * 16 + (lane & 15) : tile.row0 + quarter * 32 + lane;
-            const bool in_range = channel < a.n && (TWO || quarter * 32 + lane < a.tile_rows);
+            const int channel = TWO ? tile.row0 + quarter * a.rows + (lane & 15) : tile.row0 + quarter * 32 + lane;
+            const bool in_range = channel < a.n && (TWO ? (lane & 15) < a.rows : quarter * 32 + lane < a.rows);
             float factor = 0.0f;
-            if (mine && in_range) {
+            if (in_range) {
                 if (MODE == LINEAR) factor = a.scales[channel];
                 else if (MODE == PAIR) factor = (lane < 16 ? a.scales : a.up_scales)[channel];
                 else if (MODE == EXPERTS_PAIR) factor = a.scales[static_cast<size_t>(tile.expert) * 2 * a.n + (lane < 16 ? 0 : a.n) + channel];
                 else factor = a.scales[static_cast<size_t>(tile.expert) * a.n + channel];
             }
-            if (!wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag)) break;
+            LaneInfo &info = control.lanes[round & 1];  // (the sums of two tiles before are out: all passed the barrier of the last one)
+            if (thread < tile.count) {
+                float scale = a.lane_scales[tile.lane0 + thread];
+                int to = tile.lane0 + thread;
+                if (MODE == EXPERTS_DOWN) {
+                    to = a.pair_of[to];
+                    scale = __fmul_rn(scale, a.weights_of[to]);
+                }
+                info.scale[thread] = scale;
+                info.to[thread] = to;
+            }
+            if (!all_of<1, 32 * OUTPUT_WARPS>(wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t accumulator = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (round & 1) * acc_columns;
             if (mine)
@@ -450,44 +526,33 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                                    "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
                                  : "r"(accumulator + static_cast<uint32_t>(column))
                                  : "memory");
-                    const int count = min(16, tile.count - column), first_lane = tile.lane0 + column;
-                    // thread i < 16 fetches what belongs to lane i of these sixteen
-                    float lane_scale = 0.0f;
-                    int pair = 0;
-                    if (lane < count) {
-                        lane_scale = a.lane_scales[first_lane + lane];
-                        if (MODE == EXPERTS_DOWN) {
-                            pair = a.pair_of[first_lane + lane];
-                            lane_scale = __fmul_rn(lane_scale, a.weights_of[pair]);
-                        }
-                    }
+                    const int count = min(16, tile.count - column);
+                    float residual[16];
+                    if (MODE == LINEAR && a.residual != nullptr)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (in_range && i < count) residual[i] = bf16_bits_to_f32(a.residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (TWO) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {  // the warp's lower half finishes lane i, its upper half lane i + 1
-                            const float low = scaled(static_cast<int>(d[i]), factor, __shfl_sync(0xffffffffu, lane_scale, i));
-                            const float high = scaled(static_cast<int>(d[i + 1]), factor, __shfl_sync(0xffffffffu, lane_scale, i + 1));
+                            const float low = scaled(static_cast<int>(d[i]), factor, info.scale[column + i]);
+                            const float high = scaled(static_cast<int>(d[i + 1]), factor, info.scale[column + i + 1]);
                             const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? high : low, 16);
                             const float product = lane < 16 ? silu_product(low, other) : silu_product(other, high);
                             const int at = i + (lane >> 4);
                             if (in_range && at < count) {
-                                const size_t out = static_cast<size_t>(first_lane + at) * a.n + channel;
+                                const size_t out = static_cast<size_t>(tile.lane0 + column + at) * a.n + channel;
                                 if (MODE == PAIR) reinterpret_cast<uint16_t *>(a.y)[out] = to_bf16(product);
                                 else reinterpret_cast<float *>(a.y)[out] = product;
                             }
                         }
-                    } else {
-                        float residual[16];
-                        if (MODE == LINEAR && a.residual != nullptr)
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                if (in_range && i < count) residual[i] = bf16_bits_to_f32(a.residual[static_cast<size_t>(first_lane + i) * a.n + channel]);
+                    } else if (in_range) {
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            float value = scaled(static_cast<int>(d[i]), factor, __shfl_sync(0xffffffffu, lane_scale, i));
-                            const int to = MODE == EXPERTS_DOWN ? __shfl_sync(0xffffffffu, pair, i) : first_lane + i;
-                            if (!in_range || i >= count) continue;
-                            const size_t out = static_cast<size_t>(to) * a.n + channel;
+                            if (i >= count) break;
+                            float value = scaled(static_cast<int>(d[i]), factor, info.scale[column + i]);
+                            const size_t out = static_cast<size_t>(MODE == EXPERTS_DOWN ? info.to[column + i] : tile.lane0 + column + i) * a.n + channel;
                             if (MODE == EXPERTS_DOWN) {
                                 reinterpret_cast<float *>(a.y)[out] = value;
                             } else {
@@ -500,12 +565,13 @@ __global__ void __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_cons
                 }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(acc_empty + (round & 1) * 8) : "memory");
+            if (lane == 0) arrive_at(leader_acc_empty + (round & 1) * 8);
+            tile = next;
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    pair_sync();  // neither CTA leaves while the other still reads its memory or reports to its barriers
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
 // ---- few lanes: the weights stream by, the activations stay
@@ -638,26 +704,6 @@ __device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Whether it holds for all 128 threads of named barrier ID: they go on together or not at all.
-template <int ID>
-__device__ __forceinline__ bool all_of(bool mine) {
-    uint32_t all;
-    asm volatile(
-        "{\n"
-        ".reg .pred p, q;\n"
-        "setp.ne.u32 p, %1, 0;\n"
-        "bar.red.and.pred q, %2, 128, p;\n"
-        "selp.u32 %0, 1, 0, q;\n"
-        "}\n"
-        : "=r"(all)
-        : "r"(static_cast<uint32_t>(mine)), "n"(ID)
-        : "memory");
-    return all != 0;
-}
-__device__ __forceinline__ uint32_t shared_address(const void *pointer) { return static_cast<uint32_t>(__cvta_generic_to_shared(pointer)); }
-__device__ __forceinline__ void arrive(uint32_t barrier) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory"); }
-__device__ __forceinline__ void init_barrier(uint32_t barrier, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory"); }
-
 constexpr size_t STREAM_CONTROL = (sizeof(StreamControl) + 1023) / 1024 * 1024, STREAM_ROUTES = (sizeof(StreamRoutes) + 1023) / 1024 * 1024;
 
 template <Mode MODE>
@@ -747,7 +793,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
         }
     } else if (warp == 1) {  // ---- MMAs
         if (!GROUPED) grid_dependency_wait();
-        // instruction descriptor as in int8_gemm_kernel
+        // instruction descriptor as in int8_gemm_kernel, M = 128
         const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(max(2, a.groups)) << 17) | (8u << 24));
         const uint64_t a_first = swizzled_descriptor(ring), b_first = swizzled_descriptor(shared_address(atoms));
         int stage = 0, round = 0, builds = 0, expert = -1;
@@ -816,7 +862,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                 if (which == expert) continue;
                 expert = which;
                 const int buffer = builds & 1;
-                if (!all_of<2>(wait_barrier(b_empty + buffer * 8, static_cast<uint32_t>((builds / 2 + 1) & 1), a.error_flag))) break;
+                if (!all_of<2, 128>(wait_barrier(b_empty + buffer * 8, static_cast<uint32_t>((builds / 2 + 1) & 1), a.error_flag))) break;
                 quantise_few<128, float, HeldF32>(a, atoms + buffer * atom_bytes, control.amax[buffer], control.lane_scales[buffer], thread - 128,
                                                   [&](int token) -> const float * {
                                                       const int route = routes.lead[which][token];
@@ -856,7 +902,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                 float2 factor = make_float2(0.0f, 0.0f);
                 if (thread < all) factor = factors(thread);
                 alive = alive && wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag);
-                if (!all_of<3>(alive)) break;  // and: the sums of the tile before have been read
+                if (!all_of<3, 128>(alive)) break;  // and: the sums of the tile before have been read
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t d[8];
                 asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -1009,37 +1055,45 @@ bool encode(CUtensorMap *map, const int8_t *matrix, int64_t rows, int k, int box
 }
 
 // As many stages as fit, with room for an A operand of 128 rows at the last one's base.
-void plan_stages(Int8Args &args) {
-    const size_t stage = static_cast<size_t>(args.tile_rows + args.tile_lanes) * BLOCK_K, last = std::max(stage, static_cast<size_t>(ROWS) * BLOCK_K);
-    args.stages = static_cast<int>(std::min<size_t>(MAX_STAGES, 1 + (SMEM_LIMIT - CONTROL_BYTES - last) / stage));
-}
-size_t shared_bytes(const Int8Args &args) {
-    const size_t stage = static_cast<size_t>(args.tile_rows + args.tile_lanes) * BLOCK_K;
-    return CONTROL_BYTES + static_cast<size_t>(args.stages - 1) * stage + std::max(stage, static_cast<size_t>(ROWS) * BLOCK_K);
+size_t stage_bytes(const Int8Args &args, bool pair) { return static_cast<size_t>((pair ? ROWS : (args.rows + 7) / 8 * 8) + args.tile_lanes / 2) * BLOCK_K; }
+size_t plan_stages(Int8Args &args, bool pair) {
+    const size_t stage = stage_bytes(args, pair), last = std::max(stage, static_cast<size_t>(ROWS) * BLOCK_K);
+    args.stages = static_cast<int>(std::min<size_t>(MAX_STAGES, 1 + (SMEM_LIMIT - GEMM_CONTROL - last) / stage));
+    return GEMM_CONTROL + static_cast<size_t>(args.stages - 1) * stage + last;
 }
 
 template <Mode MODE>
-cudaError_t launch_gemm(const Int8Args &args, int most_tiles, cudaStream_t stream) {
+cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
+    const size_t bytes = plan_stages(args, MODE == PAIR || MODE == EXPERTS_PAIR);
     const cudaError_t status = cudaFuncSetAttribute(int8_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM_LIMIT));
     if (status != cudaSuccess) return status;
-    return launch_dependent(int8_gemm_kernel<MODE>, dim3(std::min(most_tiles, multiprocessors())), dim3(THREADS), shared_bytes(args), 1, stream, args);
+    return launch_dependent(int8_gemm_kernel<MODE>, dim3(2 * std::min(most_tiles, multiprocessors() / 2)), dim3(THREADS), bytes, 1, stream, args);
 }
 
-// Tiles of a matrix of n output channels (`pair`: two weight rows each) for that many lanes.
+// Tiles of a matrix of n output channels (`pair`: two weight rows each) for that many lanes, by an estimate of the cycles
+// they take: of a block of 128 columns the tensor pipe needs half the lanes' number for each of four instructions, or as
+// long as it reads the weights, the copies arrive at some 56 bytes per cycle and multiprocessor, and the weights, which the first of a
+// row's tiles brings in, at some 23; and every tile has its start and end.
 void plan_dense(Int8Args &args, bool pair) {
-    const int padded = (args.lanes + 15) / 16 * 16, count = multiprocessors();
-    args.lane_tiles = (padded + MAX_LANES - 1) / MAX_LANES;
-    args.tile_lanes = ((padded + args.lane_tiles - 1) / args.lane_tiles + 15) / 16 * 16;
-    args.lane_tiles = (padded + args.tile_lanes - 1) / args.tile_lanes;
-    args.box_lanes = args.tile_lanes;
-    // as few waves of the chip as 128 rows allow, and then as few rows as make that many waves
-    const int step = pair ? 16 : 8, most = pair ? 64 : 128;
-    const int waves = ((args.n + most - 1) / most * args.lane_tiles + count - 1) / count;
-    int rows = step;
-    while (rows < most && ((args.n + rows - 1) / rows * args.lane_tiles + count - 1) / count > waves) rows += step;
-    args.row_tiles = (args.n + rows - 1) / rows;
-    args.tile_rows = pair ? 2 * rows : rows;
-    plan_stages(args);
+    const int64_t pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K;
+    const int padded = (args.lanes + 31) / 32 * 32, least = (padded + MAX_LANES - 1) / MAX_LANES, most = pair ? 16 : 128;
+    int64_t best = 0;
+    for (int split = least; split <= least + 3 && (split == least || padded / split >= 32); split++) {
+        const int lanes = ((padded + split - 1) / split + 31) / 32 * 32;
+        for (int rows = most; rows >= 1; rows -= rows > 32 ? 4 : 1) {
+            const int64_t outputs = 2 * rows * (pair ? 4 : 1), weight_rows = pair ? 8 * rows : rows, row_tiles = (args.n + outputs - 1) / outputs;
+            const int64_t lane_tiles = (padded + lanes - 1) / lanes, waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
+            const int64_t tensor = 4 * std::max(lanes / 2, 36), copies = (weight_rows + lanes / 2) * BLOCK_K / 56, memory = weight_rows * BLOCK_K / (23 * lane_tiles);
+            const int64_t cost = waves * (blocks * std::max({tensor, copies, memory}) + 1000);
+            if (best != 0 && cost >= best) continue;
+            best = cost;
+            args.rows = rows;
+            args.row_tiles = static_cast<int>(row_tiles);
+            args.tile_lanes = lanes;
+            args.lane_tiles = static_cast<int>(lane_tiles);
+        }
+    }
+    args.box_lanes = args.tile_lanes / 2;
 }
 
 }  // namespace
@@ -1116,7 +1170,7 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
     Int8Args args = {};
     args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
     plan_dense(args, TWO);
-    if (!encode(&args.weights, w, n, k, TWO ? 16 : args.tile_rows) || (TWO && !encode(&args.up, up, n, k, 16)) || !encode(&args.activations, rows.values, lanes, k, args.box_lanes))
+    if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.box_lanes))
         return cudaErrorInvalidValue;
     args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
     return launch_gemm<MODE>(args, args.row_tiles * args.lane_tiles, stream);
@@ -1177,14 +1231,13 @@ struct ExpertsScratch {
 void plan_experts(Int8Args &args, int pairs, int experts, bool pair) {
     // room for twice an expert's even share, so that most experts meet their weights once
     const int share = (pairs + experts - 1) / experts;
-    int lanes = 16;
+    int lanes = 32;
     while (lanes < 2 * share && lanes < MAX_LANES) lanes *= 2;
     args.tile_lanes = lanes;
-    args.box_lanes = std::min(lanes, 32);
-    args.tile_rows = 128;
-    const int outputs = pair ? 64 : 128;
+    args.box_lanes = std::min(lanes / 2, 32);
+    args.rows = pair ? 16 : 128;
+    const int outputs = pair ? 128 : 256;  // of a pair of CTAs
     args.row_tiles = (args.n + outputs - 1) / outputs;
-    plan_stages(args);
 }
 
 }  // namespace
@@ -1226,8 +1279,8 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     second.n = hidden, second.k = inter;
     plan_experts(first, pairs, experts, true);
     plan_experts(second, pairs, experts, false);
-    if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, 16) || !encode(&first.activations, part.xq, pairs, hidden, first.box_lanes) ||
-        !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.tile_rows) || !encode(&second.activations, part.hq, pairs, inter, second.box_lanes))
+    if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) || !encode(&first.activations, part.xq, pairs, hidden, first.box_lanes) ||
+        !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows) || !encode(&second.activations, part.hq, pairs, inter, second.box_lanes))
         return cudaErrorInvalidValue;
     first.scales = gate_up_scales, second.scales = down_scales;
     first.lane_scales = part.x_scales, second.lane_scales = part.h_scales;
