@@ -12,8 +12,8 @@
 // the MMA's A operand is then whatever lies behind in shared memory, and the rest of the accumulator is never read.  So a
 // matrix is cut into as many row tiles as the chip has multiprocessors, and few lanes need no split of K.
 //
-// The gate/up pair takes both matrices in one tile: every 32 rows of A are sixteen of gate and the same sixteen of up, so
-// that the two factors of an output meet by one exchange between the two halves of a warp.
+// The gate/up pair multiplies the same lanes by a tile of each matrix into sums that lie side by side, so that one thread holds both
+// factors of an output.
 //
 // The experts' products are the same kernel over tiles that expert_groups_kernel makes of the routes.
 // Waits are bounded; a wait that expires sets the error word, and the CTA still frees its tensor memory.  The unbounded wait
@@ -218,12 +218,13 @@ __device__ __forceinline__ uint4 quantise(const Held &held, const RowScale &row)
 
 // One CTA per row of x, which its threads hold in registers, HELD times sixteen values each; what is wider is read again,
 // from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once to the place of each
-// of its top_k routes, where it has one.  Bound by DRAM for large batches, by the chain of loads, barrier and stores for small
+// of its top_k routes, where it has one.  With weights the scale is that of row times its route's weight.  Bound by DRAM for large batches, by the chain of loads, barrier and stores for small
 // ones.
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.
 template <typename T, typename Held, int HELD>
 __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__restrict__ scales, const int *__restrict__ places,
-                                                            const int *__restrict__ row_count, int top_k, int k, int wide) {
+                                                            const int *__restrict__ row_count, const int *__restrict__ pair_of, const float *__restrict__ weights, int top_k, int k,
+                                                            int wide) {
     __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
@@ -267,18 +268,19 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *__restrict_
     }
     for (int copy = threadIdx.x; copy < copies; copy += blockDim.x) {
         const int place = places != nullptr ? own_places[copy] : static_cast<int>(blockIdx.x);
-        if (place >= 0) scales[place] = scale.scale;
+        if (place >= 0) scales[place] = weights != nullptr ? __fmul_rn(scale.scale, weights[pair_of[place]]) : scale.scale;
     }
 }
 
 // The rows are cut so that a thread holds its part of up to 32768 columns (bf16) or 16384 (f32), with as many threads as
 // sixteen columns each ask for up to 256, then more columns each.
 template <typename T, typename Held, int MOST>
-cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int rows, int top_k, int k, cudaStream_t stream) {
+cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, const int *pair_of, const float *weights, int rows, int top_k,
+                                 int k, cudaStream_t stream) {
     const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto with = [&](auto kernel, int held) {
         const int threads = std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
-        return launch_dependent(kernel, dim3(rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, top_k, k, wide);
+        return launch_dependent(kernel, dim3(rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, pair_of, weights, top_k, k, wide);
     };
     if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1>, 1);
     if (parts <= 1024 || MOST == 2) return with(quantise_rows_kernel<T, Held, 2>, 2);
@@ -288,18 +290,17 @@ cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int
 // ---- the product
 
 struct Int8Args {
-    CUtensorMap weights, up, activations;  // boxes of 128 columns x rows (a pair: quarter_rows) weight rows, and x box_lanes lanes
+    CUtensorMap weights, up, activations;  // boxes of 128 columns x rows weight rows, and x tile_lanes / 2 lanes
     const float *scales, *up_scales, *lane_scales;
     void *y;
     const uint16_t *residual;
     int lanes, n, k, to_f32;
     int *error_flag;
-    int rows;  // weight rows of a CTA (linear), or output channels of every quarter of it (pair)
-    int tile_lanes, box_lanes, lane_tiles, row_tiles, stages;
+    int rows;  // output channels of a CTA's tile
+    int tile_lanes, lane_tiles, row_tiles, stages, buffers;
     // experts
     const int4 *tiles;
     const int *tile_count, *pair_of;
-    const float *weights_of;
 };
 
 struct Tile {
@@ -308,60 +309,62 @@ struct Tile {
 };
 template <Mode MODE>
 __device__ __forceinline__ Tile tile_at(const Int8Args &a, int index, int rank) {
-    constexpr bool TWO = MODE == PAIR || MODE == EXPERTS_PAIR;
     Tile tile;
-    const int outputs = TWO ? 4 * a.rows : a.rows;
     if (MODE == LINEAR || MODE == PAIR) {
-        tile.row0 = (index / a.lane_tiles * 2 + rank) * outputs;
+        tile.row0 = (index / a.lane_tiles * 2 + rank) * a.rows;
         tile.lane0 = index % a.lane_tiles * a.tile_lanes;
         tile.count = min(a.tile_lanes, a.lanes - tile.lane0);
         tile.expert = 0;
     } else {
         const int4 group = a.tiles[index / a.row_tiles];
-        tile.row0 = (index % a.row_tiles * 2 + rank) * outputs;
+        tile.row0 = (index % a.row_tiles * 2 + rank) * a.rows;
         tile.expert = group.x;
         tile.lane0 = group.y;
         tile.count = group.z;
     }
     return tile;
 }
-// Box `which` of a stage's weights: visit(map, row of the matrix, row of the stage).
-template <Mode MODE, typename Visit>
-__device__ __forceinline__ void visit_weights(const Int8Args &a, const Tile &tile, int which, Visit visit) {
-    if (MODE == LINEAR || MODE == EXPERTS_DOWN) {
-        visit(&a.weights, tile.expert * a.n + tile.row0, 0);
-    } else {  // for every quarter of the accumulator's rows, sixteen of gate and the same sixteen of up
-        const bool up = which & 1;
-        const int row = tile.row0 + (which >> 1) * a.rows;
-        if (MODE == PAIR) visit(up ? &a.up : &a.weights, row, which * 16);
-        else visit(&a.weights, tile.expert * 2 * a.n + (up ? a.n : 0) + row, which * 16);
-    }
+// Gate's (or the only) weight rows of a tile, or up's: map and row of the matrix.
+template <Mode MODE>
+__device__ __forceinline__ const CUtensorMap *weights_of(const Int8Args &a, const Tile &tile, int up, int *row) {
+    *row = MODE == EXPERTS_PAIR ? (tile.expert * 2 + up) * a.n + tile.row0 : tile.expert * a.n + tile.row0;
+    return MODE == PAIR && up ? &a.up : &a.weights;
 }
 
 // The outputs' arithmetic, the same to the bit in every kernel (no contraction).
 __device__ __forceinline__ float scaled(int sum, float factor, float lane_scale) { return __fmul_rn(__fmul_rn(static_cast<float>(sum), factor), lane_scale); }
 __device__ __forceinline__ float silu_product(float gate, float up) { return __fmul_rn(__fdividef(gate, __fadd_rn(1.0f, __expf(-gate))), up); }
 
-// What belongs to the lanes of a tile: its scale (the down product: times the route's weight) and where its row goes.
-struct LaneInfo {
+// What belongs to the lanes of a tile: the scale and where the row goes.
+struct alignas(16) LaneInfo {
     float scale[MAX_LANES];
     int to[MAX_LANES];
 };
 struct GemmControl {
+    LaneInfo lanes[2];
     uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
     uint32_t tmem;
-    LaneInfo lanes[2];
 };
 constexpr size_t GEMM_CONTROL = (sizeof(GemmControl) + 1023) / 1024 * 1024;
+
+__device__ __forceinline__ void load_sums(uint32_t address, int (&d)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]),
+                   "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
+                 : "r"(address)
+                 : "memory");
+}
 
 template <Mode MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr bool GROUPED = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN, TWO = MODE == PAIR || MODE == EXPERTS_PAIR;
+    constexpr int MATRICES = TWO ? 2 : 1;
     GemmControl &control = *reinterpret_cast<GemmControl *>(smem);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;         // rank: of the CTA in its pair
-    const uint32_t a_bytes = TWO ? ROWS * BLOCK_K : static_cast<uint32_t>((a.rows + 7) / 8 * 8) * BLOCK_K, stage_bytes = a_bytes + static_cast<uint32_t>(a.tile_lanes / 2) * BLOCK_K;
+    const uint32_t a_bytes = static_cast<uint32_t>((a.rows + 7) / 8 * 8) * BLOCK_K, half_box = static_cast<uint32_t>(a.tile_lanes / 2) * BLOCK_K,
+                   stage_bytes = MATRICES * a_bytes + half_box;
     const uint32_t base = shared_address(smem) + static_cast<uint32_t>(GEMM_CONTROL);
     const uint32_t full = shared_address(control.full), empty = shared_address(control.empty), acc_full = shared_address(control.acc_full),
                    acc_empty = shared_address(control.acc_empty);
@@ -379,9 +382,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t acc_columns = (static_cast<uint32_t>(a.tile_lanes) + 31u) & ~31u;
+    // one accumulator: the sums of the tile's lanes, gate's and then up's
+    const uint32_t acc_columns = static_cast<uint32_t>(MATRICES * a.tile_lanes);
     uint32_t columns = 32;
-    while (columns < 2 * acc_columns) columns *= 2;
+    while (columns < static_cast<uint32_t>(a.buffers) * acc_columns) columns *= 2;
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tmem)), "r"(columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -395,25 +399,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(shared_address(&control.tmem)) : "memory");
     tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
 
-    if (warp == 0) {  // ---- copies: this CTA's weight rows and its half of the lanes
-        const int weight_boxes = TWO ? 8 : 1;
+    if (warp == 0) {  // ---- copies: this CTA's weight rows and its half of the lanes, one box each (a box takes some 65 cycles to issue)
         int stage = 0, issued = 0;
         uint32_t parity = 1;  // the first round waits for no release
-        if (!GROUPED) {
-            const Tile tile = tile_at<MODE>(a, pair, rank);
-            for (int block = 0; block < min(a.stages, blocks); block++)
-                if (lane < weight_boxes) visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int) { prefetch_tile(map, block * BLOCK_K, row); });
+        if (!GROUPED && lane < MATRICES) {
+            int row;
+            const CUtensorMap *map = weights_of<MODE>(a, tile_at<MODE>(a, pair, rank), lane, &row);
+            for (int block = 0; block < min(a.stages, blocks); block++) prefetch_tile(map, block * BLOCK_K, row);
         }
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
+        const uint32_t bytes = 2 * (static_cast<uint32_t>(MATRICES * a.rows) * BLOCK_K + half_box);  // of both CTAs
         bool alive = true;
         Tile tile = pair < tiles ? tile_at<MODE>(a, pair, rank) : Tile{};
         for (int index = pair; index < tiles && alive; index += pairs) {
             const Tile next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, rank) : tile;
-            const int half = (tile.count + 31) / 32 * 16, lane_boxes = (half + a.box_lanes - 1) / a.box_lanes;
-            const uint32_t bytes = 2 * static_cast<uint32_t>((TWO ? 8 : 1) * a.rows + lane_boxes * a.box_lanes) * BLOCK_K;  // of both CTAs
+            int row;
+            const CUtensorMap *map = lane < MATRICES ? weights_of<MODE>(a, tile, lane, &row) : &a.activations;
+            const uint32_t offset = static_cast<uint32_t>(lane) * a_bytes;
+            if (lane == MATRICES) row = tile.lane0 + rank * ((tile.count + 31) / 32 * 16);
             for (int block = 0; block < blocks; block++) {
-                const uint32_t target = base + static_cast<uint32_t>(stage) * stage_bytes, barrier = leader_full + stage * 8;
                 if (!wait_barrier(empty + stage * 8, parity, a.error_flag)) {
                     for (int s = 0; rank == 0 && s < a.stages && s < issued; s++) {  // the copies in flight land before the CTAs give their memory up
                         const int which = (issued - 1 - s) % a.stages;
@@ -424,11 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                 }
                 if (rank == 0 && elect_one()) expect_bytes(full + stage * 8, bytes);
                 __syncwarp();
-                if (lane < weight_boxes)
-                    visit_weights<MODE>(a, tile, lane, [&](const CUtensorMap *map, int row, int at) { copy_tile_of_pair(target + at * BLOCK_K, map, block * BLOCK_K, row, barrier); });
-                if (lane < lane_boxes)
-                    copy_tile_of_pair(target + a_bytes + static_cast<uint32_t>(lane * a.box_lanes) * BLOCK_K, &a.activations, block * BLOCK_K,
-                                      tile.lane0 + rank * half + lane * a.box_lanes, barrier);
+                if (lane <= MATRICES) copy_tile_of_pair(base + static_cast<uint32_t>(stage) * stage_bytes + offset, map, block * BLOCK_K, row, leader_full + stage * 8);
                 __syncwarp();
                 issued++;
                 if (++stage == a.stages) {
@@ -440,19 +441,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
     } else if (warp == 1) {  // ---- MMAs, by the first CTA for both
         const uint64_t first = swizzled_descriptor(base);
-        int stage = 0, round = 0;
-        uint32_t parity = 0;
+        int stage = 0, buffer = 0;
+        uint32_t parity = 0, buffer_parity = 1;
         bool alive = rank == 0;
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
         int count = alive && pair < tiles ? tile_at<MODE>(a, pair, 0).count : 0;
-        for (int index = pair; index < tiles && alive; index += pairs, round++) {
+        for (int index = pair; index < tiles && alive; index += pairs) {
             const int next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, 0).count : 0;
             // instruction descriptor: s32 accumulator, A and B signed bytes, both K-major, N / 8 in bits 17-22, M / 16 in bits 24-28
             // (M = 256 with bytes: N in steps of 32)
             const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>((count + 31) / 32 * 4) << 17) | (16u << 24));
-            const uint32_t accumulator = tmem + (round & 1) * acc_columns;
-            if (!wait_barrier(acc_empty + (round & 1) * 8, static_cast<uint32_t>((round / 2 + 1) & 1), a.error_flag)) break;
+            const uint32_t accumulator = tmem + static_cast<uint32_t>(buffer) * acc_columns;
+            if (!wait_barrier(acc_empty + buffer * 8, buffer_parity, a.error_flag)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int block = 0; block < blocks; block++) {
                 if (!wait_barrier(full + stage * 8, parity, a.error_flag)) {
@@ -461,21 +462,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) {
-                    const uint64_t a_stage = first + static_cast<uint64_t>(stage) * (stage_bytes >> 4), b_stage = a_stage + (a_bytes >> 4);
+                    const uint64_t a_stage = first + static_cast<uint64_t>(stage) * (stage_bytes >> 4), b_stage = a_stage + MATRICES * (a_bytes >> 4);
 #pragma unroll
-                    for (int step = 0; step < 4; step++) {  // K = 32 per instruction
-                        const uint32_t accumulate = (block > 0 || step > 0) ? 1u : 0u;
+                    for (int step = 0; step < 4 * MATRICES; step++) {  // K = 32 per instruction
+                        const int matrix = step >> 2, part = step & 3;
+                        const uint32_t accumulate = (block > 0 || part > 0) ? 1u : 0u;
                         asm volatile(
                             "{\n"
                             ".reg .pred p;\n"
                             "setp.ne.b32 p, %4, 0;\n"
                             "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
-                            "}\n" ::"r"(accumulator),
-                            "l"(a_stage + step * 2), "l"(b_stage + step * 2), "r"(instruction), "r"(accumulate)
+                            "}\n" ::"r"(accumulator + static_cast<uint32_t>(matrix * a.tile_lanes)),
+                            "l"(a_stage + matrix * (a_bytes >> 4) + part * 2), "l"(b_stage + part * 2), "r"(instruction), "r"(accumulate)
                             : "memory");
                     }
                     commit_to_pair(empty + stage * 8);
-                    if (block == blocks - 1) commit_to_pair(acc_full + (round & 1) * 8);
+                    if (block == blocks - 1) commit_to_pair(acc_full + buffer * 8);
                 }
                 __syncwarp();
                 if (++stage == a.stages) {
@@ -484,89 +486,113 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                 }
             }
             count = next;
+            if (++buffer == a.buffers) {
+                buffer = 0;
+                buffer_parity ^= 1;
+            }
         }
     } else if (warp >= 4) {  // ---- outputs: thread = row of the accumulator
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
-        const int quarter = warp & 3, part = (warp - 4) >> 2, thread = threadIdx.x - 128;
-        int round = 0;
-        Tile tile = pair < tiles ? tile_at<MODE>(a, pair, rank) : Tile{};
-        for (int index = pair; index < tiles; index += pairs, round++) {
-            const Tile next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, rank) : tile;
-            const bool mine = TWO || quarter * 32 < a.rows;
-            // the output channel of this thread, and its factor: a lane of a pair's upper half holds up's row of the same channel
-            const int channel = TWO ? tile.row0 + quarter * a.rows + (lane & 15) : tile.row0 + quarter * 32 + lane;
-            const bool in_range = channel < a.n && (TWO ? (lane & 15) < a.rows : quarter * 32 + lane < a.rows);
-            float factor = 0.0f;
-            if (in_range) {
-                if (MODE == LINEAR) factor = a.scales[channel];
-                else if (MODE == PAIR) factor = (lane < 16 ? a.scales : a.up_scales)[channel];
-                else if (MODE == EXPERTS_PAIR) factor = a.scales[static_cast<size_t>(tile.expert) * 2 * a.n + (lane < 16 ? 0 : a.n) + channel];
-                else factor = a.scales[static_cast<size_t>(tile.expert) * a.n + channel];
+        const int quarter = warp & 3, part = (warp - 4) >> 2, thread = threadIdx.x - 128, row = quarter * 32 + lane;
+        // what a tile's outputs take besides its sums; fetched a tile ahead
+        struct Extra {
+            float factor, up_factor, scale;
+            int to;
+        };
+        auto fetch = [&](const Tile &tile) {
+            Extra extra = {};
+            const int channel = tile.row0 + row;
+            if (row < a.rows && channel < a.n) {
+                const size_t at = (GROUPED ? static_cast<size_t>(tile.expert) * MATRICES * a.n : 0) + channel;
+                extra.factor = a.scales[at];
+                if (TWO) extra.up_factor = MODE == PAIR ? a.up_scales[at] : a.scales[at + a.n];
             }
-            LaneInfo &info = control.lanes[round & 1];  // (the sums of two tiles before are out: all passed the barrier of the last one)
             if (thread < tile.count) {
-                float scale = a.lane_scales[tile.lane0 + thread];
-                int to = tile.lane0 + thread;
-                if (MODE == EXPERTS_DOWN) {
-                    to = a.pair_of[to];
-                    scale = __fmul_rn(scale, a.weights_of[to]);
+                extra.scale = a.lane_scales[tile.lane0 + thread];
+                extra.to = MODE == EXPERTS_DOWN ? a.pair_of[tile.lane0 + thread] : tile.lane0 + thread;
+                if (MODE == LINEAR && a.residual != nullptr) {  // the tile's part of this lane's row, into L2
+                    const char *from = reinterpret_cast<const char *>(a.residual + static_cast<size_t>(extra.to) * a.n + tile.row0);
+                    for (int at = 0; at < 2 * min(a.rows, a.n - tile.row0); at += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + at));
                 }
-                info.scale[thread] = scale;
-                info.to[thread] = to;
             }
-            if (!all_of<1, 32 * OUTPUT_WARPS>(wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag))) break;
+            return extra;
+        };
+        int round = 0, buffer = 0;
+        uint32_t buffer_parity = 0;
+        Tile tile = {}, next = {};
+        Extra extra = {};
+        if (pair < tiles) {
+            tile = tile_at<MODE>(a, pair, rank);
+            if (pair + pairs < tiles) next = tile_at<MODE>(a, pair + pairs, rank);
+            extra = fetch(tile);
+        }
+        for (int index = pair; index < tiles; index += pairs, round++) {
+            LaneInfo &info = control.lanes[round & 1];  // (what stood there two tiles before is out: all threads have passed the last tile's barrier)
+            info.scale[thread] = extra.scale;
+            info.to[thread] = extra.to;
+            const float factor = extra.factor, up_factor = extra.up_factor;
+            if (!all_of<1, 32 * OUTPUT_WARPS>(wait_barrier(acc_full + buffer * 8, buffer_parity, a.error_flag))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t accumulator = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (round & 1) * acc_columns;
-            if (mine)
+            Tile after = {};
+            if (index + 2 * pairs < tiles) after = tile_at<MODE>(a, index + 2 * pairs, rank);
+            if (index + pairs < tiles) extra = fetch(next);
+            const uint32_t accumulator = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buffer) * acc_columns;
+            const int channel = tile.row0 + row;
+            const bool in_range = row < a.rows && channel < a.n;
+            if (quarter * 32 < a.rows) {
+                const uint16_t *residual = MODE == LINEAR ? a.residual : nullptr;
+                uint16_t beside[16];
+                auto fetch_beside = [&](int column) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (in_range && column + i < tile.count) beside[i] = residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel];
+                };
+                if (residual != nullptr) fetch_beside(part * 16);
                 for (int column = part * 16; column < tile.count; column += 32) {
-                    uint32_t d[16];
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]),
-                                   "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
-                                 : "r"(accumulator + static_cast<uint32_t>(column))
-                                 : "memory");
-                    const int count = min(16, tile.count - column);
-                    float residual[16];
-                    if (MODE == LINEAR && a.residual != nullptr)
+                    int sums[16], up_sums[16];
+                    load_sums(accumulator + static_cast<uint32_t>(column), sums);
+                    if (TWO) load_sums(accumulator + static_cast<uint32_t>(a.tile_lanes + column), up_sums);
+                    float scales[16];
+                    int to[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        *reinterpret_cast<float4 *>(scales + i) = *reinterpret_cast<const float4 *>(info.scale + column + i);
+                        *reinterpret_cast<int4 *>(to + i) = *reinterpret_cast<const int4 *>(info.to + column + i);
+                    }
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    float values[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        values[i] = scaled(sums[i], factor, scales[i]);
+                        if (TWO) values[i] = silu_product(values[i], scaled(up_sums[i], up_factor, scales[i]));
+                        if (MODE == LINEAR && residual != nullptr) values[i] = __fadd_rn(values[i], bf16_bits_to_f32(beside[i]));
+                    }
+                    if (residual != nullptr && column + 32 < tile.count) fetch_beside(column + 32);
+                    const bool f32 = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN || (MODE == LINEAR && a.to_f32);
+                    const int count = in_range ? tile.count - column : 0;
+                    if (f32) {
+                        float *const out = static_cast<float *>(a.y) + channel;
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                            if (in_range && i < count) residual[i] = bf16_bits_to_f32(a.residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel]);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (TWO) {
+                            if (i < count) out[static_cast<size_t>(to[i]) * a.n] = values[i];
+                    } else {
+                        uint16_t *const out = static_cast<uint16_t *>(a.y) + channel;
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {  // the warp's lower half finishes lane i, its upper half lane i + 1
-                            const float low = scaled(static_cast<int>(d[i]), factor, info.scale[column + i]);
-                            const float high = scaled(static_cast<int>(d[i + 1]), factor, info.scale[column + i + 1]);
-                            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? high : low, 16);
-                            const float product = lane < 16 ? silu_product(low, other) : silu_product(other, high);
-                            const int at = i + (lane >> 4);
-                            if (in_range && at < count) {
-                                const size_t out = static_cast<size_t>(tile.lane0 + column + at) * a.n + channel;
-                                if (MODE == PAIR) reinterpret_cast<uint16_t *>(a.y)[out] = to_bf16(product);
-                                else reinterpret_cast<float *>(a.y)[out] = product;
-                            }
-                        }
-                    } else if (in_range) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            if (i >= count) break;
-                            float value = scaled(static_cast<int>(d[i]), factor, info.scale[column + i]);
-                            const size_t out = static_cast<size_t>(MODE == EXPERTS_DOWN ? info.to[column + i] : tile.lane0 + column + i) * a.n + channel;
-                            if (MODE == EXPERTS_DOWN) {
-                                reinterpret_cast<float *>(a.y)[out] = value;
-                            } else {
-                                if (a.residual != nullptr) value = __fadd_rn(value, residual[i]);
-                                if (a.to_f32) reinterpret_cast<float *>(a.y)[out] = value;
-                                else reinterpret_cast<uint16_t *>(a.y)[out] = to_bf16(value);
-                            }
-                        }
+                        for (int i = 0; i < 16; i++)
+                            if (i < count) out[static_cast<size_t>(to[i]) * a.n] = to_bf16(values[i]);
                     }
                 }
+            }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) arrive_at(leader_acc_empty + (round & 1) * 8);
+            if (lane == 0) arrive_at(leader_acc_empty + buffer * 8);
             tile = next;
+            next = after;
+            if (++buffer == a.buffers) {
+                buffer = 0;
+                buffer_parity ^= 1;
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1054,11 +1080,14 @@ bool encode(CUtensorMap *map, const int8_t *matrix, int64_t rows, int k, int box
                                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// As many stages as fit, with room for an A operand of 128 rows at the last one's base.
-size_t stage_bytes(const Int8Args &args, bool pair) { return static_cast<size_t>((pair ? ROWS : (args.rows + 7) / 8 * 8) + args.tile_lanes / 2) * BLOCK_K; }
+// As many stages as fit, with room for an A operand of 128 rows at the last one's base; two accumulators where tensor memory
+// has room for them.
 size_t plan_stages(Int8Args &args, bool pair) {
-    const size_t stage = stage_bytes(args, pair), last = std::max(stage, static_cast<size_t>(ROWS) * BLOCK_K);
+    const int matrices = pair ? 2 : 1;
+    const size_t a_bytes = static_cast<size_t>((args.rows + 7) / 8 * 8) * BLOCK_K, stage = matrices * a_bytes + static_cast<size_t>(args.tile_lanes / 2) * BLOCK_K;
+    const size_t last = std::max(stage, (matrices - 1) * a_bytes + static_cast<size_t>(ROWS) * BLOCK_K);
     args.stages = static_cast<int>(std::min<size_t>(MAX_STAGES, 1 + (SMEM_LIMIT - GEMM_CONTROL - last) / stage));
+    args.buffers = 2 * matrices * args.tile_lanes <= 512 ? 2 : 1;
     return GEMM_CONTROL + static_cast<size_t>(args.stages - 1) * stage + last;
 }
 
@@ -1071,20 +1100,21 @@ cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
 }
 
 // Tiles of a matrix of n output channels (`pair`: two weight rows each) for that many lanes, by an estimate of the cycles
-// they take: of a block of 128 columns the tensor pipe needs half the lanes' number for each of four instructions, or as
-// long as it reads the weights, the copies arrive at some 56 bytes per cycle and multiprocessor, and the weights, which the first of a
-// row's tiles brings in, at some 23; and every tile has its start and end.
+// they take: of a block of 128 columns the tensor pipe needs half the lanes' number for each of four instructions a matrix
+// (the waits around them 310 at least), the copies arrive at some 56 bytes per cycle and multiprocessor, and the weights,
+// which the first of a row's tiles brings in, at some 23; and every tile has its start and end, outputs that no other tile's
+// sums hide (the last one's, and all of a pair's with one accumulator) among them.
 void plan_dense(Int8Args &args, bool pair) {
-    const int64_t pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K;
-    const int padded = (args.lanes + 31) / 32 * 32, least = (padded + MAX_LANES - 1) / MAX_LANES, most = pair ? 16 : 128;
+    const int64_t pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1;
+    const int padded = (args.lanes + 31) / 32 * 32, least = (padded + MAX_LANES - 1) / MAX_LANES;
     int64_t best = 0;
-    for (int split = least; split <= least + 3 && (split == least || padded / split >= 32); split++) {
+    for (int split = least; split <= 2 * least + 2 && (split == least || padded / split >= 32); split++) {
         const int lanes = ((padded + split - 1) / split + 31) / 32 * 32;
-        for (int rows = most; rows >= 1; rows -= rows > 32 ? 4 : 1) {
-            const int64_t outputs = 2 * rows * (pair ? 4 : 1), weight_rows = pair ? 8 * rows : rows, row_tiles = (args.n + outputs - 1) / outputs;
-            const int64_t lane_tiles = (padded + lanes - 1) / lanes, waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
-            const int64_t tensor = 4 * std::max(lanes / 2, 36), copies = (weight_rows + lanes / 2) * BLOCK_K / 56, memory = weight_rows * BLOCK_K / (23 * lane_tiles);
-            const int64_t cost = waves * (blocks * std::max({tensor, copies, memory}) + 1000);
+        for (int rows = ROWS; rows >= 1; rows -= rows > 32 ? 4 : 1) {
+            const int64_t row_tiles = (args.n + 2 * rows - 1) / (2 * rows), lane_tiles = (padded + lanes - 1) / lanes, waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
+            const int64_t tensor = matrices * std::max(2 * lanes, 310), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
+            const int64_t outputs = 12 * lanes * matrices, shown = 2 * matrices * lanes <= 512 ? 1 : waves;
+            const int64_t cost = waves * (blocks * std::max({tensor, copies, memory}) + 1000) + shown * outputs;
             if (best != 0 && cost >= best) continue;
             best = cost;
             args.rows = rows;
@@ -1093,7 +1123,6 @@ void plan_dense(Int8Args &args, bool pair) {
             args.lane_tiles = static_cast<int>(lane_tiles);
         }
     }
-    args.box_lanes = args.tile_lanes / 2;
 }
 
 }  // namespace
@@ -1165,12 +1194,12 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
         }
     }
     const Int8Rows rows(scratch, lanes, k);
-    const cudaError_t status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, lanes, 1, k, stream);
+    const cudaError_t status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream);
     if (status != cudaSuccess) return status;
     Int8Args args = {};
     args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
     plan_dense(args, TWO);
-    if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.box_lanes))
+    if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.tile_lanes / 2))
         return cudaErrorInvalidValue;
     args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
     return launch_gemm<MODE>(args, args.row_tiles * args.lane_tiles, stream);
@@ -1228,16 +1257,14 @@ struct ExpertsScratch {
 };
 
 // Tiles of the experts' products.  pairs: routes of the call, the most there can be.
-void plan_experts(Int8Args &args, int pairs, int experts, bool pair) {
+void plan_experts(Int8Args &args, int pairs, int experts) {
     // room for twice an expert's even share, so that most experts meet their weights once
     const int share = (pairs + experts - 1) / experts;
     int lanes = 32;
     while (lanes < 2 * share && lanes < MAX_LANES) lanes *= 2;
     args.tile_lanes = lanes;
-    args.box_lanes = std::min(lanes / 2, 32);
-    args.rows = pair ? 16 : 128;
-    const int outputs = pair ? 128 : 256;  // of a pair of CTAs
-    args.row_tiles = (args.n + outputs - 1) / outputs;
+    args.rows = ROWS;
+    args.row_tiles = (args.n + 2 * ROWS - 1) / (2 * ROWS);
 }
 
 }  // namespace
@@ -1277,15 +1304,15 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     Int8Args first = {}, second = {};
     first.n = inter, first.k = hidden;
     second.n = hidden, second.k = inter;
-    plan_experts(first, pairs, experts, true);
-    plan_experts(second, pairs, experts, false);
-    if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) || !encode(&first.activations, part.xq, pairs, hidden, first.box_lanes) ||
-        !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows) || !encode(&second.activations, part.hq, pairs, inter, second.box_lanes))
+    plan_experts(first, pairs, experts);
+    plan_experts(second, pairs, experts);
+    if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) || !encode(&first.activations, part.xq, pairs, hidden, first.tile_lanes / 2) ||
+        !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows) || !encode(&second.activations, part.hq, pairs, inter, second.tile_lanes / 2))
         return cudaErrorInvalidValue;
     first.scales = gate_up_scales, second.scales = down_scales;
     first.lane_scales = part.x_scales, second.lane_scales = part.h_scales;
     first.y = part.h, second.y = part.parts;
-    second.pair_of = part.pair_of, second.weights_of = weights;
+    second.pair_of = part.pair_of;
     for (Int8Args *args : {&first, &second}) {
         args->tiles = part.tiles;
         args->tile_count = part.counts;
@@ -1295,11 +1322,11 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     cudaError_t status = launch_dependent(expert_groups_kernel, dim3(1), dim3(GROUP_THREADS), 0, 1, stream, ids, pairs, experts, first.tile_lanes, part.tiles, part.counts,
                                           part.place_of, part.pair_of);
     if (status != cudaSuccess) return status;
-    status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, tokens, top_k, hidden, stream);
+    status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, nullptr, nullptr, tokens, top_k, hidden, stream);
     if (status != cudaSuccess) return status;
     status = launch_gemm<EXPERTS_PAIR>(first, most_tiles * first.row_tiles, stream);
     if (status != cudaSuccess) return status;
-    status = launch_quantise_rows<float, HeldF32, 2>(part.h, part.hq, part.h_scales, nullptr, part.counts + 1, pairs, 1, inter, stream);
+    status = launch_quantise_rows<float, HeldF32, 2>(part.h, part.hq, part.h_scales, nullptr, part.counts + 1, part.pair_of, weights, pairs, 1, inter, stream);
     if (status != cudaSuccess) return status;
     status = launch_gemm<EXPERTS_DOWN>(second, most_tiles * second.row_tiles, stream);
     return status != cudaSuccess ? status : sum();
