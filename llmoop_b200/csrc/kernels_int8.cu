@@ -99,10 +99,16 @@ __device__ __forceinline__ void copy_tile_of_pair(uint32_t target, const CUtenso
 __device__ __forceinline__ void commit_to_pair(uint32_t barrier) {  // that barrier of both CTAs
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier), "h"(static_cast<uint16_t>(3)) : "memory");
 }
-__device__ __forceinline__ void arrive_at(uint32_t barrier) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier) : "memory"); }
+// Relaxed: a release to the other CTA would first wait for this thread's stores to global memory (12000 cycles a tile where
+// the outputs took 500).  What it hands over are sums that have been read.
+__device__ __forceinline__ void arrive_at(uint32_t barrier) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier) : "memory"); }
 __device__ __forceinline__ void pair_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_end() {  // orders no memory
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 // Into L2, which later writes to the tile reach: safe ahead of the wait for the kernel in front, whatever that writes.
 __device__ __forceinline__ void prefetch_tile(const CUtensorMap *map, int column, int row) {
@@ -596,7 +602,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    pair_sync();  // neither CTA leaves while the other still reads its memory or reports to its barriers
+    pair_end();  // neither CTA leaves while the other still reads its memory or reports to its barriers
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
