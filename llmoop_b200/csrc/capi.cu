@@ -7,6 +7,7 @@
 
 #include "../../include/nerve_b200.h"
 #include "engine.hpp"
+#include "launch.cuh"
 #include "state_abi.hpp"
 #include "stream_runtime.hpp"
 
@@ -106,7 +107,6 @@ public:
     bool take_error() { return __atomic_exchange_n(host_word_, 0, __ATOMIC_ACQ_REL) != 0; }
 
 private:
-    static constexpr int MAX_DEVICES = 64;
     static OperatorDevice *all() {
         static OperatorDevice devices[MAX_DEVICES];
         return devices;

@@ -18,6 +18,10 @@
 // The experts' products are the same kernel over tiles that expert_groups_kernel makes of the routes.
 // Waits are bounded; a wait that expires sets the error word, and the CTA still frees its tensor memory.  The unbounded wait
 // for the kernel in front comes before them in every role, so none of them counts that kernel's time.
+//
+// No pointer here is __restrict__: what the kernel in front writes may only be read behind the wait for it, and a load through a
+// const __restrict__ pointer, which promises that nobody writes, is free to move in front of that (the routes of a replayed
+// graph were read before they were there).
 #include <cuda.h>
 
 #include <algorithm>
@@ -105,10 +109,6 @@ __device__ __forceinline__ void arrive_at(uint32_t barrier) { asm volatile("mbar
 __device__ __forceinline__ void pair_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void pair_end() {  // orders no memory
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 // Into L2, which later writes to the tile reach: safe ahead of the wait for the kernel in front, whatever that writes.
 __device__ __forceinline__ void prefetch_tile(const CUtensorMap *map, int column, int row) {
@@ -222,75 +222,82 @@ __device__ __forceinline__ uint4 quantise(const Held &held, const RowScale &row)
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// One CTA per row of x, which its threads hold in registers, HELD times sixteen values each; what is wider is read again,
-// from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once to the place of each
-// of its top_k routes, where it has one.  With weights the scale is that of row times its route's weight.  Bound by DRAM for large batches, by the chain of loads, barrier and stores for small
-// ones.
+// A row of x is one CTA's, or one warp's (WARP), whose threads hold it in registers, HELD times sixteen values each; what is
+// wider is read again, from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once
+// to the place of each of its top_k routes, where it has one.  With weights the scale is that of the row times its route's weight.
+// Bound by DRAM for large batches, by the chain of loads, barrier and stores for small ones.
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.
-template <typename T, typename Held, int HELD>
-__global__ void __launch_bounds__(512) quantise_rows_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__restrict__ scales, const int *__restrict__ places,
-                                                            const int *__restrict__ row_count, const int *__restrict__ pair_of, const float *__restrict__ weights, int top_k, int k,
-                                                            int wide) {
+template <typename T, typename Held, int HELD, bool WARP>
+__global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *q, float *scales, const int *places,
+                                                            const int *row_count, const int *pair_of, const float *weights, int rows,
+                                                            int top_k, int k, int wide) {
     __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
-    if (row_count != nullptr && static_cast<int>(blockIdx.x) >= *row_count) return;
-    const T *row = x + static_cast<size_t>(blockIdx.x) * k;
-    const int step = blockDim.x * 16;
+    const int at_row = WARP ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
+    if (row_count != nullptr) rows = *row_count;
+    if (at_row >= rows) return;
+    const T *row = x + static_cast<size_t>(at_row) * k;
+    const int step = (WARP ? 32 : static_cast<int>(blockDim.x)) * 16, first = static_cast<int>(WARP ? threadIdx.x & 31 : threadIdx.x) * 16;
     Held held[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; i++)
-        if (static_cast<int>(threadIdx.x) * 16 + i * step < k) held[i].load(row, threadIdx.x * 16 + i * step, wide);
+        if (first + i * step < k) held[i].load(row, first + i * step, wide);
     uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < HELD; i++)
-        if (static_cast<int>(threadIdx.x) * 16 + i * step < k) amax = max(amax, held[i].amax());
-    for (int at = threadIdx.x * 16 + HELD * step; at < k; at += step) {
+        if (first + i * step < k) amax = max(amax, held[i].amax());
+    for (int at = first + HELD * step; at < k; at += step) {
         Held more;
         more.load(row, at, wide);
         amax = max(amax, more.amax());
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = amax;
-    __syncthreads();
-    for (int warp = 0; warp < static_cast<int>(blockDim.x >> 5); warp++) amax = max(amax, warps[warp]);
+    if (!WARP) {
+        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = amax;
+        __syncthreads();
+        for (int warp = 0; warp < static_cast<int>(blockDim.x >> 5); warp++) amax = max(amax, warps[warp]);
+    }
     const RowScale scale = row_scale(amax);
     const int copies = places != nullptr ? top_k : 1;
-    const int *own_places = places + (places != nullptr ? static_cast<size_t>(blockIdx.x) * top_k : 0);
+    const int *own_places = places + (places != nullptr ? static_cast<size_t>(at_row) * top_k : 0);
     auto store = [&](int at, const Held &values) {
         const uint4 packed = quantise(values, scale);
         for (int copy = 0; copy < copies; copy++) {
-            const int place = places != nullptr ? own_places[copy] : static_cast<int>(blockIdx.x);
+            const int place = places != nullptr ? own_places[copy] : at_row;
             if (place >= 0) *reinterpret_cast<uint4 *>(q + static_cast<size_t>(place) * k + at) = packed;
         }
     };
 #pragma unroll
     for (int i = 0; i < HELD; i++)
-        if (static_cast<int>(threadIdx.x) * 16 + i * step < k) store(threadIdx.x * 16 + i * step, held[i]);
-    for (int at = threadIdx.x * 16 + HELD * step; at < k; at += step) {
+        if (first + i * step < k) store(first + i * step, held[i]);
+    for (int at = first + HELD * step; at < k; at += step) {
         Held more;
         more.load(row, at, wide);
         store(at, more);
     }
-    for (int copy = threadIdx.x; copy < copies; copy += blockDim.x) {
-        const int place = places != nullptr ? own_places[copy] : static_cast<int>(blockIdx.x);
+    for (int copy = first / 16; copy < copies; copy += step / 16) {
+        const int place = places != nullptr ? own_places[copy] : at_row;
         if (place >= 0) scales[place] = weights != nullptr ? __fmul_rn(scale.scale, weights[pair_of[place]]) : scale.scale;
     }
 }
 
-// The rows are cut so that a thread holds its part of up to 32768 columns (bf16) or 16384 (f32), with as many threads as
-// sixteen columns each ask for up to 256, then more columns each.
+// Rows of up to 1024 columns of which there are more than the chip has warps to wait with are a warp's each (16384 rows of 768
+// f32 values: 20 us with a CTA each, 12 with a warp).  Otherwise as many threads as sixteen columns each ask for up to 256, then
+// more columns each.
 template <typename T, typename Held, int MOST>
 cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, const int *pair_of, const float *weights, int rows, int top_k,
                                  int k, cudaStream_t stream) {
     const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    auto with = [&](auto kernel, int held) {
-        const int threads = std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
-        return launch_dependent(kernel, dim3(rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, pair_of, weights, top_k, k, wide);
+    auto with = [&](auto kernel, int held, int warp_rows) {
+        const int threads = warp_rows != 0 ? 32 * warp_rows : std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
+        return launch_dependent(kernel, dim3(warp_rows != 0 ? (rows + warp_rows - 1) / warp_rows : rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, pair_of,
+                                weights, rows, top_k, k, wide);
     };
-    if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1>, 1);
-    if (parts <= 1024 || MOST == 2) return with(quantise_rows_kernel<T, Held, 2>, 2);
-    return with(quantise_rows_kernel<T, Held, MOST>, MOST);
+    if (parts <= 64 && rows >= 1024) return with(quantise_rows_kernel<T, Held, 2, true>, 2, 8);
+    if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1, false>, 1, 0);
+    if (parts <= 1024 || MOST == 2) return with(quantise_rows_kernel<T, Held, 2, false>, 2, 0);
+    return with(quantise_rows_kernel<T, Held, MOST, false>, MOST, 0);
 }
 
 // ---- the product
@@ -445,6 +452,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             }
             tile = next;
         }
+        // the MMAs' reports on the last stages are in before this CTA's barriers go
+        for (int s = 0; alive && s < a.stages && s < issued; s++) {
+            const int which = (issued - 1 - s) % a.stages;
+            alive = wait_barrier(empty + which * 8, static_cast<uint32_t>(((issued - 1 - s) / a.stages) & 1), a.error_flag);
+        }
     } else if (warp == 1) {  // ---- MMAs, by the first CTA for both
         const uint64_t first = swizzled_descriptor(base);
         int stage = 0, buffer = 0;
@@ -548,13 +560,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             const bool in_range = row < a.rows && channel < a.n;
             if (quarter * 32 < a.rows) {
                 const uint16_t *residual = MODE == LINEAR ? a.residual : nullptr;
-                uint16_t beside[16];
-                auto fetch_beside = [&](int column) {
+                uint16_t beside[2][16];  // of this step and the next
+                auto fetch_beside = [&](uint16_t(&to)[16], int column) {
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                        if (in_range && column + i < tile.count) beside[i] = residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel];
+                        if (in_range && column + i < tile.count) to[i] = residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel];
                 };
-                if (residual != nullptr) fetch_beside(part * 16);
+                if (residual != nullptr) fetch_beside(beside[0], part * 16), fetch_beside(beside[1], part * 16 + 32);
                 for (int column = part * 16; column < tile.count; column += 32) {
                     int sums[16], up_sums[16];
                     load_sums(accumulator + static_cast<uint32_t>(column), sums);
@@ -572,9 +584,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                     for (int i = 0; i < 16; i++) {
                         values[i] = scaled(sums[i], factor, scales[i]);
                         if (TWO) values[i] = silu_product(values[i], scaled(up_sums[i], up_factor, scales[i]));
-                        if (MODE == LINEAR && residual != nullptr) values[i] = __fadd_rn(values[i], bf16_bits_to_f32(beside[i]));
+                        if (MODE == LINEAR && residual != nullptr) {
+                            values[i] = __fadd_rn(values[i], bf16_bits_to_f32(beside[0][i]));
+                            beside[0][i] = beside[1][i];
+                        }
                     }
-                    if (residual != nullptr && column + 32 < tile.count) fetch_beside(column + 32);
+                    if (residual != nullptr) fetch_beside(beside[1], column + 64);
                     const bool f32 = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN || (MODE == LINEAR && a.to_f32);
                     const int count = in_range ? tile.count - column : 0;
                     if (f32) {
@@ -602,7 +617,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    pair_end();  // neither CTA leaves while the other still reads its memory or reports to its barriers
+    pair_sync();  // neither CTA leaves while the other still reads its memory or reports to its barriers: the release waits for those reports
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
@@ -993,9 +1008,10 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
 
 // One CTA counts the routes of every expert, gives each a place behind those of the experts before it, and cuts every
 // expert's places into tiles of tile_lanes.  Which of an expert's routes comes first is left to chance: a row's result does
-// not depend on its place.  Routes to no expert (ids outside 0..experts-1) get place -1.
-constexpr int GROUP_THREADS = 1024;  // and the most experts
-__global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int *__restrict__ ids, int pairs, int experts, int tile_lanes, int4 *tiles, int *counts_out,
+// not depend on its place.  Routes to no expert (ids outside 0..experts-1) get place -1.  A thread holds GROUP_HELD routes from
+// one pass to the other, all requested together (one after the other, 16384 routes: 14 us).
+constexpr int GROUP_THREADS = 1024, GROUP_HELD = 16;  // threads: and the most experts
+__global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int *ids, int pairs, int experts, int tile_lanes, int4 *tiles, int *counts_out,
                                                                       int *place_of, int *pair_of) {
     __shared__ int count[GROUP_THREADS], cursor[GROUP_THREADS], warp_places[32], warp_tiles[32];
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
@@ -1003,9 +1019,15 @@ __global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int 
     grid_launch_dependents();
     __syncthreads();
     grid_dependency_wait();
-    for (int pair = thread; pair < pairs; pair += GROUP_THREADS) {
+    int held[GROUP_HELD];
+#pragma unroll
+    for (int i = 0; i < GROUP_HELD; i++) held[i] = thread + i * GROUP_THREADS < pairs ? ids[thread + i * GROUP_THREADS] : -1;
+#pragma unroll
+    for (int i = 0; i < GROUP_HELD; i++)
+        if (static_cast<uint32_t>(held[i]) < static_cast<uint32_t>(experts)) atomicAdd(&count[held[i]], 1);
+    for (int pair = thread + GROUP_HELD * GROUP_THREADS; pair < pairs; pair += GROUP_THREADS) {
         const int expert = ids[pair];
-        if (expert >= 0 && expert < experts) atomicAdd(&count[expert], 1);
+        if (static_cast<uint32_t>(expert) < static_cast<uint32_t>(experts)) atomicAdd(&count[expert], 1);
     }
     __syncthreads();
     // thread = expert: places and tiles in front of it
@@ -1023,19 +1045,22 @@ __global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int 
     cursor[thread] = places;
     for (int i = 0; i < own_tiles; i++) tiles[tile + i] = make_int4(thread, places + i * tile_lanes, min(tile_lanes, own - i * tile_lanes), 0);
     __syncthreads();
-    for (int pair = thread; pair < pairs; pair += GROUP_THREADS) {
-        const int expert = ids[pair];
-        int place = -1;
-        if (expert >= 0 && expert < experts) {
-            place = atomicAdd(&cursor[expert], 1);
-            pair_of[place] = pair;
+    auto place = [&](int pair, int expert) {
+        int at = -1;
+        if (static_cast<uint32_t>(expert) < static_cast<uint32_t>(experts)) {
+            at = atomicAdd(&cursor[expert], 1);
+            pair_of[at] = pair;
         }
-        place_of[pair] = place;
-    }
+        place_of[pair] = at;
+    };
+#pragma unroll
+    for (int i = 0; i < GROUP_HELD; i++)
+        if (thread + i * GROUP_THREADS < pairs) place(thread + i * GROUP_THREADS, held[i]);
+    for (int pair = thread + GROUP_HELD * GROUP_THREADS; pair < pairs; pair += GROUP_THREADS) place(pair, ids[pair]);
 }
 
 // y[token] = the sum of its routes' weighted rows, in their order (+ residual), rounded once.  Four columns to a thread.
-__global__ void experts_sum_kernel(const float *__restrict__ parts, const int *__restrict__ ids, const uint16_t *residual, uint16_t *y, int top_k, int experts, int hidden,
+__global__ void experts_sum_kernel(const float *parts, const int *ids, const uint16_t *residual, uint16_t *y, int top_k, int experts, int hidden,
                                    int wide) {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -1100,7 +1125,7 @@ size_t plan_stages(Int8Args &args, bool pair) {
 template <Mode MODE>
 cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
     const size_t bytes = plan_stages(args, MODE == PAIR || MODE == EXPERTS_PAIR);
-    const cudaError_t status = cudaFuncSetAttribute(int8_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM_LIMIT));
+    const cudaError_t status = allow_shared_memory<int8_gemm_kernel<MODE>>(SMEM_LIMIT);
     if (status != cudaSuccess) return status;
     return launch_dependent(int8_gemm_kernel<MODE>, dim3(2 * std::min(most_tiles, multiprocessors() / 2)), dim3(THREADS), bytes, 1, stream, args);
 }
@@ -1169,7 +1194,7 @@ bool plan_stages(StreamArgs &args, int tiles, bool two_buffers, size_t tables, s
 }
 template <Mode MODE>
 cudaError_t launch_stream(const StreamArgs &args, int tiles, size_t bytes, cudaStream_t stream) {
-    const cudaError_t status = cudaFuncSetAttribute(int8_stream_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM_LIMIT));
+    const cudaError_t status = allow_shared_memory<int8_stream_kernel<MODE>>(SMEM_LIMIT);
     if (status != cudaSuccess) return status;
     return launch_dependent(int8_stream_kernel<MODE>, dim3(std::min(tiles, multiprocessors())), dim3(STREAM_THREADS), bytes, 1, stream, args);
 }
@@ -1263,14 +1288,27 @@ struct ExpertsScratch {
 };
 
 // Tiles of the experts' products.  pairs: routes of the call, the most there can be.
-void plan_experts(Int8Args &args, int pairs, int experts) {
-    // room for twice an expert's even share, so that most experts meet their weights once
+int expert_tile_lanes(int pairs, int experts) {  // room for twice an expert's even share, so that most experts meet their weights once
     const int share = (pairs + experts - 1) / experts;
     int lanes = 32;
     while (lanes < 2 * share && lanes < MAX_LANES) lanes *= 2;
-    args.tile_lanes = lanes;
-    args.rows = ROWS;
-    args.row_tiles = (args.n + 2 * ROWS - 1) / (2 * ROWS);
+    return lanes;
+}
+// As plan_dense, for as many lane tiles as there are experts, each with its even share.
+void plan_experts(Int8Args &args, int pairs, int experts, bool pair) {
+    args.tile_lanes = expert_tile_lanes(pairs, experts);
+    const int64_t count = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1, tiles = std::min(experts, pairs),
+                  share = (pairs / tiles + 31) / 32 * 32;
+    int64_t best = 0;
+    for (int rows = ROWS; rows >= 16; rows -= 4) {
+        const int64_t row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * tiles + count - 1) / count;
+        const int64_t tensor = matrices * std::max<int64_t>(2 * share, 310), copies = (matrices * rows + args.tile_lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / 23;
+        const int64_t cost = waves * (blocks * std::max({tensor, copies, memory}) + 1000);
+        if (best != 0 && cost >= best) continue;
+        best = cost;
+        args.rows = rows;
+        args.row_tiles = static_cast<int>(row_tiles);
+    }
 }
 
 }  // namespace
@@ -1310,8 +1348,8 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     Int8Args first = {}, second = {};
     first.n = inter, first.k = hidden;
     second.n = hidden, second.k = inter;
-    plan_experts(first, pairs, experts);
-    plan_experts(second, pairs, experts);
+    plan_experts(first, pairs, experts, true);
+    plan_experts(second, pairs, experts, false);
     if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) || !encode(&first.activations, part.xq, pairs, hidden, first.tile_lanes / 2) ||
         !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows) || !encode(&second.activations, part.hq, pairs, inter, second.tile_lanes / 2))
         return cudaErrorInvalidValue;

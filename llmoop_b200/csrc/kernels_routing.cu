@@ -9,7 +9,8 @@
 // All of it is held in 64 bits: experts next to one another are told apart as the definition does, not by what the last bit
 // of an exponential made of them.
 //
-// One warp per token, expert e with thread e % 32.
+// One warp per token, expert e with thread e % 32.  (No pointer is __restrict__: loads through those may move in front of the wait
+// for the kernel that writes the logits.)
 #include "common.cuh"
 #include "kernels.cuh"
 #include "launch.cuh"
@@ -39,8 +40,8 @@ __device__ __forceinline__ double value_of(uint64_t key) {  // of a key above 0
 constexpr int TOKENS_PER_CTA = 4;
 
 template <typename T, int PER_THREAD>
-__global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(const T *__restrict__ logits, const float *__restrict__ bias, int *__restrict__ ids,
-                                                                            float *__restrict__ weights, int tokens, Routing routing) {
+__global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(const T *logits, const float *bias, int *ids,
+                                                                            float *weights, int tokens, Routing routing) {
     grid_launch_dependents();
     grid_dependency_wait();
     const int token = blockIdx.x * TOKENS_PER_CTA + (threadIdx.x >> 5), lane = threadIdx.x & 31;
