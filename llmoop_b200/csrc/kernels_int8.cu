@@ -224,13 +224,14 @@ __device__ __forceinline__ uint4 quantise(const Held &held, const RowScale &row)
 
 // A row of x is one CTA's, or one warp's (WARP), whose threads hold it in registers, HELD times sixteen values each; what is
 // wider is read again, from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once
-// to the place of each of its top_k routes, where it has one.  With weights the scale is that of the row times its route's weight.
+// to the place of each of its top_k routes, where it has one, and leaves there which route that is (a store of its own for every
+// route, which expert_groups_kernel's one CTA would take 8 us for).  With weights the scale is that of the row times its route's weight.
 // Bound by DRAM for large batches, by the chain of loads, barrier and stores for small ones.
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.
 template <typename T, typename Held, int HELD, bool WARP>
 __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *q, float *scales, const int *places,
-                                                            const int *row_count, const int *pair_of, const float *weights, int rows,
-                                                            int top_k, int k, int wide) {
+                                                            const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
+                                                            int k, int wide) {
     __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
@@ -278,7 +279,9 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
     }
     for (int copy = first / 16; copy < copies; copy += step / 16) {
         const int place = places != nullptr ? own_places[copy] : at_row;
-        if (place >= 0) scales[place] = weights != nullptr ? __fmul_rn(scale.scale, weights[pair_of[place]]) : scale.scale;
+        if (place < 0) continue;
+        scales[place] = weights != nullptr ? __fmul_rn(scale.scale, weights[pair_of[place]]) : scale.scale;
+        if (places != nullptr) pair_of[place] = at_row * top_k + copy;
     }
 }
 
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 // f32 values: 20 us with a CTA each, 12 with a warp).  Otherwise as many threads as sixteen columns each ask for up to 256, then
 // more columns each.
 template <typename T, typename Held, int MOST>
-cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, const int *pair_of, const float *weights, int rows, int top_k,
+cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
                                  int k, cudaStream_t stream) {
     const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto with = [&](auto kernel, int held, int warp_rows) {
@@ -1008,55 +1011,63 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
 
 // One CTA counts the routes of every expert, gives each a place behind those of the experts before it, and cuts every
 // expert's places into tiles of tile_lanes.  Which of an expert's routes comes first is left to chance: a row's result does
-// not depend on its place.  Routes to no expert (ids outside 0..experts-1) get place -1.  A thread holds GROUP_HELD routes from
-// one pass to the other, all requested together (one after the other, 16384 routes: 14 us).
+// not depend on its place.  Routes to no expert (ids outside 0..experts-1) get place -1.  A thread holds GROUP_HELD routes and
+// their ranks among their expert's.
 constexpr int GROUP_THREADS = 1024, GROUP_HELD = 16;  // threads: and the most experts
 __global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int *ids, int pairs, int experts, int tile_lanes, int4 *tiles, int *counts_out,
-                                                                      int *place_of, int *pair_of) {
-    __shared__ int count[GROUP_THREADS], cursor[GROUP_THREADS], warp_places[32], warp_tiles[32];
+                                                                      int *place_of) {
+    __shared__ int count[GROUP_THREADS], later[GROUP_THREADS], first[GROUP_THREADS], warp_places[32], warp_tiles[32];
     const int thread = threadIdx.x, warp = thread >> 5, lane = thread & 31;
     count[thread] = 0;
+    later[thread] = 0;
     grid_launch_dependents();
     __syncthreads();
     grid_dependency_wait();
-    int held[GROUP_HELD];
+    int held[GROUP_HELD], rank[GROUP_HELD];
 #pragma unroll
     for (int i = 0; i < GROUP_HELD; i++) held[i] = thread + i * GROUP_THREADS < pairs ? ids[thread + i * GROUP_THREADS] : -1;
+    auto routed = [&](int expert) { return static_cast<uint32_t>(expert) < static_cast<uint32_t>(experts); };
 #pragma unroll
-    for (int i = 0; i < GROUP_HELD; i++)
-        if (static_cast<uint32_t>(held[i]) < static_cast<uint32_t>(experts)) atomicAdd(&count[held[i]], 1);
-    for (int pair = thread + GROUP_HELD * GROUP_THREADS; pair < pairs; pair += GROUP_THREADS) {
+    for (int i = 0; i < GROUP_HELD; i++) rank[i] = routed(held[i]) ? atomicAdd(&count[held[i]], 1) : 0;
+    for (int pair = thread + GROUP_HELD * GROUP_THREADS; pair < pairs; pair += GROUP_THREADS) {  // these are ranked behind the others
         const int expert = ids[pair];
-        if (static_cast<uint32_t>(expert) < static_cast<uint32_t>(experts)) atomicAdd(&count[expert], 1);
+        if (routed(expert)) atomicAdd(&later[expert], 1);
     }
     __syncthreads();
     // thread = expert: places and tiles in front of it
-    const int own = count[thread], own_tiles = (own + tile_lanes - 1) / tile_lanes;
+    const int own = count[thread] + later[thread], own_tiles = (own + tile_lanes - 1) / tile_lanes;
     int places = own, tile = own_tiles;
-    for (int offset = 1; offset < 32; offset *= 2) {
-        const int p = __shfl_up_sync(0xffffffffu, places, offset), t = __shfl_up_sync(0xffffffffu, tile, offset);
-        if (lane >= offset) places += p, tile += t;
-    }
+    auto scan = [&](int &p, int &t) {  // inclusive, of a warp
+        for (int offset = 1; offset < 32; offset *= 2) {
+            const int other_p = __shfl_up_sync(0xffffffffu, p, offset), other_t = __shfl_up_sync(0xffffffffu, t, offset);
+            if (lane >= offset) p += other_p, t += other_t;
+        }
+    };
+    scan(places, tile);
     if (lane == 31) warp_places[warp] = places, warp_tiles[warp] = tile;
     __syncthreads();
-    for (int before = 0; before < warp; before++) places += warp_places[before], tile += warp_tiles[before];
+    int front_places = warp_places[lane], front_tiles = warp_tiles[lane];
+    scan(front_places, front_tiles);
+    if (warp > 0) {
+        places += __shfl_sync(0xffffffffu, front_places, warp - 1);
+        tile += __shfl_sync(0xffffffffu, front_tiles, warp - 1);
+    }
     if (thread == GROUP_THREADS - 1) counts_out[0] = tile, counts_out[1] = places;
     places -= own, tile -= own_tiles;
-    cursor[thread] = places;
+    first[thread] = places;
+    later[thread] = places + count[thread];
     for (int i = 0; i < own_tiles; i++) tiles[tile + i] = make_int4(thread, places + i * tile_lanes, min(tile_lanes, own - i * tile_lanes), 0);
     __syncthreads();
-    auto place = [&](int pair, int expert) {
-        int at = -1;
-        if (static_cast<uint32_t>(expert) < static_cast<uint32_t>(experts)) {
-            at = atomicAdd(&cursor[expert], 1);
-            pair_of[at] = pair;
-        }
-        place_of[pair] = at;
-    };
 #pragma unroll
-    for (int i = 0; i < GROUP_HELD; i++)
-        if (thread + i * GROUP_THREADS < pairs) place(thread + i * GROUP_THREADS, held[i]);
-    for (int pair = thread + GROUP_HELD * GROUP_THREADS; pair < pairs; pair += GROUP_THREADS) place(pair, ids[pair]);
+    for (int i = 0; i < GROUP_HELD; i++) {
+        const int pair = thread + i * GROUP_THREADS;
+        if (pair >= pairs) break;
+        place_of[pair] = routed(held[i]) ? first[held[i]] + rank[i] : -1;
+    }
+    for (int pair = thread + GROUP_HELD * GROUP_THREADS; pair < pairs; pair += GROUP_THREADS) {
+        const int expert = ids[pair];
+        place_of[pair] = routed(expert) ? atomicAdd(&later[expert], 1) : -1;
+    }
 }
 
 // y[token] = the sum of its routes' weighted rows, in their order (+ residual), rounded once.  Four columns to a thread.
@@ -1364,9 +1375,9 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     }
     const int most_tiles = pairs / first.tile_lanes + std::min(experts, pairs);
     cudaError_t status = launch_dependent(expert_groups_kernel, dim3(1), dim3(GROUP_THREADS), 0, 1, stream, ids, pairs, experts, first.tile_lanes, part.tiles, part.counts,
-                                          part.place_of, part.pair_of);
+                                          part.place_of);
     if (status != cudaSuccess) return status;
-    status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, nullptr, nullptr, tokens, top_k, hidden, stream);
+    status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, part.pair_of, nullptr, tokens, top_k, hidden, stream);
     if (status != cudaSuccess) return status;
     status = launch_gemm<EXPERTS_PAIR>(first, most_tiles * first.row_tiles, stream);
     if (status != cudaSuccess) return status;
