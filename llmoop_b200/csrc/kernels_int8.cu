@@ -313,7 +313,7 @@ struct Int8Args {
     int lanes, n, k, to_f32;
     int *error_flag;
     int rows;  // output channels of a CTA's tile
-    int tile_lanes, lane_tiles, row_tiles, stages, buffers;
+    int tile_lanes, lane_tiles, row_tiles, stages;
     // experts
     const int4 *tiles;
     const int *tile_count, *pair_of;
@@ -398,10 +398,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // one accumulator: the sums of the tile's lanes, gate's and then up's
-    const uint32_t acc_columns = static_cast<uint32_t>(MATRICES * a.tile_lanes);
+    // An accumulator: the sums of the tile's lanes, in steps of 32, gate's and then up's.  Those of the CTA's even tiles lie at the
+    // front of tensor memory, of its odd ones at the back: where two successive ones have room beside one another, the outputs of
+    // the one are written while the other fills.
     uint32_t columns = 32;
-    while (columns < static_cast<uint32_t>(a.buffers) * acc_columns) columns *= 2;
+    while (columns < static_cast<uint32_t>(2 * MATRICES * a.tile_lanes) && columns < 512) columns *= 2;
+    auto width_of = [&](int count) { return static_cast<uint32_t>(MATRICES * ((count + 31) / 32 * 32)); };
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tmem)), "r"(columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -462,19 +464,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
     } else if (warp == 1) {  // ---- MMAs, by the first CTA for both
         const uint64_t first = swizzled_descriptor(base);
-        int stage = 0, buffer = 0;
-        uint32_t parity = 0, buffer_parity = 1;
+        int stage = 0, round = 0;
+        uint32_t parity = 0, last_width = 0;
         bool alive = rank == 0;
         grid_dependency_wait();
         const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
         int count = alive && pair < tiles ? tile_at<MODE>(a, pair, 0).count : 0;
-        for (int index = pair; index < tiles && alive; index += pairs) {
+        for (int index = pair; index < tiles && alive; index += pairs, round++) {
             const int next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, 0).count : 0;
             // instruction descriptor: s32 accumulator, A and B signed bytes, both K-major, N / 8 in bits 17-22, M / 16 in bits 24-28
             // (M = 256 with bytes: N in steps of 32)
-            const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>((count + 31) / 32 * 4) << 17) | (16u << 24));
-            const uint32_t accumulator = tmem + static_cast<uint32_t>(buffer) * acc_columns;
-            if (!wait_barrier(acc_empty + buffer * 8, buffer_parity, a.error_flag)) break;
+            const uint32_t lanes = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>((count + 31) / 32 * 32)), width = MATRICES * lanes;
+            const uint32_t instruction = (2u << 4) | (1u << 7) | (1u << 10) | (lanes / 8 << 17) | (16u << 24);
+            const uint32_t accumulator = tmem + ((round & 1) != 0 ? columns - width : 0u);
+            if (!wait_barrier(acc_empty + (round & 1) * 8, static_cast<uint32_t>((round / 2 + 1) & 1), a.error_flag)) break;
+            if (width + last_width > columns && !wait_barrier(acc_empty + ((round - 1) & 1) * 8, static_cast<uint32_t>(((round - 1) / 2) & 1), a.error_flag)) break;
+            last_width = width;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int block = 0; block < blocks; block++) {
                 if (!wait_barrier(full + stage * 8, parity, a.error_flag)) {
@@ -493,12 +498,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                             ".reg .pred p;\n"
                             "setp.ne.b32 p, %4, 0;\n"
                             "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
-                            "}\n" ::"r"(accumulator + static_cast<uint32_t>(matrix * a.tile_lanes)),
+                            "}\n" ::"r"(accumulator + matrix * lanes),
                             "l"(a_stage + matrix * (a_bytes >> 4) + part * 2), "l"(b_stage + part * 2), "r"(instruction), "r"(accumulate)
                             : "memory");
                     }
                     commit_to_pair(empty + stage * 8);
-                    if (block == blocks - 1) commit_to_pair(acc_full + buffer * 8);
+                    if (block == blocks - 1) commit_to_pair(acc_full + (round & 1) * 8);
                 }
                 __syncwarp();
                 if (++stage == a.stages) {
@@ -507,10 +512,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                 }
             }
             count = next;
-            if (++buffer == a.buffers) {
-                buffer = 0;
-                buffer_parity ^= 1;
-            }
         }
     } else if (warp >= 4) {  // ---- outputs: thread = row of the accumulator
         grid_dependency_wait();
@@ -539,8 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             }
             return extra;
         };
-        int round = 0, buffer = 0;
-        uint32_t buffer_parity = 0;
+        int round = 0;
         Tile tile = {}, next = {};
         Extra extra = {};
         if (pair < tiles) {
@@ -553,12 +553,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             info.scale[thread] = extra.scale;
             info.to[thread] = extra.to;
             const float factor = extra.factor, up_factor = extra.up_factor;
-            if (!all_of<1, 32 * OUTPUT_WARPS>(wait_barrier(acc_full + buffer * 8, buffer_parity, a.error_flag))) break;
+            if (!all_of<1, 32 * OUTPUT_WARPS>(wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             Tile after = {};
             if (index + 2 * pairs < tiles) after = tile_at<MODE>(a, index + 2 * pairs, rank);
             if (index + pairs < tiles) extra = fetch(next);
-            const uint32_t accumulator = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buffer) * acc_columns;
+            const uint32_t width = width_of(tile.count), accumulator = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + ((round & 1) != 0 ? columns - width : 0u);
             const int channel = tile.row0 + row;
             const bool in_range = row < a.rows && channel < a.n;
             if (quarter * 32 < a.rows) {
@@ -573,7 +573,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                 for (int column = part * 16; column < tile.count; column += 32) {
                     int sums[16], up_sums[16];
                     load_sums(accumulator + static_cast<uint32_t>(column), sums);
-                    if (TWO) load_sums(accumulator + static_cast<uint32_t>(a.tile_lanes + column), up_sums);
+                    if (TWO) load_sums(accumulator + width / 2 + static_cast<uint32_t>(column), up_sums);
                     float scales[16];
                     int to[16];
 #pragma unroll
@@ -610,13 +610,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) arrive_at(leader_acc_empty + buffer * 8);
+            if (lane == 0) arrive_at(leader_acc_empty + (round & 1) * 8);
             tile = next;
             next = after;
-            if (++buffer == a.buffers) {
-                buffer = 0;
-                buffer_parity ^= 1;
-            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1122,14 +1118,12 @@ bool encode(CUtensorMap *map, const int8_t *matrix, int64_t rows, int k, int box
                                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// As many stages as fit, with room for an A operand of 128 rows at the last one's base; two accumulators where tensor memory
-// has room for them.
+// As many stages as fit, with room for an A operand of 128 rows at the last one's base.
 size_t plan_stages(Int8Args &args, bool pair) {
     const int matrices = pair ? 2 : 1;
     const size_t a_bytes = static_cast<size_t>((args.rows + 7) / 8 * 8) * BLOCK_K, stage = matrices * a_bytes + static_cast<size_t>(args.tile_lanes / 2) * BLOCK_K;
     const size_t last = std::max(stage, (matrices - 1) * a_bytes + static_cast<size_t>(ROWS) * BLOCK_K);
     args.stages = static_cast<int>(std::min<size_t>(MAX_STAGES, 1 + (SMEM_LIMIT - GEMM_CONTROL - last) / stage));
-    args.buffers = 2 * matrices * args.tile_lanes <= 512 ? 2 : 1;
     return GEMM_CONTROL + static_cast<size_t>(args.stages - 1) * stage + last;
 }
 
@@ -1299,10 +1293,12 @@ struct ExpertsScratch {
 };
 
 // Tiles of the experts' products.  pairs: routes of the call, the most there can be.
-int expert_tile_lanes(int pairs, int experts) {  // room for twice an expert's even share, so that most experts meet their weights once
+// Room for twice an expert's even share, so that most experts meet their weights once, as long as two accumulators of the pair fit
+// into tensor memory (2048 tokens over 128 experts: gate/up 85 us, 91 with tiles of up to 256).
+int expert_tile_lanes(int pairs, int experts) {
     const int share = (pairs + experts - 1) / experts;
     int lanes = 32;
-    while (lanes < 2 * share && lanes < MAX_LANES) lanes *= 2;
+    while (lanes < 2 * share && lanes < 128) lanes *= 2;
     return lanes;
 }
 // As plan_dense, for as many lane tiles as there are experts, each with its even share.
