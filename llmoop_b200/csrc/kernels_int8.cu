@@ -138,6 +138,10 @@ __device__ __forceinline__ void init_barrier(uint32_t barrier, int count) { asm 
 
 // NaN stays NaN.
 __device__ __forceinline__ uint16_t to_bf16(float value) { return __bfloat16_as_ushort(__float2bfloat16_rn(value)); }
+__device__ __forceinline__ uint32_t two_bf16(float low, float high) {
+    const __nv_bfloat162 both = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t *>(&both);
+}
 
 // ---- quantisation of activation rows
 
@@ -313,7 +317,7 @@ struct Int8Args {
     int lanes, n, k, to_f32;
     int *error_flag;
     int rows;  // output channels of a CTA's tile
-    int tile_lanes, lane_tiles, row_tiles, stages;
+    int tile_lanes, lane_tiles, row_tiles, stages, wide;  // wide: bf16 outputs and residual in sixteen bytes
     // experts
     const int4 *tiles;
     const int *tile_count, *pair_of;
@@ -361,7 +365,14 @@ struct GemmControl {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
     uint32_t tmem;
 };
-constexpr size_t GEMM_CONTROL = (sizeof(GemmControl) + 1023) / 1024 * 1024;
+// bf16 outputs pass through shared memory: a warp's 32 channels of sixteen lanes, PITCH floats a lane (so that eight threads that
+// read sixteen bytes each meet all banks), leave it as sixteen bytes a thread.
+constexpr int PITCH = 36;
+struct Transposed {
+    float values[OUTPUT_WARPS][16 * PITCH];
+};
+template <Mode MODE>
+constexpr size_t gemm_control() { return (sizeof(GemmControl) + (MODE == LINEAR || MODE == PAIR ? sizeof(Transposed) : 0) + 1023) / 1024 * 1024; }
 
 __device__ __forceinline__ void load_sums(uint32_t address, int (&d)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -381,7 +392,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;         // rank: of the CTA in its pair
     const uint32_t a_bytes = static_cast<uint32_t>((a.rows + 7) / 8 * 8) * BLOCK_K, half_box = static_cast<uint32_t>(a.tile_lanes / 2) * BLOCK_K,
                    stage_bytes = MATRICES * a_bytes + half_box;
-    const uint32_t base = shared_address(smem) + static_cast<uint32_t>(GEMM_CONTROL);
+    const uint32_t base = shared_address(smem) + static_cast<uint32_t>(gemm_control<MODE>());
     const uint32_t full = shared_address(control.full), empty = shared_address(control.empty), acc_full = shared_address(control.acc_full),
                    acc_empty = shared_address(control.acc_empty);
     // the first CTA's barriers, which both CTAs' copies and outputs report to
@@ -563,13 +574,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             const bool in_range = row < a.rows && channel < a.n;
             if (quarter * 32 < a.rows) {
                 const uint16_t *residual = MODE == LINEAR ? a.residual : nullptr;
-                uint16_t beside[2][16];  // of this step and the next
-                auto fetch_beside = [&](uint16_t(&to)[16], int column) {
+                // Wide outputs: thread = eight channels of lanes lane / 4 and lane / 4 + 8.  What is added to them is fetched a step ahead.
+                const bool wide = (MODE == LINEAR || MODE == PAIR) && a.wide;
+                const int eight = tile.row0 + quarter * 32 + (lane & 3) * 8;
+                const bool eight_in_range = quarter * 32 + (lane & 3) * 8 < a.rows && eight < a.n;
+                float *const transposed = reinterpret_cast<Transposed *>(smem + sizeof(GemmControl))->values[warp - 4];
+                uint4 beside[2];
+                auto fetch_beside = [&](int column) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (in_range && column + i < tile.count) to[i] = residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel];
+                    for (int half = 0; half < 2; half++)
+                        if (eight_in_range && column + half * 8 + lane / 4 < tile.count)
+                            beside[half] = *reinterpret_cast<const uint4 *>(residual + static_cast<size_t>(tile.lane0 + column + half * 8 + lane / 4) * a.n + eight);
                 };
-                if (residual != nullptr) fetch_beside(beside[0], part * 16), fetch_beside(beside[1], part * 16 + 32);
+                if (wide && residual != nullptr) fetch_beside(part * 16);
                 for (int column = part * 16; column < tile.count; column += 32) {
                     int sums[16], up_sums[16];
                     load_sums(accumulator + static_cast<uint32_t>(column), sums);
@@ -579,7 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         *reinterpret_cast<float4 *>(scales + i) = *reinterpret_cast<const float4 *>(info.scale + column + i);
-                        *reinterpret_cast<int4 *>(to + i) = *reinterpret_cast<const int4 *>(info.to + column + i);
+                        if (GROUPED) *reinterpret_cast<int4 *>(to + i) = *reinterpret_cast<const int4 *>(info.to + column + i);
                     }
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     float values[16];
@@ -587,24 +604,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                     for (int i = 0; i < 16; i++) {
                         values[i] = scaled(sums[i], factor, scales[i]);
                         if (TWO) values[i] = silu_product(values[i], scaled(up_sums[i], up_factor, scales[i]));
-                        if (MODE == LINEAR && residual != nullptr) {
-                            values[i] = __fadd_rn(values[i], bf16_bits_to_f32(beside[0][i]));
-                            beside[0][i] = beside[1][i];
-                        }
                     }
-                    if (residual != nullptr) fetch_beside(beside[1], column + 64);
-                    const bool f32 = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN || (MODE == LINEAR && a.to_f32);
+                    if (wide) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) transposed[i * PITCH + lane] = values[i];
+                        __syncwarp();
+                        uint4 out[2];
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const float4 *from = reinterpret_cast<const float4 *>(transposed + (half * 8 + lane / 4) * PITCH + (lane & 3) * 8);
+                            const float4 low = from[0], high = from[1];
+                            float v[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+                            if (residual != nullptr) {
+                                const uint32_t words[4] = {beside[half].x, beside[half].y, beside[half].z, beside[half].w};
+#pragma unroll
+                                for (int i = 0; i < 8; i++) v[i] = __fadd_rn(v[i], i & 1 ? bf16_hi(words[i >> 1]) : bf16_lo(words[i >> 1]));
+                            }
+                            out[half] = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
+                        }
+                        if (residual != nullptr) fetch_beside(column + 32);
+#pragma unroll
+                        for (int half = 0; half < 2; half++)
+                            if (eight_in_range && column + half * 8 + lane / 4 < tile.count)
+                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.y) + static_cast<size_t>(tile.lane0 + column + half * 8 + lane / 4) * a.n + eight) = out[half];
+                        __syncwarp();
+                        continue;
+                    }
                     const int count = in_range ? tile.count - column : 0;
-                    if (f32) {
+                    if (GROUPED) {
                         float *const out = static_cast<float *>(a.y) + channel;
 #pragma unroll
                         for (int i = 0; i < 16; i++)
                             if (i < count) out[static_cast<size_t>(to[i]) * a.n] = values[i];
                     } else {
-                        uint16_t *const out = static_cast<uint16_t *>(a.y) + channel;
+                        const size_t at = static_cast<size_t>(tile.lane0 + column) * a.n + channel;
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (i < count) out[static_cast<size_t>(to[i]) * a.n] = to_bf16(values[i]);
+                        for (int i = 0; i < 16; i++) {
+                            if (i >= count) continue;
+                            if (residual != nullptr) values[i] = __fadd_rn(values[i], bf16_bits_to_f32(residual[at + static_cast<size_t>(i) * a.n]));
+                            if (MODE == LINEAR && a.to_f32) static_cast<float *>(a.y)[at + static_cast<size_t>(i) * a.n] = values[i];
+                            else static_cast<uint16_t *>(a.y)[at + static_cast<size_t>(i) * a.n] = to_bf16(values[i]);
+                        }
                     }
                 }
             }
@@ -1119,17 +1159,18 @@ bool encode(CUtensorMap *map, const int8_t *matrix, int64_t rows, int k, int box
 }
 
 // As many stages as fit, with room for an A operand of 128 rows at the last one's base.
-size_t plan_stages(Int8Args &args, bool pair) {
-    const int matrices = pair ? 2 : 1;
+template <Mode MODE>
+size_t plan_stages(Int8Args &args) {
+    constexpr int matrices = MODE == PAIR || MODE == EXPERTS_PAIR ? 2 : 1;
     const size_t a_bytes = static_cast<size_t>((args.rows + 7) / 8 * 8) * BLOCK_K, stage = matrices * a_bytes + static_cast<size_t>(args.tile_lanes / 2) * BLOCK_K;
     const size_t last = std::max(stage, (matrices - 1) * a_bytes + static_cast<size_t>(ROWS) * BLOCK_K);
-    args.stages = static_cast<int>(std::min<size_t>(MAX_STAGES, 1 + (SMEM_LIMIT - GEMM_CONTROL - last) / stage));
-    return GEMM_CONTROL + static_cast<size_t>(args.stages - 1) * stage + last;
+    args.stages = static_cast<int>(std::min<size_t>(MAX_STAGES, 1 + (SMEM_LIMIT - gemm_control<MODE>() - last) / stage));
+    return gemm_control<MODE>() + static_cast<size_t>(args.stages - 1) * stage + last;
 }
 
 template <Mode MODE>
 cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
-    const size_t bytes = plan_stages(args, MODE == PAIR || MODE == EXPERTS_PAIR);
+    const size_t bytes = plan_stages<MODE>(args);
     const cudaError_t status = allow_shared_memory<int8_gemm_kernel<MODE>>(SMEM_LIMIT);
     if (status != cudaSuccess) return status;
     return launch_dependent(int8_gemm_kernel<MODE>, dim3(2 * std::min(most_tiles, multiprocessors() / 2)), dim3(THREADS), bytes, 1, stream, args);
@@ -1146,7 +1187,7 @@ void plan_dense(Int8Args &args, bool pair) {
     int64_t best = 0;
     for (int split = least; split <= 2 * least + 2 && (split == least || padded / split >= 32); split++) {
         const int lanes = ((padded + split - 1) / split + 31) / 32 * 32;
-        for (int rows = ROWS; rows >= 1; rows -= rows > 32 ? 4 : 1) {
+        for (int rows = ROWS; rows >= 8; rows -= 8) {  // (in steps of sixteen bytes of outputs)
             const int64_t row_tiles = (args.n + 2 * rows - 1) / (2 * rows), lane_tiles = (padded + lanes - 1) / lanes, waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
             const int64_t tensor = matrices * std::max(2 * lanes, 310), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
             const int64_t outputs = 12 * lanes * matrices, shown = 2 * matrices * lanes <= 512 ? 1 : waves;
@@ -1238,6 +1279,7 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
     if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.tile_lanes / 2))
         return cudaErrorInvalidValue;
     args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
+    args.wide = !to_f32 && n % 8 == 0 && (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) % 16 == 0;
     return launch_gemm<MODE>(args, args.row_tiles * args.lane_tiles, stream);
 }
 
