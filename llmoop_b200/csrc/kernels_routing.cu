@@ -6,10 +6,12 @@
 //   ids      = the top_k largest choices within the chosen_groups best groups, the lower number first among equals;
 //              -1 where open experts run out
 //   weights  = their scores (0 for -1), over the sum of the chosen ones' where renormalised, times scale
-// All of it is held in 64 bits: experts next to one another are told apart as the definition does, not by what the last bit
-// of an exponential made of them.
+// The definition holds all of it in 64 bits: experts next to one another are told apart as it does, not by what the last bit of an
+// exponential made of them.  64-bit exponentials and keys are also what such a kernel spends its time on (16384 tokens of 256
+// experts in 8 groups: 81 us), so that 32 bits, with a bound on the error, find the few candidates, which alone are scored and ranked
+// in 64; tokens that cannot be decided so (groups closer than the error, infinities) are done by the definition.
 //
-// One warp per token, expert e with thread e % 32.  (No pointer is __restrict__: loads through those may move in front of the wait
+// One warp per token.  (No pointer is __restrict__: loads through those may move in front of the wait
 // for the kernel that writes the logits.)
 #include "common.cuh"
 #include "kernels.cuh"
@@ -39,13 +41,10 @@ __device__ __forceinline__ double value_of(uint64_t key) {  // of a key above 0
 
 constexpr int TOKENS_PER_CTA = 4;
 
+// One token by the definition.  Expert e with thread e % 32.
 template <typename T, int PER_THREAD>
-__global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(const T *logits, const float *bias, int *ids,
-                                                                            float *weights, int tokens, Routing routing) {
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const int token = blockIdx.x * TOKENS_PER_CTA + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (token >= tokens) return;
+__device__ __noinline__ void route_in_64_bits(const T *logits, const float *bias, int *ids, float *weights, int token, const Routing &routing) {
+    const int lane = threadIdx.x & 31;
     const int experts = routing.experts;
     const float infinity = __uint_as_float(0x7f800000u);
     float logit[PER_THREAD];
@@ -157,17 +156,255 @@ __global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(cons
     }
 }
 
+// Unsigned numbers in the order of the values, above 0.  (-0 lies in front of 0.)
+__device__ __forceinline__ uint32_t key_of(float value) {
+    const uint32_t bits = __float_as_uint(value);
+    return bits ^ (static_cast<uint32_t>(static_cast<int>(bits) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key); }  // of a key above 0
+
+// Scores in 32 bits, by 2^x and 1 / x as the chip has them: off by less than 1.5e-6 (the error of the exponential grows with the
+// distance from the largest, which the score's smallness outweighs).
+__device__ __forceinline__ float fast_exp(float x) {
+    float out;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(out) : "f"(x * 1.4426950408889634f));
+    return out;
+}
+__device__ __forceinline__ float fast_inverse(float x) {
+    float out;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(out) : "f"(x));
+    return out;
+}
+// How far two choices, or sums of two, have to lie apart to be as far apart in truth.
+__device__ __forceinline__ float margin(float value) { return 1.6e-5f * (1.0f + fabsf(value)); }
+
+// PER_THREAD successive values, in sixteen bytes where they lie so.
+template <int PER_THREAD>
+__device__ __forceinline__ void load_run(const float *from, float (&to)[PER_THREAD]) {
+    if constexpr (PER_THREAD % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j += 4) {
+            const float4 four = *reinterpret_cast<const float4 *>(from + j);
+            to[j] = four.x, to[j + 1] = four.y, to[j + 2] = four.z, to[j + 3] = four.w;
+        }
+    }
+}
+template <int PER_THREAD>
+__device__ __forceinline__ void load_run(const uint16_t *from, float (&to)[PER_THREAD]) {
+    if constexpr (PER_THREAD % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j += 4) {
+            const uint2 four = *reinterpret_cast<const uint2 *>(from + j);
+            to[j] = bf16_lo(four.x), to[j + 1] = bf16_hi(four.x), to[j + 2] = bf16_lo(four.y), to[j + 3] = bf16_hi(four.y);
+        }
+    }
+}
+
+struct Plan {
+    Routing routing;
+    int per;      // experts of a thread
+    int threads;  // of a group; 0 where a group is not a run of whole threads
+    int runs;     // logits and bias lie in runs of `per` = PER_THREAD on boundaries of sixteen (bf16: eight) bytes
+};
+struct Candidates {
+    uint32_t expert[32];
+    float logit[32];
+    double choice[32];
+    uint32_t sorted_expert[32];
+    double sorted_score[32];
+};
+
+// A token whose candidates are found in 32 bits, with a bound on the error, and ranked in 64; false where that is not certain to
+// choose what the definition does.  Without a bias experts are in the order of their logits, which needs no arithmetic; groups of
+// ranks closer than the error are not decided here.  Thread l holds the `per` experts from l * per on, so that a group is a run of
+// threads.
+template <typename T, int PER_THREAD>
+__device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *bias, int *ids, float *weights, int token, const Plan &plan, Candidates &found) {
+    const Routing &routing = plan.routing;
+    const int lane = threadIdx.x & 31, experts = routing.experts, per = plan.per, base = lane * per;
+    const T *row = logits + static_cast<size_t>(token) * experts;
+    const float infinity = __uint_as_float(0x7f800000u);
+    float logit[PER_THREAD], score[PER_THREAD];
+    if (plan.runs) {
+        load_run<PER_THREAD>(row + base, logit);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) logit[j] = j < per && base + j < experts ? logit_of(row, base + j) : -infinity;
+    }
+    float top = -infinity;
+#pragma unroll
+    for (int j = 0; j < PER_THREAD; j++) top = fmaxf(top, logit[j]);
+    top = value_of(__reduce_max_sync(0xffffffffu, key_of(top)));
+    // (the scores of larger logits meet in 64 bits, too, or have no f32 form)
+    if (top == infinity || (routing.sigmoid && top > 30.0f)) return false;
+    const bool scored = bias != nullptr || (routing.groups > 1 && routing.group_scores > 1);
+    if (scored && routing.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) score[j] = fast_inverse(1.0f + fast_exp(-logit[j]));
+    } else if (scored) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) {
+            score[j] = fast_exp(fmaxf(logit[j], -infinity) - top);  // (NaN counts as -infinity)
+            sum += score[j];
+        }
+        const float inverse = fast_inverse(warp_sum(sum));
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) score[j] *= inverse;
+    }
+    uint32_t key[PER_THREAD];  // of the choice, or of the logit; 0: closed
+    if (bias != nullptr) {
+        float own[PER_THREAD];
+        if (plan.runs) {
+            load_run<PER_THREAD>(bias + base, own);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; j++) own[j] = j < per && base + j < experts ? bias[base + j] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) {
+            const float value = score[j] + own[j];
+            key[j] = logit[j] > -infinity && value > -infinity ? key_of(value) : 0u;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) key[j] = logit[j] > -infinity ? key_of(logit[j] + 0.0f) : 0u;
+    }
+    if (routing.groups > 1) {
+        const int threads = plan.threads, own_group = lane / threads, first = own_group * threads;
+        const bool by_score = bias == nullptr && scored;
+        uint32_t best = 0, next = 0;
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) {
+            const uint32_t value = by_score && key[j] != 0 ? key_of(score[j]) : key[j];
+            next = max(next, min(best, value));
+            best = max(best, value);
+        }
+        uint32_t group_best = 0, group_next = 0;
+        for (int other = 0; other < threads; other++) {
+            const uint32_t b = __shfl_sync(0xffffffffu, best, first + other), n = __shfl_sync(0xffffffffu, next, first + other);
+            group_next = max(max(group_next, n), min(group_best, b));
+            group_best = max(group_best, b);
+        }
+        const bool open = own_group < routing.groups && group_best != 0;
+        float rank = open ? value_of(group_best) : -infinity;
+        if (routing.group_scores > 1 && open && group_next != 0) rank += value_of(group_next);
+        int before = 0;
+        for (int group = 0; group < routing.groups; group++) {
+            const float other = __shfl_sync(0xffffffffu, rank, group * threads);
+            before += other > rank || (other == rank && group < own_group);
+        }
+        const bool kept = open && before < routing.chosen_groups;
+        const uint32_t first_left = __reduce_max_sync(0xffffffffu, open && !kept ? key_of(rank) : 0u), last_kept = __reduce_min_sync(0xffffffffu, kept ? key_of(rank) : 0xffffffffu);
+        if (first_left != 0) {  // (equal logits are equal scores; whatever else lies close is not decided here)
+            const float in = value_of(last_kept), out = value_of(first_left);
+            if (scored ? !(in - out > margin(in)) : in == out) return false;
+        }
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++) key[j] = kept ? key[j] : 0u;
+    }
+    // The top_k-th largest of the threads' own largest keys is no more than the top_k-th largest of all: what is not further below
+    // it than the error is a candidate, few more than top_k.
+    uint32_t own_best = 0, limit = 0;
+#pragma unroll
+    for (int j = 0; j < PER_THREAD; j++) own_best = max(own_best, key[j]);
+    for (int route = 0; route < routing.top_k; route++) {
+        limit = __reduce_max_sync(0xffffffffu, own_best);
+        if (limit == 0) break;
+        if (own_best == limit) own_best = 0;
+    }
+    if (limit == 0) limit = 1;  // all that are open
+    else if (bias != nullptr) limit = key_of(value_of(limit) - margin(value_of(limit)));
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < PER_THREAD; j++) {
+        const bool candidate = key[j] >= limit;
+        const uint32_t all = __ballot_sync(0xffffffffu, candidate);
+        const int place = count + __popc(all & ((1u << lane) - 1u));
+        if (candidate && place < 32) {
+            found.expert[place] = static_cast<uint32_t>(base + j);
+            found.logit[place] = logit[j];
+        }
+        count += __popc(all);
+    }
+    if (count > 32) return false;
+    __syncwarp();
+    // one candidate to a thread: its score in 64 bits, and the number of those in front of it
+    double sum = 0.0;  // of the softmax's terms, where more than their order and ratios count
+    if (!routing.sigmoid && (bias != nullptr || !routing.renormalise)) {
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j++)
+            if (logit[j] > -infinity) sum += exp(static_cast<double>(logit[j]) - static_cast<double>(top));
+#pragma unroll
+        for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+    }
+    const uint32_t my_expert = lane < count ? found.expert[lane] : 0u;
+    double own_score = 0.0, choice = 0.0;
+    if (lane < count) {
+        const double own_logit = static_cast<double>(found.logit[lane]);
+        own_score = exp(routing.sigmoid ? -own_logit : own_logit - static_cast<double>(top));
+        if (routing.sigmoid) own_score = 1.0 / (1.0 + own_score);
+        else if (sum > 0.0) own_score /= sum;
+        choice = bias != nullptr ? own_score + static_cast<double>(bias[my_expert]) : own_score;
+        found.choice[lane] = choice;
+    }
+    if (__any_sync(0xffffffffu, lane < count && own_score < 1e-250)) return false;  // where scores run out of exponents
+    __syncwarp();
+    int place = 0;
+    for (int other = 0; other < count; other++) {
+        const double theirs = found.choice[other];
+        place += theirs > choice || (theirs == choice && found.expert[other] < my_expert);
+    }
+    if (lane < count) {
+        found.sorted_expert[place] = my_expert;
+        found.sorted_score[place] = own_score;
+    }
+    __syncwarp();
+    const bool chosen = lane < min(count, routing.top_k);
+    double weight = chosen ? found.sorted_score[lane] : 0.0;
+    if (routing.renormalise) {
+        double total = weight;
+#pragma unroll
+        for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
+        weight = total > 0.0 ? weight / total : 0.0;
+    }
+    if (lane < routing.top_k) {
+        ids[static_cast<size_t>(token) * routing.top_k + lane] = chosen ? static_cast<int>(found.sorted_expert[lane]) : -1;
+        weights[static_cast<size_t>(token) * routing.top_k + lane] = static_cast<float>(weight * static_cast<double>(routing.scale));
+    }
+    return true;
+}
+
+template <typename T, int PER_THREAD>
+__global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(const T *logits, const float *bias, int *ids, float *weights, int tokens, Plan plan) {
+    __shared__ Candidates found[TOKENS_PER_CTA];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int warp = static_cast<int>(threadIdx.x >> 5), token = blockIdx.x * TOKENS_PER_CTA + warp;
+    if (token >= tokens) return;
+    if (plan.routing.top_k <= 32 && (plan.routing.groups == 1 || plan.threads > 0) && route_in_32_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan, found[warp])) return;
+    route_in_64_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan.routing);
+}
+
 template <typename T>
 cudaError_t launch(const T *logits, const float *bias, int *ids, float *weights, int tokens, const Routing &routing, cudaStream_t stream) {
     const dim3 grid((tokens + TOKENS_PER_CTA - 1) / TOKENS_PER_CTA), block(32 * TOKENS_PER_CTA);
-    auto with = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, 1, stream, logits, bias, ids, weights, tokens, routing); };
-    const int per_thread = (routing.experts + 31) / 32;
-    if (per_thread <= 1) return with(route_experts_kernel<T, 1>);
-    if (per_thread <= 2) return with(route_experts_kernel<T, 2>);
-    if (per_thread <= 4) return with(route_experts_kernel<T, 4>);
-    if (per_thread <= 8) return with(route_experts_kernel<T, 8>);
-    if (per_thread <= 16) return with(route_experts_kernel<T, 16>);
-    return with(route_experts_kernel<T, 32>);
+    Plan plan = {};
+    plan.routing = routing;
+    plan.per = (routing.experts + 31) / 32;
+    const int size = routing.experts / routing.groups;
+    plan.threads = size % plan.per == 0 ? size / plan.per : 0;
+    auto with = [&](auto kernel, int per_thread) {
+        plan.runs = per_thread % 4 == 0 && routing.experts == 32 * per_thread && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 &&
+                    reinterpret_cast<uintptr_t>(bias) % 16 == 0;
+        return launch_dependent(kernel, grid, block, 0, 1, stream, logits, bias, ids, weights, tokens, plan);
+    };
+    if (plan.per <= 1) return with(route_experts_kernel<T, 1>, 1);
+    if (plan.per <= 2) return with(route_experts_kernel<T, 2>, 2);
+    if (plan.per <= 4) return with(route_experts_kernel<T, 4>, 4);
+    if (plan.per <= 8) return with(route_experts_kernel<T, 8>, 8);
+    if (plan.per <= 16) return with(route_experts_kernel<T, 16>, 16);
+    return with(route_experts_kernel<T, 32>, 32);
 }
 
 }  // namespace
