@@ -673,7 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
 constexpr int FEW = 8, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
 constexpr uint32_t ATOM = 1024, STREAM_STAGE = ROWS * BLOCK_K;
 constexpr int FEW_ROUTES = 128;          // of the experts' form
-constexpr int STREAM_SMALL_SHARE = 16;   // stages
+constexpr int STREAM_SMALL_SHARE = 48;   // stages
 
 struct StreamArgs {
     CUtensorMap weights, up;  // boxes of 128 columns x rows weight rows
@@ -827,15 +827,15 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    // not before the tensor memory is this CTA's: one of the next kernel's that took it first would wait for this one
+    // not before the tensor memory is this CTA's: one of the next kernel's that took it first would wait for this one.  The experts'
+    // gate/up product also waits for the kernel in front before: the down product, which starts then, may read the routes and the
+    // weights while this one still runs, and waits for its rows alone.
+    if (MODE == EXPERTS_PAIR) grid_dependency_wait();
     grid_launch_dependents();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(shared_address(&control.tmem)) : "memory");
     tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
-    if (GROUPED) {
-        grid_dependency_wait();
-        find_routes(a, control, routes);
-    }
+    if (GROUPED) find_routes(a, control, routes);
     const int tiles = (GROUPED ? control.used : 1) * a.row_tiles;
     const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.x / gridDim.x), last_tile = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.x + 1) / gridDim.x);
 
@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
             }
         }
     } else if (warp == 1) {  // ---- MMAs
-        if (!GROUPED) grid_dependency_wait();
+        if (MODE != EXPERTS_PAIR) grid_dependency_wait();
         // instruction descriptor as in int8_gemm_kernel, M = 128
         const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(max(2, a.groups)) << 17) | (8u << 24));
         const uint64_t a_first = swizzled_descriptor(ring), b_first = swizzled_descriptor(shared_address(atoms));
@@ -932,7 +932,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
         }
     } else if (warp >= 4) {
         const int thread = threadIdx.x - 128;
-        if (!GROUPED) grid_dependency_wait();
+        if (MODE != EXPERTS_PAIR) grid_dependency_wait();
         if (!DOWN) {  // ---- quantisation, once
             auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
             quantise_few<256, uint16_t, HeldBf16>(a, atoms, control.amax[0], control.lane_scales[0], thread,
@@ -1182,22 +1182,22 @@ cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
 // which the first of a row's tiles brings in, at some 23; and every tile has its start and end, outputs that no other tile's
 // sums hide (the last one's, and all of a pair's with one accumulator) among them.
 void plan_dense(Int8Args &args, bool pair) {
-    const int64_t pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1;
+    const int pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1;
     const int padded = (args.lanes + 31) / 32 * 32, least = (padded + MAX_LANES - 1) / MAX_LANES;
     int64_t best = 0;
     for (int split = least; split <= 2 * least + 2 && (split == least || padded / split >= 32); split++) {
-        const int lanes = ((padded + split - 1) / split + 31) / 32 * 32;
+        const int lanes = ((padded + split - 1) / split + 31) / 32 * 32, lane_tiles = (padded + lanes - 1) / lanes;
         for (int rows = ROWS; rows >= 8; rows -= 8) {  // (in steps of sixteen bytes of outputs)
-            const int64_t row_tiles = (args.n + 2 * rows - 1) / (2 * rows), lane_tiles = (padded + lanes - 1) / lanes, waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
-            const int64_t tensor = matrices * std::max(2 * lanes, 310), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
+            const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
+            const int tensor = matrices * std::max(2 * lanes, 310), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
             const int64_t outputs = 12 * lanes * matrices, shown = 2 * matrices * lanes <= 512 ? 1 : waves;
-            const int64_t cost = waves * (blocks * std::max({tensor, copies, memory}) + 1000) + shown * outputs;
+            const int64_t cost = static_cast<int64_t>(waves) * (static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000) + shown * outputs;
             if (best != 0 && cost >= best) continue;
             best = cost;
             args.rows = rows;
-            args.row_tiles = static_cast<int>(row_tiles);
+            args.row_tiles = row_tiles;
             args.tile_lanes = lanes;
-            args.lane_tiles = static_cast<int>(lane_tiles);
+            args.lane_tiles = lane_tiles;
         }
     }
 }
@@ -1211,14 +1211,21 @@ size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // Tiles of `matrices` matrices of n output channels for the few-lane kernel: as few rows for the busiest CTA as possible, a
 // tile counted as the bytes of four rows more.
 void plan_stream(StreamArgs &args, int matrices, bool pair) {
-    const int count = multiprocessors(), most = pair ? 64 : 128;
+    const int count = multiprocessors(), most = std::min(pair ? 64 : 128, args.n);
     int64_t best = 0;
-    for (int rows = std::min(most, args.n); rows >= 1; rows--) {
-        const int64_t tiles = static_cast<int64_t>(matrices) * ((args.n + rows - 1) / rows), cost = (tiles + count - 1) / count * (rows + 4);
+    for (int waves = 1, tries = 0; tries < 8; waves++) {  // the fewest rows that many waves have room for
+        const int tiles = static_cast<int>(static_cast<int64_t>(count) * waves / matrices);  // of a matrix
+        const int rows = tiles > 0 ? (args.n + tiles - 1) / tiles : args.n;
+        if (rows > most) {
+            waves += std::max(0, static_cast<int>((static_cast<int64_t>(args.n) * matrices / most + count - 1) / count) - waves - 2);
+            continue;
+        }
+        tries++;
+        const int64_t cost = static_cast<int64_t>(waves) * (rows + 4);
         if (best == 0 || cost < best) best = cost, args.rows = rows;
     }
     args.row_tiles = (args.n + args.rows - 1) / args.rows;
-    args.groups = args.rows * 4 <= most ? 4 : args.rows * 2 <= most ? 2 : 1;
+    args.groups = args.rows * 4 <= (pair ? 64 : 128) ? 4 : args.rows * 2 <= (pair ? 64 : 128) ? 2 : 1;
 }
 size_t stream_bytes(const StreamArgs &args, bool two_buffers, size_t tables) {
     const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups;
@@ -1301,8 +1308,8 @@ cudaError_t launch_linear_int8_silu_pair(const uint16_t *x, const int8_t *gate, 
 
 namespace {
 
-// The scratch buffer of one call, in parts on 256-byte boundaries; the weighted rows of the down product take the place of
-// what the gate/up product read and wrote.
+// The scratch buffer of one call, in parts on 256-byte boundaries.  The weighted rows of the down product take the place of
+// what the gate/up product read and wrote, but for calls of few tokens, whose down product reads the latter itself.
 struct ExpertsScratch {
     int4 *tiles;
     int *counts, *place_of, *pair_of;
@@ -1328,7 +1335,7 @@ struct ExpertsScratch {
         xq = reinterpret_cast<int8_t *>(take(pairs * hidden));
         h = reinterpret_cast<float *>(take(pairs * inter * sizeof(float)));
         const size_t product_end = used;
-        used = shared;
+        if (tokens > FEW) used = shared;
         parts = reinterpret_cast<float *>(take(pairs * hidden * sizeof(float)));
         bytes = std::max(product_end, used);
     }
@@ -1346,17 +1353,18 @@ int expert_tile_lanes(int pairs, int experts) {
 // As plan_dense, for as many lane tiles as there are experts, each with its even share.
 void plan_experts(Int8Args &args, int pairs, int experts, bool pair) {
     args.tile_lanes = expert_tile_lanes(pairs, experts);
-    const int64_t count = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1, tiles = std::min(experts, pairs),
-                  share = (pairs / tiles + 31) / 32 * 32;
+    const int count = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1, tiles = std::min(experts, pairs),
+              share = (pairs / tiles + 31) / 32 * 32;
     int64_t best = 0;
-    for (int rows = ROWS; rows >= 16; rows -= 4) {
-        const int64_t row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * tiles + count - 1) / count;
-        const int64_t tensor = matrices * std::max<int64_t>(2 * share, 310), copies = (matrices * rows + args.tile_lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / 23;
-        const int64_t cost = waves * (blocks * std::max({tensor, copies, memory}) + 1000);
+    for (int rows = ROWS; rows >= 16; rows -= 8) {
+        const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * tiles + count - 1) / count;
+        const int tensor = matrices * std::max(2 * std::min(share, args.tile_lanes), 310), copies = (matrices * rows + args.tile_lanes / 2) * BLOCK_K / 56,
+                  memory = matrices * rows * BLOCK_K / 23;
+        const int64_t cost = static_cast<int64_t>(waves) * (static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000);
         if (best != 0 && cost >= best) continue;
         best = cost;
         args.rows = rows;
-        args.row_tiles = static_cast<int>(row_tiles);
+        args.row_tiles = row_tiles;
     }
 }
 

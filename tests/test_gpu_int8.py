@@ -251,7 +251,7 @@ def _routes(g, tokens, top_k, count):
 
 @pytest.mark.parametrize("tokens,top_k,count,hidden,inter", [
     (1, 1, 1, 16, 16), (1, 2, 4, 64, 32), (3, 3, 8, 80, 48), (1, 8, 128, 2048, 768), (24, 8, 128, 2048, 768), (37, 2, 5, 1008, 336), (131, 6, 60, 256, 144),
-    (300, 4, 8, 512, 128), (70, 1, 2, 128, 1040), (513, 2, 3, 272, 80), (65, 5, 1024, 64, 32),
+    (8, 16, 128, 4096, 256), (7, 12, 16, 1024, 512), (300, 4, 8, 512, 128), (70, 1, 2, 128, 1040), (513, 2, 3, 272, 80), (65, 5, 1024, 64, 32),
 ])
 @pytest.mark.parametrize("with_residual", [False, True])
 def test_experts(tokens, top_k, count, hidden, inter, with_residual):
