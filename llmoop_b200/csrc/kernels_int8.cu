@@ -89,6 +89,8 @@ __device__ __forceinline__ void copy_tile(uint32_t target, const CUtensorMap *ma
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // ---- of a pair of CTAs (cta_group::2)
 __device__ __forceinline__ uint32_t of_rank(uint32_t address, int rank) {  // the same place in that CTA's shared memory
     uint32_t out;
@@ -172,6 +174,11 @@ struct HeldBf16 {
         return max(most & 0xffff0000u, most << 16);
     }
     __device__ __forceinline__ float value(int i) const { return i & 1 ? bf16_hi(word(i >> 1)) : bf16_lo(word(i >> 1)); }
+    __device__ __forceinline__ void scale_up() {  // exact
+        uint32_t *w = reinterpret_cast<uint32_t *>(words);
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = (__float_as_uint(bf16_lo(w[i]) * 0x1p+90f) >> 16) | (__float_as_uint(bf16_hi(w[i]) * 0x1p+90f) & 0xffff0000u);
+    }
 };
 struct HeldF32 {
     float4 words[4];
@@ -189,38 +196,41 @@ struct HeldF32 {
         for (int i = 0; i < 16; i++) most = max(most, __float_as_uint(fabsf(value(i))));
         return most;
     }
+    __device__ __forceinline__ void scale_up() {
+#pragma unroll
+        for (int i = 0; i < 4; i++) words[i] = make_float4(words[i].x * 0x1p+90f, words[i].y * 0x1p+90f, words[i].z * 0x1p+90f, words[i].w * 0x1p+90f);
+    }
 };
 
-struct RowScale {
-    float multiplier, scale;
-    bool tiny;
-};
-// q = rint(x multiplier), or of x 2^90 for rows of tiny values, whose 127 / amax is not finite.  The multiplier is rounded up:
-// a bf16 quotient 127 x / amax is 2^-16 of itself away from the nearest tie (both significands are whole numbers below 256)
-// unless it is one; ties are x = amax / 2, whose 63.5 a multiplier too large sends to the even 64 as an exact one does, and
-// those of an amax of 254 powers of two, whose multiplier is exact.
-__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {  // magnitudes compare as their bits do; infinities and NaN are the largest
-    const float amax = __uint_as_float(amax_bits);
-    const bool finite = amax <= 3.4028234e38f;
-    RowScale row;
-    row.tiny = amax < 0x1p-90f;
-    row.multiplier = finite && amax > 0.0f ? __fdiv_ru(127.0f, row.tiny ? amax * 0x1p+90f : amax) : 0.0f;
-    row.scale = finite ? amax / 127.0f : __uint_as_float(0x7fffffffu);  // a row with an infinity or a NaN is NaN throughout
-    return row;
+// q = rint(x multiplier); rows of tiny values, whose 127 / amax is not finite, are taken times 2^90 (scale_up).  The multiplier is
+// 127 / amax, or up to two steps more: a bf16 quotient 127 x / amax is 2^-16 of itself away from the nearest tie (both
+// significands are whole numbers below 256) unless it is one; ties are x = amax / 2, whose 63.5 a multiplier too large sends to
+// the even 64 as the true one does, and those of an amax of 254 powers of two, whose multiplier is a power of two and exact.
+// (An approximate reciprocal, a step of Newton's and a look at the remainder: the division rounded up takes a kernel of
+// microseconds 0.4 us.)
+constexpr float UP = 0x1p+90f;
+__device__ __forceinline__ bool is_tiny(uint32_t amax_bits) { return amax_bits < 0x12800000u; }  // 2^-90
+__device__ __forceinline__ bool is_finite(uint32_t amax_bits) { return amax_bits < 0x7f800000u; }
+__device__ __forceinline__ float row_multiplier(uint32_t amax_bits) {  // magnitudes compare as their bits do; infinities and NaN are the largest
+    const float amax = __uint_as_float(amax_bits) * (is_tiny(amax_bits) ? UP : 1.0f);
+    float inverse;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(amax));
+    const float first = 127.0f * inverse, second = __fmaf_rn(__fmaf_rn(-first, amax, 127.0f), inverse, first);
+    const float up = __fmaf_rn(-second, amax, 127.0f) > 0.0f ? __uint_as_float(__float_as_uint(second) + 1u) : second;
+    return amax_bits != 0 && is_finite(amax_bits) ? up : 0.0f;
+}
+__device__ __forceinline__ float row_scale(uint32_t amax_bits) {  // a row with an infinity or a NaN is NaN throughout
+    return is_finite(amax_bits) ? __uint_as_float(amax_bits) / 127.0f : __uint_as_float(0x7fffffffu);
 }
 // Sixteen whole numbers as bytes.
 template <typename Held>
-__device__ __forceinline__ uint4 quantise(const Held &held, const RowScale &row) {
+__device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
     uint32_t out[4];
 #pragma unroll
     for (int word = 0; word < 4; word++) {
         uint32_t b[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float x = held.value(4 * word + i);
-            if (row.tiny) x *= 0x1p+90f;
-            b[i] = __float_as_uint(__fmaf_rn(x, row.multiplier, 12582912.0f));  // 1.5 * 2^23: one rounding, to even; two's complement in the low bits
-        }
+        for (int i = 0; i < 4; i++) b[i] = __float_as_uint(__fmaf_rn(held.value(4 * word + i), multiplier, 12582912.0f));  // 1.5 * 2^23: one rounding, to even; two's complement in the low bits
         out[word] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
     return make_uint4(out[0], out[1], out[2], out[3]);
@@ -263,11 +273,12 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
         __syncthreads();
         for (int warp = 0; warp < static_cast<int>(blockDim.x >> 5); warp++) amax = max(amax, warps[warp]);
     }
-    const RowScale scale = row_scale(amax);
+    const float multiplier = row_multiplier(amax);
     const int copies = places != nullptr ? top_k : 1;
     const int *own_places = places + (places != nullptr ? static_cast<size_t>(at_row) * top_k : 0);
-    auto store = [&](int at, const Held &values) {
-        const uint4 packed = quantise(values, scale);
+    auto store = [&](int at, Held &values) {
+        if (is_tiny(amax)) values.scale_up();
+        const uint4 packed = quantise(values, multiplier);
         for (int copy = 0; copy < copies; copy++) {
             const int place = places != nullptr ? own_places[copy] : at_row;
             if (place >= 0) *reinterpret_cast<uint4 *>(q + static_cast<size_t>(place) * k + at) = packed;
@@ -284,7 +295,7 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
     for (int copy = first / 16; copy < copies; copy += step / 16) {
         const int place = places != nullptr ? own_places[copy] : at_row;
         if (place < 0) continue;
-        scales[place] = weights != nullptr ? __fmul_rn(scale.scale, weights[pair_of[place]]) : scale.scale;
+        scales[place] = weights != nullptr ? __fmul_rn(row_scale(amax), weights[pair_of[place]]) : row_scale(amax);
         if (places != nullptr) pair_of[place] = at_row * top_k + copy;
     }
 }
@@ -398,6 +409,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
     // the first CTA's barriers, which both CTAs' copies and outputs report to
     const uint32_t leader_full = of_rank(full, 0), leader_acc_empty = of_rank(acc_empty, 0);
     const int blocks = (a.k + BLOCK_K - 1) / BLOCK_K;
+    if (threadIdx.x == 32) prefetch_map(&a.weights);
+    if (threadIdx.x == 64) prefetch_map(&a.activations);
+    if (MODE == PAIR && threadIdx.x == 96) prefetch_map(&a.up);
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) {
             init_barrier(full + s * 8, 1);
@@ -677,11 +691,11 @@ constexpr int STREAM_SMALL_SHARE = 48;   // stages
 
 struct StreamArgs {
     CUtensorMap weights, up;  // boxes of 128 columns x rows weight rows
-    const void *x;            // bf16 rows; the down product: f32
+    const void *x;            // bf16 rows; the down product: f32; on 16-byte boundaries
     const float *scales, *up_scales;
     void *y;
     const uint16_t *residual;
-    int lanes, n, k, to_f32, wide;
+    int lanes, n, k, to_f32;
     int *error_flag;
     int rows, groups, row_tiles, stages;  // output channels of a tile
     // experts
@@ -708,24 +722,24 @@ struct StreamRoutes {
 };
 constexpr int NO_ROUTE = 1 << 30;
 
-// All threads.  The used experts are numbered in the order of their first routes, the same in every CTA.
+// The first 128 threads, beside the others' quantisation.  The used experts are numbered in the order of their first routes, the
+// same in every CTA.
 __device__ __forceinline__ void find_routes(const StreamArgs &a, StreamControl &control, StreamRoutes &routes) {
+    auto sync = [] { asm volatile("bar.sync 4, 128;" ::: "memory"); };
     const int thread = threadIdx.x, count = a.lanes * a.top_k;
-    for (int e = thread; e < a.experts; e += STREAM_THREADS) routes.slot[e] = NO_ROUTE;
-    for (int i = thread; i < FEW_ROUTES * FEW; i += STREAM_THREADS) (&routes.lead[0][0])[i] = NO_ROUTE;
-    __syncthreads();
-    int expert = -1;
-    if (thread < count) {
-        expert = a.ids[thread];
-        if (expert < 0 || expert >= a.experts) expert = -1;
-        routes.ids[thread] = expert;
-        if (expert >= 0) atomicMin(&routes.slot[expert], thread);
-    }
-    __syncthreads();
+    int expert = thread < count ? a.ids[thread] : -1;
+    if (expert >= a.experts) expert = -1;
+    for (int e = thread; e < a.experts; e += FEW_ROUTES) routes.slot[e] = NO_ROUTE;
+#pragma unroll
+    for (int i = 0; i < FEW; i++) routes.lead[thread][i] = NO_ROUTE;
+    sync();
+    routes.ids[thread] = expert;
+    if (expert >= 0) atomicMin(&routes.slot[expert], thread);
+    sync();
     const bool first = expert >= 0 && routes.slot[expert] == thread;
     const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-    if (thread < FEW_ROUTES && (thread & 31) == 0) routes.before[thread >> 5] = __popc(firsts);
-    __syncthreads();
+    if ((thread & 31) == 0) routes.before[thread >> 5] = __popc(firsts);
+    sync();
     int number = __popc(firsts & ((1u << (thread & 31)) - 1u)), used = 0;
     for (int warp = 0; warp < FEW_ROUTES / 32; warp++) {
         if (warp < thread >> 5) number += routes.before[warp];
@@ -736,57 +750,78 @@ __device__ __forceinline__ void find_routes(const StreamArgs &a, StreamControl &
         routes.expert[number] = expert;
     }
     if (thread == 0) control.used = used;
-    __syncthreads();
+    sync();
     if (expert >= 0) atomicMin(&routes.lead[routes.slot[expert]][thread / a.top_k], thread);
-    __syncthreads();
+    sync();
 }
 
-// Quantises rows into atoms at `atoms`, by THREADS_ threads of which this is number `thread`.  row_of(lane): where lane's
-// row starts, NULL for a lane without one.  sync(): among those threads.  The first two parts of a thread stay in registers.
-template <int COUNT, typename T, typename Held, typename RowOf, typename Sync>
-__device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms, uint32_t *amax, float *scales, int thread, RowOf row_of, Sync sync) {
-    const int parts = a.k / 16, all = a.lanes * parts;
-    constexpr int KEPT = sizeof(T) == 2 ? 2 : 1;
+// Quantises rows into atoms at `atoms`, by WARPS warps of which this is number `warp`.  row_of(lane): where lane's row
+// starts, NULL for a lane without one.  sync(): among those warps; fetched(): the rows have been read.  A warp takes thirty-two
+// parts of sixteen columns at a time and requests BATCH such together (one after the other four lanes of 4096 columns took 6.4 us,
+// each the latency of L2); where there are no more, it keeps them from the search for the largest to the quantisation.
+template <int WARPS, int BATCH, typename T, typename Held, typename RowOf, typename Sync, typename Fetched>
+__device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms, uint32_t *amax, float *scales, int warp, RowOf row_of, Sync sync, Fetched fetched) {
+    const int parts = a.k / 16, runs = (parts + 31) / 32, thread = warp * 32 + static_cast<int>(threadIdx.x & 31);
     if (thread < FEW) amax[thread] = 0;
-    sync();
-    Held kept[KEPT];
-    const bool even = parts % 32 == 0;  // a warp's thirty-two parts are of one row
-    for (int i = 0, part = thread; part < all; i++, part += COUNT) {
-        const int lane = part / parts;
-        const T *row = row_of(lane);
-        if (row == nullptr) continue;
-        Held values;
-        values.load(row, (part - lane * parts) * 16, a.wide);
+    struct Position {
+        int lane, run;
+    };
+    auto advance = [&](Position at) {
+        at.run += WARPS;
+        while (at.run >= runs) at.run -= runs, at.lane++;
+        return at;
+    };
+    auto start = [&] {
+        Position at{0, warp};
+        while (at.run >= runs) at.run -= runs, at.lane++;
+        return at;
+    };
+    Held held[BATCH];
+    auto load = [&](Position at) {
 #pragma unroll
-        for (int j = 0; j < KEPT; j++)
-            if (i == j) kept[j] = values;
-        uint32_t most = values.amax();
-        if (even) {
-            most = __reduce_max_sync(0xffffffffu, most);
-            if ((thread & 31) == 0) atomicMax(&amax[lane], most);
-        } else {
-            atomicMax(&amax[lane], most);
+        for (int j = 0; j < BATCH; j++) {
+            if (at.lane >= a.lanes) break;
+            const T *row = row_of(at.lane);
+            const int part = at.run * 32 + static_cast<int>(threadIdx.x & 31);
+            if (row != nullptr && part < parts) held[j].load(row, part * 16, true);
+            at = advance(at);
+        }
+        return at;
+    };
+    Position first = start(), next = load(first);
+    const bool all_held = next.lane >= a.lanes;
+    sync();  // amax is 0
+    while (true) {
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) {
+            if (first.lane >= a.lanes) break;
+            const int part = first.run * 32 + static_cast<int>(threadIdx.x & 31);
+            const uint32_t most = __reduce_max_sync(0xffffffffu, row_of(first.lane) != nullptr && part < parts ? held[j].amax() : 0u);
+            if ((threadIdx.x & 31) == 0) atomicMax(&amax[first.lane], most);
+            first = advance(first);
+        }
+        if (first.lane >= a.lanes) break;
+        load(first);
+    }
+    fetched();
+    sync();
+    // (rolled up: in a kernel of microseconds every instruction is fetched for the first time)
+    first = start();
+#pragma unroll 1
+    while (first.lane < a.lanes) {
+        if (!all_held) load(first);
+#pragma unroll 1
+        for (int j = 0; j < BATCH && first.lane < a.lanes; j++) {
+            const int part = first.run * 32 + static_cast<int>(threadIdx.x & 31);
+            if (is_tiny(amax[first.lane])) held[0].scale_up();
+            if (row_of(first.lane) != nullptr && part < parts)
+                *reinterpret_cast<uint4 *>(atoms + (part >> 3) * ATOM + first.lane * BLOCK_K + (((part & 7) ^ first.lane) << 4)) = quantise(held[0], row_multiplier(amax[first.lane]));
+#pragma unroll
+            for (int i = 0; i + 1 < BATCH; i++) held[i] = held[i + 1];
+            first = advance(first);
         }
     }
-    sync();
-    if (thread < FEW) scales[thread] = row_scale(amax[thread]).scale;
-    RowScale scale = {};
-    int scaled = -1;
-    for (int i = 0, part = thread; part < all; i++, part += COUNT) {
-        const int lane = part / parts, at = part - lane * parts;
-        const T *row = row_of(lane);
-        if (row == nullptr) continue;
-        if (lane != scaled) {
-            scale = row_scale(amax[lane]);
-            scaled = lane;
-        }
-        Held values;
-        if (i >= KEPT) values.load(row, at * 16, a.wide);
-#pragma unroll
-        for (int j = 0; j < KEPT; j++)
-            if (i == j) values = kept[j];
-        *reinterpret_cast<uint4 *>(atoms + (at >> 3) * ATOM + lane * BLOCK_K + (((at & 7) ^ lane) << 4)) = quantise(values, scale);
-    }
+    if (thread < FEW) scales[thread] = row_scale(amax[thread]);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
@@ -806,6 +841,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     const uint32_t full = shared_address(control.full), empty = shared_address(control.empty), acc_full = shared_address(control.acc_full),
                    acc_empty = shared_address(control.acc_empty), b_full = shared_address(control.b_full), b_empty = shared_address(control.b_empty);
     constexpr int QUANTISING = DOWN ? 4 : 8;  // warps
+    if (threadIdx.x == 32) prefetch_map(&a.weights);
+    if (MODE == PAIR && threadIdx.x == 96) prefetch_map(&a.up);
     if (threadIdx.x == 0) {
         for (int s = 0; s < STREAM_MAX_STAGES; s++) {
             init_barrier(full + s * 8, 1);
@@ -835,7 +872,20 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(shared_address(&control.tmem)) : "memory");
     tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
-    if (GROUPED) find_routes(a, control, routes);
+    auto quantise_all = [&] {  // ---- the lanes, once, by warps 4-11
+        auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        auto fetched = [] {
+            if (!GROUPED) asm volatile("bar.arrive 5, 288;" ::: "memory");
+        };
+        quantise_few<8, 4, uint16_t, HeldBf16>(a, atoms, control.amax[0], control.lane_scales[0], warp - 4,
+                                               [&](int row) { return static_cast<const uint16_t *>(a.x) + static_cast<size_t>(row) * a.k; }, sync, fetched);
+        __syncwarp();
+        if (lane == 0) arrive(b_full);
+        sync();  // the outputs read the scales
+    };
+    if (GROUPED && warp < 4) find_routes(a, control, routes);
+    if (MODE == EXPERTS_PAIR && warp >= 4) quantise_all();
+    if (GROUPED) __syncthreads();  // the routes are known (and the rows quantised)
     const int tiles = (GROUPED ? control.used : 1) * a.row_tiles;
     const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.x / gridDim.x), last_tile = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.x + 1) / gridDim.x);
 
@@ -846,6 +896,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
             if (first_tile < last_tile && lane < copies)
                 for (int step = 0; step < min(steps, a.stages); step++) prefetch_tile(map, (step * a.groups + group) * BLOCK_K, first_tile * a.rows);
             grid_dependency_wait();
+            asm volatile("bar.sync 5, 288;" ::: "memory");  // the lanes' rows first: behind a ring of weights their quantisation waits 3 us
         }
         const uint32_t bytes = static_cast<uint32_t>(copies * a.rows) * BLOCK_K;
         int stage = 0, issued = 0;
@@ -933,14 +984,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     } else if (warp >= 4) {
         const int thread = threadIdx.x - 128;
         if (MODE != EXPERTS_PAIR) grid_dependency_wait();
-        if (!DOWN) {  // ---- quantisation, once
-            auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-            quantise_few<256, uint16_t, HeldBf16>(a, atoms, control.amax[0], control.lane_scales[0], thread,
-                                                  [&](int row) { return static_cast<const uint16_t *>(a.x) + static_cast<size_t>(row) * a.k; }, sync);
-            __syncwarp();
-            if (lane == 0) arrive(b_full);
-            sync();  // the outputs read the scales
-        } else if (warp >= 8) {  // ---- for every expert of this CTA's tiles, two at a time
+        if (MODE == LINEAR || MODE == PAIR) {
+            quantise_all();
+        } else if (DOWN && warp >= 8) {  // ---- for every expert of this CTA's tiles, two at a time
             auto sync = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
             int builds = 0, expert = -1;
             for (int tile = first_tile; tile < last_tile; tile++) {
@@ -949,12 +995,12 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                 expert = which;
                 const int buffer = builds & 1;
                 if (!all_of<2, 128>(wait_barrier(b_empty + buffer * 8, static_cast<uint32_t>((builds / 2 + 1) & 1), a.error_flag))) break;
-                quantise_few<128, float, HeldF32>(a, atoms + buffer * atom_bytes, control.amax[buffer], control.lane_scales[buffer], thread - 128,
+                quantise_few<4, 2, float, HeldF32>(a, atoms + buffer * atom_bytes, control.amax[buffer], control.lane_scales[buffer], warp - 8,
                                                   [&](int token) -> const float * {
                                                       const int route = routes.lead[which][token];
                                                       return route == NO_ROUTE ? nullptr : static_cast<const float *>(a.x) + static_cast<size_t>(route) * a.k;
                                                   },
-                                                  sync);
+                                                  sync, [] {});
                 __syncwarp();
                 if (lane == 0) arrive(b_full + buffer * 8);
                 builds++;
@@ -1265,11 +1311,10 @@ template <Mode MODE>
 cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales, const int8_t *up, const float *up_scales, void *y, const uint16_t *residual, void *scratch,
                          int lanes, int n, int k, int to_f32, int *error_flag, cudaStream_t stream) {
     constexpr bool TWO = MODE == PAIR;
-    if (lanes <= FEW) {
+    if (lanes <= FEW && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
         StreamArgs args = {};
         args.x = x, args.scales = scales, args.up_scales = up_scales, args.y = y, args.residual = residual;
         args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
-        args.wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
         plan_stream(args, 1, TWO);
         size_t bytes;
         if (plan_stages(args, args.row_tiles, false, 0, &bytes)) {
@@ -1382,13 +1427,12 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
         return launch_dependent(experts_sum_kernel, dim3(tokens, (hidden / 4 + 255) / 256), dim3(std::min(256, (hidden / 4 + 31) / 32 * 32)), 0, 1, stream, part.parts, ids,
                                 residual, y, top_k, experts, hidden, wide);
     };
-    if (tokens <= FEW && pairs <= FEW_ROUTES) {
+    if (tokens <= FEW && pairs <= FEW_ROUTES && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
         StreamArgs first = {}, second = {};
         first.n = inter, first.k = hidden, first.x = x, first.scales = gate_up_scales, first.y = part.h;
         second.n = hidden, second.k = inter, second.x = part.h, second.scales = down_scales, second.y = part.parts;
         for (StreamArgs *args : {&first, &second}) {
             args->lanes = tokens, args->ids = ids, args->weights_of = weights, args->top_k = top_k, args->experts = experts, args->error_flag = error_flag;
-            args->wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
             plan_stream(*args, std::min(experts, pairs), args == &first);
         }
         size_t first_bytes, second_bytes;
