@@ -756,11 +756,11 @@ __device__ __forceinline__ void find_routes(const StreamArgs &a, StreamControl &
 }
 
 // Quantises rows into atoms at `atoms`, by WARPS warps of which this is number `warp`.  row_of(lane): where lane's row
-// starts, NULL for a lane without one.  sync(): among those warps; fetched(): the rows have been read.  A warp takes thirty-two
+// starts, NULL for a lane without one.  sync(): among those warps.  A warp takes thirty-two
 // parts of sixteen columns at a time and requests BATCH such together (one after the other four lanes of 4096 columns took 6.4 us,
 // each the latency of L2); where there are no more, it keeps them from the search for the largest to the quantisation.
-template <int WARPS, int BATCH, typename T, typename Held, typename RowOf, typename Sync, typename Fetched>
-__device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms, uint32_t *amax, float *scales, int warp, RowOf row_of, Sync sync, Fetched fetched) {
+template <int WARPS, int BATCH, typename T, typename Held, typename RowOf, typename Sync>
+__device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms, uint32_t *amax, float *scales, int warp, RowOf row_of, Sync sync) {
     const int parts = a.k / 16, runs = (parts + 31) / 32, thread = warp * 32 + static_cast<int>(threadIdx.x & 31);
     if (thread < FEW) amax[thread] = 0;
     struct Position {
@@ -803,7 +803,6 @@ __device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms
         if (first.lane >= a.lanes) break;
         load(first);
     }
-    fetched();
     sync();
     // (rolled up: in a kernel of microseconds every instruction is fetched for the first time)
     first = start();
@@ -874,11 +873,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
     auto quantise_all = [&] {  // ---- the lanes, once, by warps 4-11
         auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-        auto fetched = [] {
-            if (!GROUPED) asm volatile("bar.arrive 5, 288;" ::: "memory");
-        };
         quantise_few<8, 4, uint16_t, HeldBf16>(a, atoms, control.amax[0], control.lane_scales[0], warp - 4,
-                                               [&](int row) { return static_cast<const uint16_t *>(a.x) + static_cast<size_t>(row) * a.k; }, sync, fetched);
+                                               [&](int row) { return static_cast<const uint16_t *>(a.x) + static_cast<size_t>(row) * a.k; }, sync);
         __syncwarp();
         if (lane == 0) arrive(b_full);
         sync();  // the outputs read the scales
@@ -893,10 +889,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
         const int copies = TWO ? 2 * a.groups : a.groups, group = TWO ? lane >> 1 : lane, up = TWO ? lane & 1 : 0;
         const CUtensorMap *const map = MODE == PAIR && up ? &a.up : &a.weights;
         if (!GROUPED) {
-            if (first_tile < last_tile && lane < copies)
-                for (int step = 0; step < min(steps, a.stages); step++) prefetch_tile(map, (step * a.groups + group) * BLOCK_K, first_tile * a.rows);
             grid_dependency_wait();
-            asm volatile("bar.sync 5, 288;" ::: "memory");  // the lanes' rows first: behind a ring of weights their quantisation waits 3 us
         }
         const uint32_t bytes = static_cast<uint32_t>(copies * a.rows) * BLOCK_K;
         int stage = 0, issued = 0;
@@ -1000,7 +993,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                                                       const int route = routes.lead[which][token];
                                                       return route == NO_ROUTE ? nullptr : static_cast<const float *>(a.x) + static_cast<size_t>(route) * a.k;
                                                   },
-                                                  sync, [] {});
+                                                  sync);
                 __syncwarp();
                 if (lane == 0) arrive(b_full + buffer * 8);
                 builds++;
@@ -1277,19 +1270,22 @@ size_t stream_bytes(const StreamArgs &args, bool two_buffers, size_t tables) {
     const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups;
     return STREAM_CONTROL + tables + static_cast<size_t>(steps * args.groups) * ATOM * (two_buffers ? 2 : 1);
 }
-// Where a CTA's share of the weights is small, two CTAs of successive calls fit on a multiprocessor if three stages leave room
-// for that: the next one quantises while this one writes its outputs.  Larger shares take all the stages there is room for.
-// False where the activations' atoms leave no room for three.
-bool plan_stages(StreamArgs &args, int tiles, bool two_buffers, size_t tables, size_t *bytes) {
+// Stages in up to `most` bytes of shared memory, or in all of it where three do not fit into those.  False where three do not
+// fit at all beside the activations' atoms.
+bool plan_stages(StreamArgs &args, size_t most, bool two_buffers, size_t tables, size_t *bytes) {
     const size_t fixed = stream_bytes(args, two_buffers, tables);
-    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, count = multiprocessors();
-    const int64_t steps = static_cast<int64_t>((tiles + count - 1) / count) * ((blocks + args.groups - 1) / args.groups);
-    size_t room = SMEM_HALF;
-    if (fixed + 3 * STREAM_STAGE > room || steps > STREAM_SMALL_SHARE) room = SMEM_LIMIT;
-    if (fixed + 3 * STREAM_STAGE > room) return false;
-    args.stages = static_cast<int>(std::min<size_t>(STREAM_MAX_STAGES, (room - fixed) / STREAM_STAGE));
+    if (fixed + 3 * STREAM_STAGE > most) most = SMEM_LIMIT;
+    if (fixed + 3 * STREAM_STAGE > most) return false;
+    args.stages = static_cast<int>(std::min<size_t>(STREAM_MAX_STAGES, (most - fixed) / STREAM_STAGE));
     *bytes = fixed + static_cast<size_t>(args.stages) * STREAM_STAGE;
     return true;
+}
+// Where a CTA's share of the weights is small, half of a multiprocessor's shared memory does: a CTA of the next call can
+// start on the other half while this one writes its outputs (one lane of 4096 x 4096: 4.3 us a call, 4.8 with all of it; four of a
+// 14336 x 4096 pair: 24.5 with half, 22 with all of it).
+size_t stream_share(const StreamArgs &args) {
+    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, count = multiprocessors(), steps = (args.row_tiles + count - 1) / count * ((blocks + args.groups - 1) / args.groups);
+    return steps <= STREAM_SMALL_SHARE ? SMEM_HALF : SMEM_LIMIT;
 }
 template <Mode MODE>
 cudaError_t launch_stream(const StreamArgs &args, int tiles, size_t bytes, cudaStream_t stream) {
@@ -1317,7 +1313,7 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
         args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
         plan_stream(args, 1, TWO);
         size_t bytes;
-        if (plan_stages(args, args.row_tiles, false, 0, &bytes)) {
+        if (plan_stages(args, stream_share(args), false, 0, &bytes)) {
             if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows))) return cudaErrorInvalidValue;
             return launch_stream<MODE>(args, args.row_tiles, bytes, stream);
         }
@@ -1436,7 +1432,7 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
             plan_stream(*args, std::min(experts, pairs), args == &first);
         }
         size_t first_bytes, second_bytes;
-        if (plan_stages(first, std::min(experts, pairs) * first.row_tiles, false, STREAM_ROUTES, &first_bytes) && plan_stages(second, std::min(experts, pairs) * second.row_tiles, true, STREAM_ROUTES, &second_bytes)) {
+        if (plan_stages(first, SMEM_LIMIT, false, STREAM_ROUTES, &first_bytes) && plan_stages(second, SMEM_HALF, true, STREAM_ROUTES, &second_bytes)) {
             if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) ||
                 !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows))
                 return cudaErrorInvalidValue;
