@@ -600,7 +600,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                         if (eight_in_range && column + half * 8 + lane / 4 < tile.count)
                             beside[half] = *reinterpret_cast<const uint4 *>(residual + static_cast<size_t>(tile.lane0 + column + half * 8 + lane / 4) * a.n + eight);
                 };
-                if (wide && residual != nullptr) fetch_beside(part * 16);
+                uint16_t narrow[16];  // the same for outputs one by one: lane column + i
+                auto fetch_narrow = [&](int column) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (in_range && column + i < tile.count) narrow[i] = residual[static_cast<size_t>(tile.lane0 + column + i) * a.n + channel];
+                };
+                if (residual != nullptr) {
+                    if (wide) fetch_beside(part * 16);
+                    else fetch_narrow(part * 16);
+                }
                 for (int column = part * 16; column < tile.count; column += 32) {
                     int sums[16], up_sums[16];
                     load_sums(accumulator + static_cast<uint32_t>(column), sums);
@@ -652,12 +661,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                             if (i < count) out[static_cast<size_t>(to[i]) * a.n] = values[i];
                     } else {
                         const size_t at = static_cast<size_t>(tile.lane0 + column) * a.n + channel;
+                        if (residual != nullptr) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            if (i >= count) continue;
-                            if (residual != nullptr) values[i] = __fadd_rn(values[i], bf16_bits_to_f32(residual[at + static_cast<size_t>(i) * a.n]));
-                            if (MODE == LINEAR && a.to_f32) static_cast<float *>(a.y)[at + static_cast<size_t>(i) * a.n] = values[i];
-                            else static_cast<uint16_t *>(a.y)[at + static_cast<size_t>(i) * a.n] = to_bf16(values[i]);
+                            for (int i = 0; i < 16; i++) values[i] = __fadd_rn(values[i], bf16_bits_to_f32(narrow[i]));
+                            fetch_narrow(column + 32);
+                        }
+                        if (MODE == LINEAR && a.to_f32) {
+                            float *const out = static_cast<float *>(a.y) + at;
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (i < count) out[static_cast<size_t>(i) * a.n] = values[i];
+                        } else {
+                            uint16_t *const out = static_cast<uint16_t *>(a.y) + at;
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (i < count) out[static_cast<size_t>(i) * a.n] = to_bf16(values[i]);
                         }
                     }
                 }

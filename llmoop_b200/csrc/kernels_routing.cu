@@ -13,6 +13,8 @@
 //
 // One warp per token.  (No pointer is __restrict__: loads through those may move in front of the wait
 // for the kernel that writes the logits.)
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.cuh"
 #include "launch.cuh"
@@ -203,7 +205,7 @@ __device__ __forceinline__ void load_run(const uint16_t *from, float (&to)[PER_T
 struct Plan {
     Routing routing;
     int per;      // experts of a thread
-    int threads;  // of a group; 0 where a group is not a run of whole threads
+    int threads;  // of a group
     int runs;     // logits and bias lie in runs of `per` = PER_THREAD on boundaries of sixteen (bf16: eight) bytes
 };
 struct Candidates {
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(cons
     grid_dependency_wait();
     const int warp = static_cast<int>(threadIdx.x >> 5), token = blockIdx.x * TOKENS_PER_CTA + warp;
     if (token >= tokens) return;
-    if (plan.routing.top_k <= 32 && (plan.routing.groups == 1 || plan.threads > 0) && route_in_32_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan, found[warp])) return;
+    if (plan.routing.top_k <= 32 && plan.per <= PER_THREAD && route_in_32_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan, found[warp])) return;
     route_in_64_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan.routing);
 }
 
@@ -392,13 +394,18 @@ cudaError_t launch(const T *logits, const float *bias, int *ids, float *weights,
     Plan plan = {};
     plan.routing = routing;
     plan.per = (routing.experts + 31) / 32;
-    const int size = routing.experts / routing.groups;
-    plan.threads = size % plan.per == 0 ? size / plan.per : 0;
+    if (routing.groups > 1) {  // as many threads to a group as make runs of equal length
+        const int size = routing.experts / routing.groups;
+        plan.threads = std::min(size, 32 / routing.groups);
+        while (size % plan.threads != 0) plan.threads--;
+        plan.per = size / plan.threads;
+    }
     auto with = [&](auto kernel, int per_thread) {
-        plan.runs = per_thread % 4 == 0 && routing.experts == 32 * per_thread && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 &&
+        plan.runs = per_thread % 4 == 0 && routing.experts == 32 * per_thread && plan.per == per_thread && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 &&
                     reinterpret_cast<uintptr_t>(bias) % 16 == 0;
         return launch_dependent(kernel, grid, block, 0, 1, stream, logits, bias, ids, weights, tokens, plan);
     };
+    // (the form in 64 bits has its experts 32 apart; a single group of 1024 takes 32 to a thread in either)
     if (plan.per <= 1) return with(route_experts_kernel<T, 1>, 1);
     if (plan.per <= 2) return with(route_experts_kernel<T, 2>, 2);
     if (plan.per <= 4) return with(route_experts_kernel<T, 4>, 4);
