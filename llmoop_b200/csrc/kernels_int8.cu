@@ -89,6 +89,10 @@ __device__ __forceinline__ void copy_tile(uint32_t target, const CUtensorMap *ma
                  : "memory");
 }
 
+// Both on 16-byte boundaries, a multiple of sixteen bytes.
+__device__ __forceinline__ void copy_bytes(uint32_t target, const uint8_t *from, uint32_t bytes, uint32_t barrier) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(target), "l"(from), "r"(bytes), "r"(barrier) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- of a pair of CTAs (cta_group::2)
@@ -241,11 +245,12 @@ __device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
 // to the place of each of its top_k routes, where it has one, and leaves there which route that is (a store of its own for every
 // route, which expert_groups_kernel's one CTA would take 8 us for).  With weights the scale is that of the row times its route's weight.
 // Bound by DRAM for large batches, by the chain of loads, barrier and stores for small ones.
-// wide: x rows start on 16-byte boundaries.  k is a multiple of 16.
+// wide: x rows start on 16-byte boundaries.  k is a multiple of 16.  width > 0: in the order of int8_stream_kernel's stages, blocks of
+// 128 columns of that many rows, sixteen bytes of a row swizzled as TMA would.
 template <typename T, typename Held, int HELD, bool WARP>
 __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *q, float *scales, const int *places,
                                                             const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
-                                                            int k, int wide) {
+                                                            int k, int wide, int width) {
     __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
@@ -281,7 +286,8 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
         const uint4 packed = quantise(values, multiplier);
         for (int copy = 0; copy < copies; copy++) {
             const int place = places != nullptr ? own_places[copy] : at_row;
-            if (place >= 0) *reinterpret_cast<uint4 *>(q + static_cast<size_t>(place) * k + at) = packed;
+            const size_t to = width > 0 ? (static_cast<size_t>(at >> 7) * width + place) * BLOCK_K + ((((at >> 4) ^ place) & 7) << 4) : static_cast<size_t>(place) * k + at;
+            if (place >= 0) *reinterpret_cast<uint4 *>(q + to) = packed;
         }
     };
 #pragma unroll
@@ -305,12 +311,12 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 // more columns each.
 template <typename T, typename Held, int MOST>
 cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
-                                 int k, cudaStream_t stream) {
+                                 int k, cudaStream_t stream, int width = 0) {
     const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto with = [&](auto kernel, int held, int warp_rows) {
         const int threads = warp_rows != 0 ? 32 * warp_rows : std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
         return launch_dependent(kernel, dim3(warp_rows != 0 ? (rows + warp_rows - 1) / warp_rows : rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, pair_of,
-                                weights, rows, top_k, k, wide);
+                                weights, rows, top_k, k, wide, width);
     };
     if (parts <= 64 && rows >= 1024) return with(quantise_rows_kernel<T, Held, 2, true>, 2, 8);
     if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1, false>, 1, 0);
@@ -385,6 +391,12 @@ struct Transposed {
 template <Mode MODE>
 constexpr size_t gemm_control() { return (sizeof(GemmControl) + (MODE == LINEAR || MODE == PAIR ? sizeof(Transposed) : 0) + 1023) / 1024 * 1024; }
 
+__device__ __forceinline__ void load_eight(uint32_t address, int (&d)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7])
+                 : "r"(address)
+                 : "memory");
+}
 __device__ __forceinline__ void load_sums(uint32_t address, int (&d)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]),
@@ -692,30 +704,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
-// ---- few lanes: the weights stream by, the activations stay
+// ---- few lanes: the weights stream by
 
-// Up to eight lanes: one launch that is bound by the weights' bytes, or for small matrices by the chain of its steps.  Every
-// CTA quantises all lanes itself while its first weights are on their way: eight rows of 128 columns make one swizzled
-// atom of 1 KB, the K-th 128 columns the K-th atom.  A stage of the ring is the MMA's 128 rows; a tile with fewer
-// weight rows puts `groups` successive blocks of 128 columns on top of one another there, 128 / groups rows to each, and
-// multiplies them by as many successive atoms side by side (N = 8 groups): of the products only those of a block with its
-// own atom count, the outputs add them up.  So a tile of 28 rows costs the tensor pipe, which reads all 128 rows at 128
-// bytes per cycle whatever N, a fourth of what one block after the other would.
-// Warps: 0 copies weights, 1 issues MMAs, 4-7 write outputs, 4-11 (the experts' down product: 8-11) quantise.
-constexpr int FEW = 8, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
+// Up to 128 lanes: bound by the weights' bytes, or for small matrices by the chain of its steps.  A stage of the ring is the
+// MMA's 128 rows; a tile with fewer weight rows puts `groups` successive blocks of 128 columns on top of one another there,
+// 128 / groups rows to each, and multiplies them by as many blocks of the activations side by side (N = groups x width): of the
+// products only those of a block with its own block count, the outputs add them up.  The tensor pipe takes some 70 cycles for
+// an instruction of 128 rows whatever N up to 128, so that a tile of 28 rows costs a fourth of what one block after the
+// other would.
+// Activations, as blocks of 128 columns of `width` swizzled rows:
+//   Up to eight lanes of few columns every CTA quantises itself while its first weights are on their way, and keeps them: one launch.
+//   More are quantised by a kernel in front, which leaves them in this order (PREPARED), and come with every stage.
+// Warps: 0 copies, 1 issues MMAs, 4-7 (PREPARED: 4-11) write outputs, 4-11 (the experts' down product: 8-11) quantise.
+constexpr int FEW = 8, STREAM_LANES = 128, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
 constexpr uint32_t ATOM = 1024, STREAM_STAGE = ROWS * BLOCK_K;
 constexpr int FEW_ROUTES = 128;          // of the experts' form
 constexpr int STREAM_SMALL_SHARE = 48;   // stages
+constexpr int STREAM_OWN = 16384;        // values of which every CTA quantises its own copy
 
 struct StreamArgs {
     CUtensorMap weights, up;  // boxes of 128 columns x rows weight rows
-    const void *x;            // bf16 rows; the down product: f32; on 16-byte boundaries
-    const float *scales, *up_scales;
+    const void *x;            // bf16 rows; the down product: f32; on 16-byte boundaries.  PREPARED: blocks of 128 columns x width rows
+    const float *scales, *up_scales, *lane_scales;
     void *y;
     const uint16_t *residual;
     int lanes, n, k, to_f32;
     int *error_flag;
-    int rows, groups, row_tiles, stages;  // output channels of a tile
+    int rows, groups, row_tiles, stages;  // rows: output channels of a tile
+    int width;                            // lanes of a block of the activations: 8, or a multiple of 16
+    int span_log;                         // 32, 64 or 128 threads of the outputs, no fewer than rows, take a lane
     // experts
     const int *ids;
     const float *weights_of;
@@ -728,7 +745,7 @@ struct StreamControl {
     int used;                                // experts with a route
     uint32_t amax[2][FEW];
     float lane_scales[2][FEW];
-    int sums[FEW][ROWS];                     // of a finished tile, per lane and row of the accumulator
+    float prepared_scales[STREAM_LANES];
 };
 // Routes by expert, for tables of up to FEW_ROUTES routes of FEW tokens.
 struct StreamRoutes {
@@ -843,21 +860,30 @@ __device__ __forceinline__ void quantise_few(const StreamArgs &a, uint8_t *atoms
 }
 
 constexpr size_t STREAM_CONTROL = (sizeof(StreamControl) + 1023) / 1024 * 1024, STREAM_ROUTES = (sizeof(StreamRoutes) + 1023) / 1024 * 1024;
+// The sums of some lanes of a finished tile, per lane and row of the accumulator, for each team of four warps.
+template <bool PREPARED>
+constexpr int SUM_LANES = PREPARED ? 16 : FEW;
+template <bool PREPARED>
+constexpr size_t STREAM_SUMS = (PREPARED ? 2 : 1) * SUM_LANES<PREPARED> * ROWS * sizeof(int);
 
-template <Mode MODE>
+template <Mode MODE, bool PREPARED>
 __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __grid_constant__ StreamArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr bool GROUPED = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN, TWO = MODE == PAIR || MODE == EXPERTS_PAIR, DOWN = MODE == EXPERTS_DOWN;
+    static_assert(!(GROUPED && PREPARED));
     StreamControl &control = *reinterpret_cast<StreamControl *>(smem);
-    StreamRoutes &routes = *reinterpret_cast<StreamRoutes *>(smem + STREAM_CONTROL);
+    StreamRoutes &routes = *reinterpret_cast<StreamRoutes *>(smem + STREAM_CONTROL + STREAM_SUMS<PREPARED>);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
     const int blocks = (a.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + a.groups - 1) / a.groups, slot_rows = ROWS / a.groups;
-    const uint32_t atom_bytes = static_cast<uint32_t>(steps * a.groups) * ATOM;
-    uint8_t *const atoms = smem + STREAM_CONTROL + (GROUPED ? STREAM_ROUTES : 0);
+    const uint32_t block_bytes = static_cast<uint32_t>(a.width) * BLOCK_K;  // of activations
+    const uint32_t products = static_cast<uint32_t>(max(16, a.groups * a.width));  // the MMA's N
+    const uint32_t atom_bytes = PREPARED ? 0u : static_cast<uint32_t>(steps * a.groups) * ATOM, stage_bytes = STREAM_STAGE + (PREPARED ? products * BLOCK_K : 0u);
+    uint8_t *const atoms = smem + STREAM_CONTROL + STREAM_SUMS<PREPARED> + (GROUPED ? STREAM_ROUTES : 0);
     const uint32_t ring = shared_address(atoms) + (DOWN ? 2 : 1) * atom_bytes;
     const uint32_t full = shared_address(control.full), empty = shared_address(control.empty), acc_full = shared_address(control.acc_full),
                    acc_empty = shared_address(control.acc_empty), b_full = shared_address(control.b_full), b_empty = shared_address(control.b_empty);
     constexpr int QUANTISING = DOWN ? 4 : 8;  // warps
+    const int teams = PREPARED && a.lanes > SUM_LANES<PREPARED> ? 2 : 1;  // of four warps that write outputs
     if (threadIdx.x == 32) prefetch_map(&a.weights);
     if (MODE == PAIR && threadIdx.x == 96) prefetch_map(&a.up);
     if (threadIdx.x == 0) {
@@ -867,15 +893,17 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
         }
         for (int s = 0; s < 2; s++) {
             init_barrier(acc_full + s * 8, 1);
-            init_barrier(acc_empty + s * 8, 4);
+            init_barrier(acc_empty + s * 8, 4 * teams);
             init_barrier(b_full + s * 8, QUANTISING);
             init_barrier(b_empty + s * 8, 2);  // the MMAs' commit and the outputs
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    constexpr uint32_t COLUMNS = 64, ACCUMULATOR = 32;
+    const uint32_t acc_columns = (products + 31u) & ~31u;
+    uint32_t columns = 64;
+    while (columns < 2 * acc_columns + (a.width < SUM_LANES<PREPARED> ? 16u : 0u)) columns *= 2;  // (the outputs read SUM_LANES at a time)
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tmem)), "r"(COLUMNS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tmem)), "r"(columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -903,12 +931,10 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     const int tiles = (GROUPED ? control.used : 1) * a.row_tiles;
     const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.x / gridDim.x), last_tile = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.x + 1) / gridDim.x);
 
-    if (warp == 0) {  // ---- weights
+    if (warp == 0) {  // ---- copies
         const int copies = TWO ? 2 * a.groups : a.groups, group = TWO ? lane >> 1 : lane, up = TWO ? lane & 1 : 0;
         const CUtensorMap *const map = MODE == PAIR && up ? &a.up : &a.weights;
-        if (!GROUPED) {
-            grid_dependency_wait();
-        }
+        if (!GROUPED) grid_dependency_wait();
         const uint32_t bytes = static_cast<uint32_t>(copies * a.rows) * BLOCK_K;
         int stage = 0, issued = 0;
         uint32_t parity = 1;  // the first round waits for no release
@@ -924,12 +950,17 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                     alive = false;
                     break;
                 }
-                if (elect_one()) expect_bytes(full + stage * 8, bytes);
+                const uint32_t stage_at = ring + static_cast<uint32_t>(stage) * stage_bytes;
+                // (the last step's missing blocks are zeros among the weights, whatever the activations' part of the stage holds)
+                const uint32_t prepared_bytes = PREPARED ? static_cast<uint32_t>(min(a.groups, blocks - step * a.groups)) * block_bytes : 0u;
+                if (elect_one()) expect_bytes(full + stage * 8, bytes + prepared_bytes);
                 __syncwarp();
                 if (lane < copies) {
-                    const uint32_t target = ring + static_cast<uint32_t>(stage) * STREAM_STAGE + static_cast<uint32_t>(group * slot_rows + up * (slot_rows / 2)) * BLOCK_K;
+                    const uint32_t target = stage_at + static_cast<uint32_t>(group * slot_rows + up * (slot_rows / 2)) * BLOCK_K;
                     const int row = MODE == EXPERTS_PAIR ? (expert * 2 + up) * a.n + row0 : expert * a.n + row0;
                     copy_tile(target, map, (step * a.groups + group) * BLOCK_K, row, full + stage * 8);
+                } else if (PREPARED && lane == copies) {
+                    copy_bytes(stage_at + STREAM_STAGE, static_cast<const uint8_t *>(a.x) + static_cast<size_t>(step * a.groups) * block_bytes, prepared_bytes, full + stage * 8);
                 }
                 __syncwarp();
                 issued++;
@@ -942,14 +973,14 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     } else if (warp == 1) {  // ---- MMAs
         if (MODE != EXPERTS_PAIR) grid_dependency_wait();
         // instruction descriptor as in int8_gemm_kernel, M = 128
-        const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(max(2, a.groups)) << 17) | (8u << 24));
+        const uint32_t instruction = __reduce_or_sync(0xffffffffu, (2u << 4) | (1u << 7) | (1u << 10) | (products / 8 << 17) | (8u << 24));
         const uint64_t a_first = swizzled_descriptor(ring), b_first = swizzled_descriptor(shared_address(atoms));
         int stage = 0, round = 0, builds = 0, expert = -1;
         uint32_t parity = 0;
         bool alive = true;
         for (int tile = first_tile; tile < last_tile && alive; tile++, round++) {
             const int which = DOWN ? tile / a.row_tiles : 0;
-            if (which != expert) {
+            if (!PREPARED && which != expert) {
                 if (!wait_barrier(b_full + (builds & 1) * 8, static_cast<uint32_t>((builds >> 1) & 1), a.error_flag)) break;
                 expert = which;
                 builds++;
@@ -958,7 +989,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
             const uint64_t b_base = b_first + static_cast<uint64_t>((builds - 1) & 1) * (DOWN ? atom_bytes >> 4 : 0);
             if (!wait_barrier(acc_empty + (round & 1) * 8, static_cast<uint32_t>((round / 2 + 1) & 1), a.error_flag)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t accumulator = tmem + (round & 1) * ACCUMULATOR;
+            const uint32_t accumulator = tmem + (round & 1) * acc_columns;
             for (int step = 0; step < steps; step++) {
                 if (!wait_barrier(full + stage * 8, parity, a.error_flag)) {
                     alive = false;
@@ -966,7 +997,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) {
-                    const uint64_t a_stage = a_first + static_cast<uint64_t>(stage) * (STREAM_STAGE >> 4), b_stage = b_base + static_cast<uint64_t>(step * a.groups) * (ATOM >> 4);
+                    const uint64_t a_stage = a_first + static_cast<uint64_t>(stage) * (stage_bytes >> 4),
+                                   b_stage = PREPARED ? a_stage + (STREAM_STAGE >> 4) : b_base + static_cast<uint64_t>(step * a.groups) * (ATOM >> 4);
 #pragma unroll
                     for (int part = 0; part < 4; part++) {  // K = 32 per instruction
                         const uint32_t accumulate = (step > 0 || part > 0) ? 1u : 0u;
@@ -993,9 +1025,11 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
             }
         }
     } else if (warp >= 4) {
-        const int thread = threadIdx.x - 128;
         if (MODE != EXPERTS_PAIR) grid_dependency_wait();
-        if (MODE == LINEAR || MODE == PAIR) {
+        if (PREPARED) {
+            if (static_cast<int>(threadIdx.x) - 128 < a.lanes) control.prepared_scales[threadIdx.x - 128] = a.lane_scales[threadIdx.x - 128];
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        } else if (!GROUPED) {
             quantise_all();
         } else if (DOWN && warp >= 8) {  // ---- for every expert of this CTA's tiles, two at a time
             auto sync = [] { asm volatile("bar.sync 2, 128;" ::: "memory"); };
@@ -1017,79 +1051,105 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                 builds++;
             }
         }
-        if (warp < 8) {  // ---- outputs
-            const int quarter = warp & 3, group = quarter * a.groups / 4;
+        const int team = (warp - 4) >> 2;
+        if (team < teams) {  // ---- outputs, SUM_LANES lanes at a time
+            constexpr int CHUNK = SUM_LANES<PREPARED>;
+            const int quarter = warp & 3, group = quarter * a.groups / 4, thread = static_cast<int>(threadIdx.x & 127);
+            const int span = 1 << a.span_log, row = thread & (span - 1), first_lane = thread >> a.span_log, lane_step = 128 >> a.span_log;
+            int(*const sums)[ROWS] = reinterpret_cast<int(*)[ROWS]>(smem + STREAM_CONTROL) + team * CHUNK;
+            auto team_sync = [&] {
+                if (team == 0) asm volatile("bar.sync 3, 128;" ::: "memory");
+                else asm volatile("bar.sync 5, 128;" ::: "memory");
+            };
             int round = 0, builds = 0, expert = -1;
             for (int tile = first_tile; tile < last_tile; tile++, round++) {
-                const int row0 = tile % a.row_tiles * a.rows, which = GROUPED ? tile / a.row_tiles : 0, outputs = min(a.rows, a.n - row0);
+                const int row0 = tile % a.row_tiles * a.rows, which = GROUPED ? tile / a.row_tiles : 0, channel = row0 + row;
+                const bool in_range = row < a.rows && channel < a.n;
                 bool alive = true;
                 if (DOWN && which != expert) {
                     expert = which;
                     alive = wait_barrier(b_full + (builds & 1) * 8, static_cast<uint32_t>((builds >> 1) & 1), a.error_flag);
                     builds++;
                 }
-                const float *scales = control.lane_scales[DOWN ? (builds - 1) & 1 : 0];
-                const size_t expert_row = GROUPED ? static_cast<size_t>(routes.expert[which]) * (TWO ? 2 : 1) * a.n : 0;
-                // what the first output of this thread needs, ahead of its sum
-                auto factors = [&](int at) {
-                    const int channel = row0 + at % a.rows;
-                    float2 factor = make_float2(0.0f, 0.0f);
-                    if (channel < a.n) {
-                        factor.x = a.scales[expert_row + channel];
-                        if (TWO) factor.y = MODE == PAIR ? a.up_scales[channel] : a.scales[expert_row + a.n + channel];
-                        else if (MODE == LINEAR && a.residual != nullptr) factor.y = bf16_bits_to_f32(a.residual[static_cast<size_t>(at / a.rows) * a.n + channel]);
-                    }
-                    return factor;
-                };
-                const int all = a.lanes * a.rows;
-                float2 factor = make_float2(0.0f, 0.0f);
-                if (thread < all) factor = factors(thread);
-                alive = alive && wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag);
-                if (!all_of<3, 128>(alive)) break;  // and: the sums of the tile before have been read
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t d[8];
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7])
-                             : "r"(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (round & 1) * ACCUMULATOR + static_cast<uint32_t>(group * FEW))
-                             : "memory");
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                const float *scales = PREPARED ? control.prepared_scales : control.lane_scales[DOWN ? (builds - 1) & 1 : 0];
+                float factor = 0.0f, up_factor = 0.0f;
+                if (in_range) {
+                    const size_t at = (GROUPED ? static_cast<size_t>(routes.expert[which]) * (TWO ? 2 : 1) * a.n : 0) + channel;
+                    factor = a.scales[at];
+                    if (TWO) up_factor = MODE == PAIR ? a.up_scales[at] : a.scales[at + a.n];
+                }
+                uint16_t beside[4];  // four lanes of the residual ahead
+                auto fetch_beside = [&](int from) {
 #pragma unroll
-                for (int i = 0; i < FEW; i++) control.sums[i][quarter * 32 + lane] = static_cast<int>(d[i]);
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) arrive(acc_empty + (round & 1) * 8);
-                asm volatile("bar.sync 3, 128;" ::: "memory");
-                for (int at = thread; at < all; at += 128) {
-                    const int row = at % a.rows, token = at / a.rows, channel = row0 + row;
-                    if (at != thread) factor = factors(at);
-                    if (row >= outputs) continue;
-                    int sum = 0, up_sum = 0;
-                    for (int g = 0; g < a.groups; g++) {
-                        sum += control.sums[token][g * slot_rows + row];
-                        if (TWO) up_sum += control.sums[token][g * slot_rows + slot_rows / 2 + row];
+                    for (int i = 0; i < 4; i++)
+                        if (in_range && from + i * lane_step < a.lanes) beside[i] = a.residual[static_cast<size_t>(from + i * lane_step) * a.n + channel];
+                };
+                if (MODE == LINEAR && a.residual != nullptr) fetch_beside(team * CHUNK + first_lane);
+                alive = alive && wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag);
+                // they go on together; and: the sums of the tile before have been read
+                if (!(team == 0 ? all_of<3, 128>(alive) : all_of<5, 128>(alive))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int chunk = team * CHUNK; chunk < a.lanes; chunk += teams * CHUNK) {
+                    const uint32_t address = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (round & 1) * acc_columns + static_cast<uint32_t>(group * a.width + chunk);
+                    int d[CHUNK];
+                    if constexpr (PREPARED) load_sums(address, d);
+                    else load_eight(address, d);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (chunk != team * CHUNK) team_sync();
+#pragma unroll
+                    for (int i = 0; i < CHUNK; i++) sums[i][quarter * 32 + lane] = d[i];
+                    if (chunk + teams * CHUNK >= a.lanes) {
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) arrive(acc_empty + (round & 1) * 8);
                     }
+                    team_sync();
+                    if (!in_range) continue;
+                    const int lanes = min(CHUNK, a.lanes - chunk);
+                    auto value_of = [&](int token, float scale) {
+                        int sum = 0, up_sum = 0;
+                        for (int g = 0; g < a.groups; g++) {
+                            sum += sums[token][g * slot_rows + row];
+                            if (TWO) up_sum += sums[token][g * slot_rows + slot_rows / 2 + row];
+                        }
+                        const float value = scaled(sum, factor, scale);
+                        return TWO ? silu_product(value, scaled(up_sum, up_factor, scale)) : value;
+                    };
                     if (DOWN) {
-                        if (routes.lead[which][token] == NO_ROUTE) continue;
                         const int id = routes.expert[which];
-                        for (int route = token * a.top_k; route < (token + 1) * a.top_k; route++)
-                            if (routes.ids[route] == id)
-                                reinterpret_cast<float *>(a.y)[static_cast<size_t>(route) * a.n + channel] = scaled(sum, factor.x, __fmul_rn(scales[token], a.weights_of[route]));
-                        continue;
+                        for (int token = first_lane; token < lanes; token += lane_step) {
+                            if (routes.lead[which][token] == NO_ROUTE) continue;
+                            for (int route = token * a.top_k; route < (token + 1) * a.top_k; route++)
+                                if (routes.ids[route] == id)
+                                    static_cast<float *>(a.y)[static_cast<size_t>(route) * a.n + channel] = value_of(token, __fmul_rn(scales[token], a.weights_of[route]));
+                        }
+                    } else if (GROUPED) {
+                        for (int token = first_lane; token < lanes; token += lane_step) {
+                            const int route = routes.lead[which][token];
+                            if (route != NO_ROUTE) static_cast<float *>(a.y)[static_cast<size_t>(route) * a.n + channel] = value_of(token, scales[token]);
+                        }
+                    } else {
+                        for (int token = first_lane; token < lanes; token += 4 * lane_step) {
+                            float value[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (token + i * lane_step >= lanes) break;
+                                value[i] = value_of(token + i * lane_step, scales[chunk + token + i * lane_step]);
+                                if (MODE == LINEAR && a.residual != nullptr) value[i] = __fadd_rn(value[i], bf16_bits_to_f32(beside[i]));
+                            }
+                            if (MODE == LINEAR && a.residual != nullptr) fetch_beside(token + 4 * lane_step < lanes ? chunk + token + 4 * lane_step : chunk + teams * CHUNK + first_lane);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (token + i * lane_step >= lanes) break;
+                                const size_t out = static_cast<size_t>(chunk + token + i * lane_step) * a.n + channel;
+                                if (MODE == LINEAR && a.to_f32) static_cast<float *>(a.y)[out] = value[i];
+                                else static_cast<uint16_t *>(a.y)[out] = to_bf16(value[i]);
+                            }
+                        }
                     }
-                    float value = scaled(sum, factor.x, scales[token]);
-                    if (TWO) value = silu_product(value, scaled(up_sum, factor.y, scales[token]));
-                    if (MODE == EXPERTS_PAIR) {
-                        const int route = routes.lead[which][token];
-                        if (route != NO_ROUTE) reinterpret_cast<float *>(a.y)[static_cast<size_t>(route) * a.n + channel] = value;
-                        continue;
-                    }
-                    if (MODE == LINEAR && a.residual != nullptr) value = __fadd_rn(value, factor.y);
-                    const size_t out = static_cast<size_t>(token) * a.n + channel;
-                    if (MODE == LINEAR && a.to_f32) reinterpret_cast<float *>(a.y)[out] = value;
-                    else reinterpret_cast<uint16_t *>(a.y)[out] = to_bf16(value);
                 }
                 if (DOWN && (tile + 1 == last_tile || (tile + 1) / a.row_tiles != which)) {  // the scales may go
-                    asm volatile("bar.sync 3, 128;" ::: "memory");
+                    team_sync();
                     if (thread == 0) arrive(b_empty + ((builds - 1) & 1) * 8);
                 }
             }
@@ -1097,7 +1157,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLUMNS) : "memory");
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
 // ---- experts: routes grouped by expert
@@ -1283,19 +1343,22 @@ void plan_stream(StreamArgs &args, int matrices, bool pair) {
     }
     args.row_tiles = (args.n + args.rows - 1) / args.rows;
     args.groups = args.rows * 4 <= (pair ? 64 : 128) ? 4 : args.rows * 2 <= (pair ? 64 : 128) ? 2 : 1;
-}
-size_t stream_bytes(const StreamArgs &args, bool two_buffers, size_t tables) {
-    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups;
-    return STREAM_CONTROL + tables + static_cast<size_t>(steps * args.groups) * ATOM * (two_buffers ? 2 : 1);
+    while (args.groups * args.width > MAX_LANES) args.groups /= 2;
+    args.span_log = args.rows <= 32 ? 5 : args.rows <= 64 ? 6 : 7;
 }
 // Stages in up to `most` bytes of shared memory, or in all of it where three do not fit into those.  False where three do not
-// fit at all beside the activations' atoms.
-bool plan_stages(StreamArgs &args, size_t most, bool two_buffers, size_t tables, size_t *bytes) {
-    const size_t fixed = stream_bytes(args, two_buffers, tables);
-    if (fixed + 3 * STREAM_STAGE > most) most = SMEM_LIMIT;
-    if (fixed + 3 * STREAM_STAGE > most) return false;
-    args.stages = static_cast<int>(std::min<size_t>(STREAM_MAX_STAGES, (most - fixed) / STREAM_STAGE));
-    *bytes = fixed + static_cast<size_t>(args.stages) * STREAM_STAGE;
+// fit at all.
+template <Mode MODE, bool PREPARED>
+bool plan_stages(StreamArgs &args, size_t most, size_t *bytes) {
+    constexpr bool GROUPED = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN;
+    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups;
+    const size_t atoms = PREPARED ? 0 : static_cast<size_t>(steps * args.groups) * ATOM * (MODE == EXPERTS_DOWN ? 2 : 1);
+    const size_t fixed = STREAM_CONTROL + STREAM_SUMS<PREPARED> + (GROUPED ? STREAM_ROUTES : 0) + atoms;
+    const size_t stage = STREAM_STAGE + (PREPARED ? static_cast<size_t>(std::max(16, args.groups * args.width)) * BLOCK_K : 0);
+    if (fixed + 3 * stage > most) most = SMEM_LIMIT;
+    if (fixed + 3 * stage > most) return false;
+    args.stages = static_cast<int>(std::min<size_t>(STREAM_MAX_STAGES, (most - fixed) / stage));
+    *bytes = fixed + static_cast<size_t>(args.stages) * stage;
     return true;
 }
 // Where a CTA's share of the weights is small, half of a multiprocessor's shared memory does: a CTA of the next call can
@@ -1305,19 +1368,25 @@ size_t stream_share(const StreamArgs &args) {
     const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, count = multiprocessors(), steps = (args.row_tiles + count - 1) / count * ((blocks + args.groups - 1) / args.groups);
     return steps <= STREAM_SMALL_SHARE ? SMEM_HALF : SMEM_LIMIT;
 }
-template <Mode MODE>
+template <Mode MODE, bool PREPARED>
 cudaError_t launch_stream(const StreamArgs &args, int tiles, size_t bytes, cudaStream_t stream) {
-    const cudaError_t status = allow_shared_memory<int8_stream_kernel<MODE>>(SMEM_LIMIT);
+    const cudaError_t status = allow_shared_memory<int8_stream_kernel<MODE, PREPARED>>(SMEM_LIMIT);
     if (status != cudaSuccess) return status;
-    return launch_dependent(int8_stream_kernel<MODE>, dim3(std::min(tiles, multiprocessors())), dim3(STREAM_THREADS), bytes, 1, stream, args);
+    return launch_dependent(int8_stream_kernel<MODE, PREPARED>, dim3(std::min(tiles, multiprocessors())), dim3(STREAM_THREADS), bytes, 1, stream, args);
 }
 
-// The activations of a linear in the caller's scratch buffer: whole numbers, then one scale per lane.
+// Lanes of a block of the few-lane kernel's activations.
+int stream_width(int lanes) { return lanes <= FEW ? FEW : (lanes + 15) / 16 * 16; }
+// The activations of a linear in the caller's scratch buffer: whole numbers, as rows or as blocks of 128 columns, then one scale per
+// lane.
+size_t row_bytes(int lanes, int k) {
+    return padded(lanes <= STREAM_LANES ? static_cast<size_t>((k + BLOCK_K - 1) / BLOCK_K) * BLOCK_K * stream_width(lanes) : static_cast<size_t>(lanes) * k);
+}
 struct Int8Rows {
     int8_t *values;
     float *scales;
     Int8Rows(void *scratch, int lanes, int k)
-        : values(static_cast<int8_t *>(scratch)), scales(reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + padded(static_cast<size_t>(lanes) * k))) {}
+        : values(static_cast<int8_t *>(scratch)), scales(reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + row_bytes(lanes, k))) {}
 };
 
 // gate alone (up == nullptr) or the pair.
@@ -1325,18 +1394,24 @@ template <Mode MODE>
 cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales, const int8_t *up, const float *up_scales, void *y, const uint16_t *residual, void *scratch,
                          int lanes, int n, int k, int to_f32, int *error_flag, cudaStream_t stream) {
     constexpr bool TWO = MODE == PAIR;
-    if (lanes <= FEW && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
-        StreamArgs args = {};
-        args.x = x, args.scales = scales, args.up_scales = up_scales, args.y = y, args.residual = residual;
-        args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
-        plan_stream(args, 1, TWO);
-        size_t bytes;
-        if (plan_stages(args, stream_share(args), false, 0, &bytes)) {
-            if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows))) return cudaErrorInvalidValue;
-            return launch_stream<MODE>(args, args.row_tiles, bytes, stream);
-        }
-    }
     const Int8Rows rows(scratch, lanes, k);
+    if (lanes <= STREAM_LANES) {
+        StreamArgs args = {};
+        args.x = x, args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
+        args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
+        args.width = stream_width(lanes);
+        plan_stream(args, 1, TWO);
+        if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows))) return cudaErrorInvalidValue;
+        size_t bytes;
+        if (lanes <= FEW && static_cast<int64_t>(lanes) * k <= STREAM_OWN && reinterpret_cast<uintptr_t>(x) % 16 == 0 && plan_stages<MODE, false>(args, stream_share(args), &bytes))
+            return launch_stream<MODE, false>(args, args.row_tiles, bytes, stream);
+        const cudaError_t status =
+            launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream, args.width);
+        if (status != cudaSuccess) return status;
+        args.x = rows.values;
+        if (!plan_stages<MODE, true>(args, stream_share(args), &bytes)) return cudaErrorInvalidValue;  // (three stages always fit)
+        return launch_stream<MODE, true>(args, args.row_tiles, bytes, stream);
+    }
     const cudaError_t status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream);
     if (status != cudaSuccess) return status;
     Int8Args args = {};
@@ -1351,7 +1426,7 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
 
 }  // namespace
 
-size_t linear_int8_scratch_bytes(int lanes, int k) { return padded(static_cast<size_t>(lanes) * k) + static_cast<size_t>(lanes) * sizeof(float); }
+size_t linear_int8_scratch_bytes(int lanes, int k) { return row_bytes(lanes, k) + static_cast<size_t>(lanes) * sizeof(float); }
 
 cudaError_t launch_linear_int8(const uint16_t *x, const int8_t *w, const float *scales, void *y, const uint16_t *residual, void *scratch, int lanes, int n, int k, int to_f32,
                                int *error_flag, cudaStream_t stream) {
@@ -1447,16 +1522,17 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
         second.n = hidden, second.k = inter, second.x = part.h, second.scales = down_scales, second.y = part.parts;
         for (StreamArgs *args : {&first, &second}) {
             args->lanes = tokens, args->ids = ids, args->weights_of = weights, args->top_k = top_k, args->experts = experts, args->error_flag = error_flag;
+            args->width = FEW;
             plan_stream(*args, std::min(experts, pairs), args == &first);
         }
         size_t first_bytes, second_bytes;
-        if (plan_stages(first, SMEM_LIMIT, false, STREAM_ROUTES, &first_bytes) && plan_stages(second, SMEM_HALF, true, STREAM_ROUTES, &second_bytes)) {
+        if (plan_stages<EXPERTS_PAIR, false>(first, SMEM_LIMIT, &first_bytes) && plan_stages<EXPERTS_DOWN, false>(second, SMEM_HALF, &second_bytes)) {
             if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) ||
                 !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows))
                 return cudaErrorInvalidValue;
-            cudaError_t status = launch_stream<EXPERTS_PAIR>(first, std::min(experts, pairs) * first.row_tiles, first_bytes, stream);
+            cudaError_t status = launch_stream<EXPERTS_PAIR, false>(first, std::min(experts, pairs) * first.row_tiles, first_bytes, stream);
             if (status != cudaSuccess) return status;
-            status = launch_stream<EXPERTS_DOWN>(second, std::min(experts, pairs) * second.row_tiles, second_bytes, stream);
+            status = launch_stream<EXPERTS_DOWN, false>(second, std::min(experts, pairs) * second.row_tiles, second_bytes, stream);
             return status != cudaSuccess ? status : sum();
         }
     }

@@ -16,6 +16,7 @@ pytestmark = pytest.mark.gpu
 SHAPES = [  # lanes, n, k: one lane to several tiles of 256, ragged rows and tails of K, more and fewer tiles than multiprocessors
     (1, 8, 16), (1, 1, 128), (2, 7, 32), (3, 129, 112), (8, 272, 256), (9, 96, 400), (16, 130, 1024), (17, 1031, 2032), (37, 256, 144), (64, 40, 4096), (129, 300, 512),
     (255, 64, 128), (256, 128, 128), (257, 257, 272), (300, 1030, 640), (1025, 72, 96), (1, 4096, 4096), (4, 20000, 128), (5, 1024, 14336), (520, 4096, 2048),
+    (8, 20000, 2176), (16, 200, 16), (33, 20000, 272), (65, 9500, 400), (113, 4096, 1040), (128, 257, 5008), (127, 19000, 128),
 ]
 
 
