@@ -1108,7 +1108,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                     const int lanes = min(CHUNK, a.lanes - chunk);
                     auto value_of = [&](int token, float scale) {
                         int sum = 0, up_sum = 0;
-                        for (int g = 0; g < a.groups; g++) {
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            if (g >= a.groups) break;
                             sum += sums[token][g * slot_rows + row];
                             if (TWO) up_sum += sums[token][g * slot_rows + slot_rows / 2 + row];
                         }
@@ -1130,17 +1132,17 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
                         }
                     } else {
                         for (int token = first_lane; token < lanes; token += 4 * lane_step) {
-                            float value[4];
+                            float value[4];  // four lanes side by side, past the last one the last one again
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                if (token + i * lane_step >= lanes) break;
-                                value[i] = value_of(token + i * lane_step, scales[chunk + token + i * lane_step]);
+                                const int at = min(token + i * lane_step, lanes - 1);
+                                value[i] = value_of(at, scales[chunk + at]);
                                 if (MODE == LINEAR && a.residual != nullptr) value[i] = __fadd_rn(value[i], bf16_bits_to_f32(beside[i]));
                             }
                             if (MODE == LINEAR && a.residual != nullptr) fetch_beside(token + 4 * lane_step < lanes ? chunk + token + 4 * lane_step : chunk + teams * CHUNK + first_lane);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                if (token + i * lane_step >= lanes) break;
+                                if (token + i * lane_step >= lanes) continue;
                                 const size_t out = static_cast<size_t>(chunk + token + i * lane_step) * a.n + channel;
                                 if (MODE == LINEAR && a.to_f32) static_cast<float *>(a.y)[out] = value[i];
                                 else static_cast<uint16_t *>(a.y)[out] = to_bf16(value[i]);
@@ -1293,12 +1295,14 @@ cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
     return launch_dependent(int8_gemm_kernel<MODE>, dim3(2 * std::min(most_tiles, multiprocessors() / 2)), dim3(THREADS), bytes, 1, stream, args);
 }
 
+// A tile's outputs, however many of the 128 rows it has.
+int64_t output_cycles(int lanes, bool pair) { return lanes * (pair ? 34 : 18); }
 // Tiles of a matrix of n output channels (`pair`: two weight rows each) for that many lanes, by an estimate of the cycles
-// they take: of a block of 128 columns the tensor pipe needs half the lanes' number for each of four instructions a matrix
-// (the waits around them 310 at least), the copies arrive at some 56 bytes per cycle and multiprocessor, and the weights,
-// which the first of a row's tiles brings in, at some 23; and every tile has its start and end, outputs that no other tile's
-// sums hide (the last one's, and all of a pair's with one accumulator) among them.
-void plan_dense(Int8Args &args, bool pair) {
+// they take, which it returns: of a block of 128 columns the tensor pipe needs half the lanes' number for each of four instructions a matrix
+// (the waits around them 330 at least), the copies arrive at some 56 bytes per cycle and multiprocessor, and the weights,
+// which the first of a row's tiles brings in, at some 23; the outputs hide behind the next tile's sums, but for the last one's
+// and all of a pair's whose two accumulators do not fit tensor memory.
+int64_t plan_dense(Int8Args &args, bool pair) {
     const int pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1;
     const int padded = (args.lanes + 31) / 32 * 32, least = (padded + MAX_LANES - 1) / MAX_LANES;
     int64_t best = 0;
@@ -1306,9 +1310,9 @@ void plan_dense(Int8Args &args, bool pair) {
         const int lanes = ((padded + split - 1) / split + 31) / 32 * 32, lane_tiles = (padded + lanes - 1) / lanes;
         for (int rows = ROWS; rows >= 8; rows -= 8) {  // (in steps of sixteen bytes of outputs)
             const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
-            const int tensor = matrices * std::max(2 * lanes, 310), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
-            const int64_t outputs = 12 * lanes * matrices, shown = 2 * matrices * lanes <= 512 ? 1 : waves;
-            const int64_t cost = static_cast<int64_t>(waves) * (static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000) + shown * outputs;
+            const int tensor = matrices * std::max(2 * lanes, 330), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
+            const int64_t sums = static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000, outputs = output_cycles(lanes, pair);
+            const int64_t cost = waves * (2 * matrices * lanes <= 512 ? std::max(sums, outputs) : sums + outputs) + outputs;
             if (best != 0 && cost >= best) continue;
             best = cost;
             args.rows = rows;
@@ -1317,6 +1321,7 @@ void plan_dense(Int8Args &args, bool pair) {
             args.lane_tiles = lane_tiles;
         }
     }
+    return best;
 }
 
 }  // namespace
@@ -1326,8 +1331,9 @@ namespace {
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Tiles of `matrices` matrices of n output channels for the few-lane kernel: as few rows for the busiest CTA as possible, a
-// tile counted as the bytes of four rows more.
-void plan_stream(StreamArgs &args, int matrices, bool pair) {
+// tile counted as the bytes of four rows more.  Returns an estimate of the cycles they take, as plan_dense does: a stage's four
+// instructions take the tensor pipe 290 cycles or twice their N, and the outputs of a tile, lane by lane, are not hidden by much.
+int64_t plan_stream(StreamArgs &args, int matrices, bool pair) {
     const int count = multiprocessors(), most = std::min(pair ? 64 : 128, args.n);
     int64_t best = 0;
     for (int waves = 1, tries = 0; tries < 8; waves++) {  // the fewest rows that many waves have room for
@@ -1345,6 +1351,10 @@ void plan_stream(StreamArgs &args, int matrices, bool pair) {
     args.groups = args.rows * 4 <= (pair ? 64 : 128) ? 4 : args.rows * 2 <= (pair ? 64 : 128) ? 2 : 1;
     while (args.groups * args.width > MAX_LANES) args.groups /= 2;
     args.span_log = args.rows <= 32 ? 5 : args.rows <= 64 ? 6 : 7;
+    const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups, weight_rows = args.groups * args.rows * (pair ? 2 : 1);
+    const int tensor = std::max(290, 2 * args.groups * args.width), copies = (weight_rows + args.groups * args.width) * BLOCK_K / 56, memory = weight_rows * BLOCK_K / 23;
+    const int64_t waves = (static_cast<int64_t>(matrices) * args.row_tiles + count - 1) / count;
+    return waves * (static_cast<int64_t>(steps) * std::max({tensor, copies, memory}) + 900 + args.lanes * (20 + (57 << args.span_log) / 128));
 }
 // Stages in up to `most` bytes of shared memory, or in all of it where three do not fit into those.  False where three do not
 // fit at all.
@@ -1395,28 +1405,30 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
                          int lanes, int n, int k, int to_f32, int *error_flag, cudaStream_t stream) {
     constexpr bool TWO = MODE == PAIR;
     const Int8Rows rows(scratch, lanes, k);
+    Int8Args args = {};
+    args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
     if (lanes <= STREAM_LANES) {
-        StreamArgs args = {};
-        args.x = x, args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
-        args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
-        args.width = stream_width(lanes);
-        plan_stream(args, 1, TWO);
-        if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows))) return cudaErrorInvalidValue;
+        const bool own = lanes <= FEW && static_cast<int64_t>(lanes) * k <= STREAM_OWN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+        StreamArgs few = {};
+        few.x = x, few.scales = scales, few.up_scales = up_scales, few.lane_scales = rows.scales, few.y = y, few.residual = residual;
+        few.lanes = lanes, few.n = n, few.k = k, few.to_f32 = to_f32, few.error_flag = error_flag;
+        few.width = stream_width(lanes);
         size_t bytes;
-        if (lanes <= FEW && static_cast<int64_t>(lanes) * k <= STREAM_OWN && reinterpret_cast<uintptr_t>(x) % 16 == 0 && plan_stages<MODE, false>(args, stream_share(args), &bytes))
-            return launch_stream<MODE, false>(args, args.row_tiles, bytes, stream);
-        const cudaError_t status =
-            launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream, args.width);
-        if (status != cudaSuccess) return status;
-        args.x = rows.values;
-        if (!plan_stages<MODE, true>(args, stream_share(args), &bytes)) return cudaErrorInvalidValue;  // (three stages always fit)
-        return launch_stream<MODE, true>(args, args.row_tiles, bytes, stream);
+        if (plan_stream(few, 1, TWO) <= plan_dense(args, TWO) || own) {
+            if (!encode(&few.weights, w, n, k, few.rows) || (TWO && !encode(&few.up, up, n, k, few.rows))) return cudaErrorInvalidValue;
+            if (own && plan_stages<MODE, false>(few, stream_share(few), &bytes)) return launch_stream<MODE, false>(few, few.row_tiles, bytes, stream);
+            const cudaError_t status =
+                launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream, few.width);
+            if (status != cudaSuccess) return status;
+            few.x = rows.values;
+            if (!plan_stages<MODE, true>(few, stream_share(few), &bytes)) return cudaErrorInvalidValue;  // (three stages always fit)
+            return launch_stream<MODE, true>(few, few.row_tiles, bytes, stream);
+        }
+    } else {
+        plan_dense(args, TWO);
     }
     const cudaError_t status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream);
     if (status != cudaSuccess) return status;
-    Int8Args args = {};
-    args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
-    plan_dense(args, TWO);
     if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.tile_lanes / 2))
         return cudaErrorInvalidValue;
     args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
@@ -1484,17 +1496,17 @@ int expert_tile_lanes(int pairs, int experts) {
     while (lanes < 2 * share && lanes < 128) lanes *= 2;
     return lanes;
 }
-// As plan_dense, for as many lane tiles as there are experts, each with its even share.
+// As plan_dense, for the tiles that experts with even shares have.
 void plan_experts(Int8Args &args, int pairs, int experts, bool pair) {
     args.tile_lanes = expert_tile_lanes(pairs, experts);
-    const int count = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1, tiles = std::min(experts, pairs),
-              share = (pairs / tiles + 31) / 32 * 32;
+    const int used = std::min(experts, pairs), share = (pairs + used - 1) / used, lane_tiles = (share + args.tile_lanes - 1) / args.tile_lanes;
+    const int count = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1, lanes = std::min((share + 31) / 32 * 32, args.tile_lanes);
     int64_t best = 0;
     for (int rows = ROWS; rows >= 16; rows -= 8) {
-        const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * tiles + count - 1) / count;
-        const int tensor = matrices * std::max(2 * std::min(share, args.tile_lanes), 310), copies = (matrices * rows + args.tile_lanes / 2) * BLOCK_K / 56,
-                  memory = matrices * rows * BLOCK_K / 23;
-        const int64_t cost = static_cast<int64_t>(waves) * (static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000);
+        const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows);
+        const int64_t waves = (static_cast<int64_t>(row_tiles) * used * lane_tiles + count - 1) / count;
+        const int tensor = matrices * std::max(2 * lanes, 330), copies = (matrices * rows + args.tile_lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
+        const int64_t cost = waves * std::max(static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000, output_cycles(lanes, pair));
         if (best != 0 && cost >= best) continue;
         best = cost;
         args.rows = rows;

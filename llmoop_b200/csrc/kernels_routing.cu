@@ -205,8 +205,8 @@ __device__ __forceinline__ void load_run(const uint16_t *from, float (&to)[PER_T
 struct Plan {
     Routing routing;
     int per;      // experts of a thread
-    int threads;  // of a group
-    int runs;     // logits and bias lie in runs of `per` = PER_THREAD on boundaries of sixteen (bf16: eight) bytes
+    int threads;  // of a group whose threads hold runs of experts; 0: experts lie 32 apart
+    int wide;     // runs of PER_THREAD logits and biases on boundaries of sixteen (bf16: eight) bytes
 };
 struct Candidates {
     uint32_t expert[32];
@@ -218,20 +218,20 @@ struct Candidates {
 
 // A token whose candidates are found in 32 bits, with a bound on the error, and ranked in 64; false where that is not certain to
 // choose what the definition does.  Without a bias experts are in the order of their logits, which needs no arithmetic; groups of
-// ranks closer than the error are not decided here.  Thread l holds the `per` experts from l * per on, so that a group is a run of
-// threads.
+// ranks closer than the error are not decided here.  Thread l holds the `per` experts from l * per on, where that makes every group a
+// run of threads and leaves few of them idle; else those 32 apart.
 template <typename T, int PER_THREAD>
 __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *bias, int *ids, float *weights, int token, const Plan &plan, Candidates &found) {
     const Routing &routing = plan.routing;
-    const int lane = threadIdx.x & 31, experts = routing.experts, per = plan.per, base = lane * per;
+    const int lane = threadIdx.x & 31, experts = routing.experts, per = plan.per, base = plan.threads > 0 ? lane * per : lane, step = plan.threads > 0 ? 1 : 32;
     const T *row = logits + static_cast<size_t>(token) * experts;
     const float infinity = __uint_as_float(0x7f800000u);
     float logit[PER_THREAD], score[PER_THREAD];
-    if (plan.runs) {
+    if (plan.wide) {
         load_run<PER_THREAD>(row + base, logit);
     } else {
 #pragma unroll
-        for (int j = 0; j < PER_THREAD; j++) logit[j] = j < per && base + j < experts ? logit_of(row, base + j) : -infinity;
+        for (int j = 0; j < PER_THREAD; j++) logit[j] = j < per && base + j * step < experts ? logit_of(row, base + j * step) : -infinity;
     }
     float top = -infinity;
 #pragma unroll
@@ -257,11 +257,11 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
     uint32_t key[PER_THREAD];  // of the choice, or of the logit; 0: closed
     if (bias != nullptr) {
         float own[PER_THREAD];
-        if (plan.runs) {
+        if (plan.wide) {
             load_run<PER_THREAD>(bias + base, own);
         } else {
 #pragma unroll
-            for (int j = 0; j < PER_THREAD; j++) own[j] = j < per && base + j < experts ? bias[base + j] : 0.0f;
+            for (int j = 0; j < PER_THREAD; j++) own[j] = j < per && base + j * step < experts ? bias[base + j * step] : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < PER_THREAD; j++) {
@@ -273,27 +273,48 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         for (int j = 0; j < PER_THREAD; j++) key[j] = logit[j] > -infinity ? key_of(logit[j] + 0.0f) : 0u;
     }
     if (routing.groups > 1) {
-        const int threads = plan.threads, own_group = lane / threads, first = own_group * threads;
         const bool by_score = bias == nullptr && scored;
-        uint32_t best = 0, next = 0;
+        auto value_at = [&](int j) { return by_score && key[j] != 0 ? key_of(score[j]) : key[j]; };
+        const int threads = plan.threads, size = experts / routing.groups;
+        uint32_t group_best = 0, group_next = 0;  // of the group of number own_group
+        int own_group = lane;
+        if (threads > 0) {
+            own_group = lane / threads;
+            const int first = own_group * threads;
+            uint32_t best = 0, next = 0;
 #pragma unroll
-        for (int j = 0; j < PER_THREAD; j++) {
-            const uint32_t value = by_score && key[j] != 0 ? key_of(score[j]) : key[j];
-            next = max(next, min(best, value));
-            best = max(best, value);
-        }
-        uint32_t group_best = 0, group_next = 0;
-        for (int other = 0; other < threads; other++) {
-            const uint32_t b = __shfl_sync(0xffffffffu, best, first + other), n = __shfl_sync(0xffffffffu, next, first + other);
-            group_next = max(max(group_next, n), min(group_best, b));
-            group_best = max(group_best, b);
+            for (int j = 0; j < PER_THREAD; j++) {
+                const uint32_t value = value_at(j);
+                next = max(next, min(best, value));
+                best = max(best, value);
+            }
+            for (int other = 0; other < threads; other++) {
+                const uint32_t b = __shfl_sync(0xffffffffu, best, first + other), n = __shfl_sync(0xffffffffu, next, first + other);
+                group_next = max(max(group_next, n), min(group_best, b));
+                group_best = max(group_best, b);
+            }
+        } else {
+            for (int group = 0; group < routing.groups; group++) {
+                uint32_t best = 0, next = 0;
+#pragma unroll
+                for (int j = 0; j < PER_THREAD; j++) {
+                    const int expert = base + j * step;
+                    const uint32_t value = expert >= group * size && expert < (group + 1) * size ? value_at(j) : 0u;
+                    next = max(next, min(best, value));
+                    best = max(best, value);
+                }
+                const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+                const int holder = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
+                const uint32_t second = __reduce_max_sync(0xffffffffu, lane == holder ? next : best);
+                if (lane == group) group_best = most, group_next = second;
+            }
         }
         const bool open = own_group < routing.groups && group_best != 0;
         float rank = open ? value_of(group_best) : -infinity;
         if (routing.group_scores > 1 && open && group_next != 0) rank += value_of(group_next);
         int before = 0;
         for (int group = 0; group < routing.groups; group++) {
-            const float other = __shfl_sync(0xffffffffu, rank, group * threads);
+            const float other = __shfl_sync(0xffffffffu, rank, group * max(threads, 1));
             before += other > rank || (other == rank && group < own_group);
         }
         const bool kept = open && before < routing.chosen_groups;
@@ -302,8 +323,15 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
             const float in = value_of(last_kept), out = value_of(first_left);
             if (scored ? !(in - out > margin(in)) : in == out) return false;
         }
+        if (threads > 0) {
 #pragma unroll
-        for (int j = 0; j < PER_THREAD; j++) key[j] = kept ? key[j] : 0u;
+            for (int j = 0; j < PER_THREAD; j++) key[j] = kept ? key[j] : 0u;
+        } else {
+            const uint32_t all_kept = __ballot_sync(0xffffffffu, kept);
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; j++)
+                if (key[j] != 0 && !((all_kept >> ((base + j * step) / size)) & 1u)) key[j] = 0;
+        }
     }
     // The top_k-th largest of the threads' own largest keys is no more than the top_k-th largest of all: what is not further below
     // it than the error is a candidate, few more than top_k.
@@ -324,7 +352,7 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         const uint32_t all = __ballot_sync(0xffffffffu, candidate);
         const int place = count + __popc(all & ((1u << lane) - 1u));
         if (candidate && place < 32) {
-            found.expert[place] = static_cast<uint32_t>(base + j);
+            found.expert[place] = static_cast<uint32_t>(base + j * step);
             found.logit[place] = logit[j];
         }
         count += __popc(all);
@@ -384,7 +412,7 @@ __global__ void __launch_bounds__(32 * TOKENS_PER_CTA) route_experts_kernel(cons
     grid_dependency_wait();
     const int warp = static_cast<int>(threadIdx.x >> 5), token = blockIdx.x * TOKENS_PER_CTA + warp;
     if (token >= tokens) return;
-    if (plan.routing.top_k <= 32 && plan.per <= PER_THREAD && route_in_32_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan, found[warp])) return;
+    if (plan.routing.top_k <= 32 && route_in_32_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan, found[warp])) return;
     route_in_64_bits<T, PER_THREAD>(logits, bias, ids, weights, token, plan.routing);
 }
 
@@ -394,18 +422,18 @@ cudaError_t launch(const T *logits, const float *bias, int *ids, float *weights,
     Plan plan = {};
     plan.routing = routing;
     plan.per = (routing.experts + 31) / 32;
-    if (routing.groups > 1) {  // as many threads to a group as make runs of equal length
-        const int size = routing.experts / routing.groups;
-        plan.threads = std::min(size, 32 / routing.groups);
-        while (size % plan.threads != 0) plan.threads--;
-        plan.per = size / plan.threads;
-    }
+    const int size = routing.experts / routing.groups;
+    for (int threads = std::min(size, 32 / routing.groups); threads * routing.groups > 16; threads--)  // (of a group, all of whose threads hold as many)
+        if (size % threads == 0 && size / threads <= 32) {
+            plan.threads = threads;
+            plan.per = size / threads;
+            break;
+        }
     auto with = [&](auto kernel, int per_thread) {
-        plan.runs = per_thread % 4 == 0 && routing.experts == 32 * per_thread && plan.per == per_thread && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 &&
+        plan.wide = per_thread % 4 == 0 && routing.experts == 32 * per_thread && plan.threads > 0 && plan.per == per_thread && reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 &&
                     reinterpret_cast<uintptr_t>(bias) % 16 == 0;
         return launch_dependent(kernel, grid, block, 0, 1, stream, logits, bias, ids, weights, tokens, plan);
     };
-    // (the form in 64 bits has its experts 32 apart; a single group of 1024 takes 32 to a thread in either)
     if (plan.per <= 1) return with(route_experts_kernel<T, 1>, 1);
     if (plan.per <= 2) return with(route_experts_kernel<T, 2>, 2);
     if (plan.per <= 4) return with(route_experts_kernel<T, 4>, 4);

@@ -183,7 +183,8 @@ ROUTINGS = [
     dict(experts=1, top_k=1), dict(experts=2, top_k=1, sigmoid=True), dict(experts=8, top_k=8), dict(experts=33, top_k=5), dict(experts=60, top_k=6, renormalise=False),
     dict(experts=64, top_k=6, groups=8, chosen_groups=3, group_scores=1), dict(experts=128, top_k=8), dict(experts=160, top_k=6, groups=8, chosen_groups=3, renormalise=False, scale=16.0),
     dict(experts=256, top_k=8, sigmoid=True, groups=8, chosen_groups=4, group_scores=2, scale=2.5), dict(experts=300, top_k=64, sigmoid=True), dict(experts=512, top_k=33),
-    dict(experts=1024, top_k=16, groups=32, chosen_groups=9, group_scores=2), dict(experts=96, top_k=12, groups=3, chosen_groups=1, group_scores=2),
+    dict(experts=1024, top_k=16, groups=32, chosen_groups=9, group_scores=2), dict(experts=561, top_k=9), dict(experts=244, top_k=15, groups=4, chosen_groups=1, group_scores=2),
+    dict(experts=200, top_k=15, groups=8, chosen_groups=5), dict(experts=1022, top_k=6, groups=2, chosen_groups=1, group_scores=2), dict(experts=96, top_k=12, groups=3, chosen_groups=1, group_scores=2),
 ]
 
 
