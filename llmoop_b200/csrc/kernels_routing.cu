@@ -237,8 +237,8 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
 #pragma unroll
     for (int j = 0; j < PER_THREAD; j++) top = fmaxf(top, logit[j]);
     top = value_of(__reduce_max_sync(0xffffffffu, key_of(top)));
-    // (the scores of larger logits meet in 64 bits, too, or have no f32 form)
-    if (top == infinity || (routing.sigmoid && top > 30.0f)) return false;
+    // (the sigmoids of larger logits next to one another meet in 64 bits)
+    if (top == infinity || (routing.sigmoid && top > 20.0f)) return false;
     const bool scored = bias != nullptr || (routing.groups > 1 && routing.group_scores > 1);
     if (scored && routing.sigmoid) {
 #pragma unroll
@@ -319,9 +319,9 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         }
         const bool kept = open && before < routing.chosen_groups;
         const uint32_t first_left = __reduce_max_sync(0xffffffffu, open && !kept ? key_of(rank) : 0u), last_kept = __reduce_min_sync(0xffffffffu, kept ? key_of(rank) : 0xffffffffu);
-        if (first_left != 0) {  // (equal logits are equal scores; whatever else lies close is not decided here)
+        if (first_left != 0) {  // (logits as close as 1e-12 may be one score in 64 bits)
             const float in = value_of(last_kept), out = value_of(first_left);
-            if (scored ? !(in - out > margin(in)) : in == out) return false;
+            if (!(in - out > (scored ? margin(in) : 1e-12f))) return false;
         }
         if (threads > 0) {
 #pragma unroll
@@ -346,9 +346,11 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
     if (limit == 0) limit = 1;  // all that are open
     else if (bias != nullptr) limit = key_of(value_of(limit) - margin(value_of(limit)));
     int count = 0;
+    uint32_t left = 0;  // the largest that is no candidate
 #pragma unroll
     for (int j = 0; j < PER_THREAD; j++) {
         const bool candidate = key[j] >= limit;
+        left = max(left, candidate ? 0u : key[j]);
         const uint32_t all = __ballot_sync(0xffffffffu, candidate);
         const int place = count + __popc(all & ((1u << lane) - 1u));
         if (candidate && place < 32) {
@@ -357,9 +359,10 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         }
         count += __popc(all);
     }
-    if (count > 32) return false;
+    if (count > 31) return false;
+    left = bias == nullptr ? __reduce_max_sync(0xffffffffu, left) : 0u;  // (with a bias the margin keeps it apart)
     __syncwarp();
-    // one candidate to a thread: its score in 64 bits, and the number of those in front of it
+    // one candidate to a thread: its score in 64 bits, and the number of those in front of it; to the next thread the logit that is left
     double sum = 0.0;  // of the softmax's terms, where more than their order and ratios count
     if (!routing.sigmoid && (bias != nullptr || !routing.renormalise)) {
 #pragma unroll
@@ -370,8 +373,8 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
     }
     const uint32_t my_expert = lane < count ? found.expert[lane] : 0u;
     double own_score = 0.0, choice = 0.0;
-    if (lane < count) {
-        const double own_logit = static_cast<double>(found.logit[lane]);
+    if (lane < count || (lane == count && left != 0)) {
+        const double own_logit = static_cast<double>(lane < count ? found.logit[lane] : value_of(left));
         own_score = exp(routing.sigmoid ? -own_logit : own_logit - static_cast<double>(top));
         if (routing.sigmoid) own_score = 1.0 / (1.0 + own_score);
         else if (sum > 0.0) own_score /= sum;
@@ -379,6 +382,9 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         found.choice[lane] = choice;
     }
     if (__any_sync(0xffffffffu, lane < count && own_score < 1e-250)) return false;  // where scores run out of exponents
+    // candidates whose scores, other than their logits, are no larger than one's that is left: the lower number may be that one's
+    const double left_score = __shfl_sync(0xffffffffu, own_score, count);
+    if (left != 0 && __any_sync(0xffffffffu, lane < count && own_score <= left_score)) return false;
     __syncwarp();
     int place = 0;
     for (int other = 0; other < count; other++) {

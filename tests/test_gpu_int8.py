@@ -121,6 +121,66 @@ def test_unaligned_inputs_and_what_lies_around_the_outputs():
     assert torch.equal(residual, want)
 
 
+def test_threads_with_streams_and_scratch_of_their_own():
+    import threading
+
+    g = ref.generator(31)
+    layer, (w, scale) = _layer(g, 8, 256, 128), ref.weights(g, 700, 256)
+    jobs = []
+    for tokens in (1, 6, 40, 200):
+        x, (ids, weights) = ref.activations(g, tokens, 256), _routes(g, tokens, 2, 8)
+        jobs.append((x, ids, weights, ref.linear(x, w, scale), ref.experts(x, ids, weights, *layer)))
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(x, ids, weights, want, want_experts):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                outs = [(ref.linear(x, w, scale), ref.experts(x, ids, weights, *layer)) for _ in range(20)]
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, want) and torch.equal(b, want_experts) for a, b in outs)
+        except BaseException as error:
+            failures.append(error)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = [".", "tests"]
+import torch, int8_reference as ref, llmoop_b200 as nb
+library = nb.library()
+g = ref.generator(1)
+w, scale = ref.weights(g, 300, 256)
+for lanes in (3, 50, 400):
+    x, y = ref.activations(g, lanes, 256), torch.zeros((lanes, 300), dtype=torch.bfloat16, device="cuda")
+    buffer = ref.scratch(library.nerve_b200_op_linear_int8_scratch_bytes(lanes, 256))[0]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # the process's first call
+        status = library.nerve_b200_op_linear_int8(*map(ref.pointer, (x, w, scale, y, None, buffer)), lanes, 300, 256, 0, ref.stream())
+        assert status == 0, library.nerve_b200_last_error()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, ref.linear(x, w, scale)) and bool(y.abs().max() > 0)
+print("first call ok")
+"""
+
+
+def test_a_process_may_capture_its_first_call():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    result = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert result.returncode == 0 and "first call ok" in result.stdout, result.stderr[-2000:]
+
+
 def test_calls_in_a_row_with_one_scratch_buffer():
     """Kernels of a call start while the ones in front drain: none may touch what an earlier call still reads."""
     g = ref.generator(5)
@@ -229,6 +289,30 @@ def test_route_experts_next_to_one_another():
     bias = torch.randn(128, generator=g, device="cuda") * 1e-7
     ids, _ = ref.route(logits, bias, r)
     assert torch.equal(ids, _route_reference(logits, bias, r)[0])
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("middle,spread", [(0.0, 1e-20), (0.0, 1e-13), (17.0, 1e-5), (19.9, 1e-4), (25.0, 1e-4), (40.0, 1.0), (-700.0, 1.0), (-760.0, 1.0)])
+def test_route_scores_that_meet_in_64_bits(middle, spread, groups, sigmoid):
+    """Logits that differ and whose scores do not, or hardly: the lower number first.  Two implementations of exp in 64 bits, each
+    within a step of the truth, may order scores that lie within a few steps of one another either way: 1 / (1 + e) is off by at most
+    a step of e's share and two roundings, four steps apart in all.  Where all scores are one number there is one answer."""
+    g = ref.generator(2)
+    r = nb.Routing(experts=96, top_k=6, sigmoid=sigmoid, groups=groups, chosen_groups=max(1, groups // 2), renormalise=False)
+    logits = middle + spread * torch.rand((16, 96), generator=g, device="cuda")
+    if not sigmoid and middle < -100:
+        logits[:, 5] = 0  # the others' terms run out of exponents
+    ids, weights = ref.route(logits, None, r)
+    want_ids, want = _route_reference(logits, None, r)
+    if spread == 1e-20 or (sigmoid and middle == 40.0) or (sigmoid and middle == -760.0):
+        assert torch.equal(ids, want_ids)
+    scores = logits.double()
+    scores = 1 / (1 + torch.exp(-scores)) if sigmoid else torch.softmax(scores, dim=1)
+    chosen, best = scores.gather(1, ids.long()), scores.gather(1, want_ids.long())
+    assert bool(((chosen - best).abs() <= 4 * 2.0 ** -52 * best).all())
+    assert all(len(set(row)) == 6 for row in ids.tolist())
+    assert bool(((weights.double() - want).abs() <= want.abs() * (ref.F32 + 2.0 ** -40) + 1e-44).all())
 
 
 def test_route_leaves_what_lies_behind():
