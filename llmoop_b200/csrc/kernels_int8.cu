@@ -41,6 +41,9 @@ constexpr int OUTPUT_WARPS = 8, THREADS = 128 + 32 * OUTPUT_WARPS;
 constexpr size_t SMEM_LIMIT = 226 * 1024, SMEM_HALF = 112 * 1024;
 constexpr unsigned int SPIN_LIMIT = 1u << 22;  // tries of 1.5 us
 
+constexpr int STREAM_LANES = 128;  // the most of the few-lane kernel
+constexpr int SPLIT_TILES = 32;    // the most tiles whose columns are split
+
 enum Mode { LINEAR, PAIR, EXPERTS_PAIR, EXPERTS_DOWN };
 
 __device__ __forceinline__ uint64_t swizzled_descriptor(uint32_t shared_address) {  // K-major, 128-byte swizzle, 1024 bytes between 8-row atoms
@@ -254,14 +257,15 @@ __device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
 // route, which expert_groups_kernel's one CTA would take 8 us for).  With weights the scale is that of the row times its route's weight.
 // Bound by DRAM for large batches, by the chain of loads, barrier and stores for small ones.
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.  width > 0: in the order of int8_stream_kernel's stages, blocks of
-// 128 columns of that many rows, sixteen bytes of a row swizzled as TMA would.
+// 128 columns of that many rows, sixteen bytes of a row swizzled as TMA would.  zeroed: what the kernel behind wants to find at zero.
 template <typename T, typename Held, int HELD, bool WARP>
 __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *q, float *scales, const int *places,
                                                             const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
-                                                            int k, int wide, int width) {
+                                                            int k, int wide, int width, uint4 *zeroed, int zeroed_count) {
     __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < zeroed_count; i += gridDim.x * blockDim.x) zeroed[i] = make_uint4(0, 0, 0, 0);
     const int at_row = WARP ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
     if (row_count != nullptr) rows = *row_count;
     if (at_row >= rows) return;
@@ -319,12 +323,12 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 // more columns each.
 template <typename T, typename Held, int MOST>
 cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
-                                 int k, cudaStream_t stream, int width = 0) {
+                                 int k, cudaStream_t stream, int width = 0, void *zeroed = nullptr, size_t zeroed_bytes = 0) {
     const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
     auto with = [&](auto kernel, int held, int warp_rows) {
         const int threads = warp_rows != 0 ? 32 * warp_rows : std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
         return launch_dependent(kernel, dim3(warp_rows != 0 ? (rows + warp_rows - 1) / warp_rows : rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, pair_of,
-                                weights, rows, top_k, k, wide, width);
+                                weights, rows, top_k, k, wide, width, static_cast<uint4 *>(zeroed), static_cast<int>(zeroed_bytes / sizeof(uint4)));
     };
     if (parts <= 64 && rows >= 1024) return with(quantise_rows_kernel<T, Held, 2, true>, 2, 8);
     if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1, false>, 1, 0);
@@ -343,6 +347,10 @@ struct Int8Args {
     int *error_flag;
     int rows;  // output channels of a CTA's tile
     int tile_lanes, lane_tiles, row_tiles, stages, wide;  // wide: bf16 outputs and residual in sixteen bytes
+    // splits > 1: as many items to a tile, each a run of its columns; their sums meet in partials (zero before), [tile][CTA][matrix][lane][ROWS],
+    // and the last one, by a count per tile and CTA, writes the outputs
+    int splits;
+    int *partials, *arrived;
     // experts
     const int4 *tiles;
     const int *tile_count, *pair_of;
@@ -388,6 +396,7 @@ struct alignas(16) LaneInfo {
 };
 struct GemmControl {
     LaneInfo lanes[2];
+    int last;
     uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
     uint32_t tmem;
 };
@@ -414,7 +423,7 @@ __device__ __forceinline__ void load_sums(uint32_t address, int (&d)[16]) {
                  : "memory");
 }
 
-template <Mode MODE>
+template <Mode MODE, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr bool GROUPED = MODE == EXPERTS_PAIR || MODE == EXPERTS_DOWN, TWO = MODE == PAIR || MODE == EXPERTS_PAIR;
@@ -429,7 +438,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                    acc_empty = shared_address(control.acc_empty);
     // the first CTA's barriers, which both CTAs' copies and outputs report to
     const uint32_t leader_full = of_rank(full, 0), leader_acc_empty = of_rank(acc_empty, 0);
-    const int blocks = (a.k + BLOCK_K - 1) / BLOCK_K;
+    const int blocks = (a.k + BLOCK_K - 1) / BLOCK_K, splits = SPLIT ? a.splits : 1;
+    // item `index`: a tile, or a run of a tile's blocks
+    auto tile_of = [&](int index) { return tile_at<MODE>(a, SPLIT ? index / splits : index, rank); };
+    auto first_block = [&](int index) { return SPLIT ? blocks * (index % splits) / splits : 0; };  // (1024 blocks at most)
+    auto last_block = [&](int index) { return SPLIT ? blocks * (index % splits + 1) / splits : blocks; };
     if (threadIdx.x == 32) prefetch_map(&a.weights);
     if (threadIdx.x == 64) prefetch_map(&a.activations);
     if (MODE == PAIR && threadIdx.x == 96) prefetch_map(&a.up);
@@ -468,21 +481,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         uint32_t parity = 1;  // the first round waits for no release
         if (!GROUPED && lane < MATRICES) {
             int row;
-            const CUtensorMap *map = weights_of<MODE>(a, tile_at<MODE>(a, pair, rank), lane, &row);
-            for (int block = 0; block < min(a.stages, blocks); block++) prefetch_tile(map, block * BLOCK_K, row);
+            const CUtensorMap *map = weights_of<MODE>(a, tile_of(pair), lane, &row);
+            for (int block = first_block(pair), s = 0; block < last_block(pair) && s < a.stages; block++, s++) prefetch_tile(map, block * BLOCK_K, row);
         }
         grid_dependency_wait();
-        const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
+        const int items = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles * splits;
         const uint32_t bytes = 2 * (static_cast<uint32_t>(MATRICES * a.rows) * BLOCK_K + half_box);  // of both CTAs
         bool alive = true;
-        Tile tile = pair < tiles ? tile_at<MODE>(a, pair, rank) : Tile{};
-        for (int index = pair; index < tiles && alive; index += pairs) {
-            const Tile next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, rank) : tile;
+        Tile tile = pair < items ? tile_of(pair) : Tile{};
+        for (int index = pair; index < items && alive; index += pairs) {
+            const Tile next = index + pairs < items ? tile_of(index + pairs) : tile;
             int row;
             const CUtensorMap *map = lane < MATRICES ? weights_of<MODE>(a, tile, lane, &row) : &a.activations;
             const uint32_t offset = static_cast<uint32_t>(lane) * a_bytes;
             if (lane == MATRICES) row = tile.lane0 + rank * ((tile.count + 31) / 32 * 16);
-            for (int block = 0; block < blocks; block++) {
+            for (int block = first_block(index), end = last_block(index); block < end; block++) {
                 if (!wait_barrier(empty + stage * 8, parity, a.error_flag)) {
                     for (int s = 0; rank == 0 && s < a.stages && s < issued; s++) {  // the copies in flight land before the CTAs give their memory up
                         const int which = (issued - 1 - s) % a.stages;
@@ -516,10 +529,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         uint32_t parity = 0, last_width = 0;
         bool alive = rank == 0;
         grid_dependency_wait();
-        const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
-        int count = alive && pair < tiles ? tile_at<MODE>(a, pair, 0).count : 0;
-        for (int index = pair; index < tiles && alive; index += pairs, round++) {
-            const int next = index + pairs < tiles ? tile_at<MODE>(a, index + pairs, 0).count : 0;
+        const int items = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles * splits;
+        int count = alive && pair < items ? tile_of(pair).count : 0;
+        for (int index = pair; index < items && alive; index += pairs, round++) {
+            const int next = index + pairs < items ? tile_of(index + pairs).count : 0;
             // instruction descriptor: s32 accumulator, A and B signed bytes, both K-major, N / 8 in bits 17-22, M / 16 in bits 24-28
             // (M = 256 with bytes: N in steps of 32)
             const uint32_t lanes = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>((count + 31) / 32 * 32)), width = MATRICES * lanes;
@@ -529,7 +542,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             if (width + last_width > columns && !wait_barrier(acc_empty + ((round - 1) & 1) * 8, static_cast<uint32_t>(((round - 1) / 2) & 1), a.error_flag)) break;
             last_width = width;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int block = 0; block < blocks; block++) {
+            const int begin = first_block(index), end = last_block(index);
+            for (int block = begin; block < end; block++) {
                 if (!wait_barrier(full + stage * 8, parity, a.error_flag)) {
                     alive = false;
                     break;
@@ -540,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
 #pragma unroll
                     for (int step = 0; step < 4 * MATRICES; step++) {  // K = 32 per instruction
                         const int matrix = step >> 2, part = step & 3;
-                        const uint32_t accumulate = (block > 0 || part > 0) ? 1u : 0u;
+                        const uint32_t accumulate = (block > begin || part > 0) ? 1u : 0u;
                         asm volatile(
                             "{\n"
                             ".reg .pred p;\n"
@@ -551,7 +565,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                             : "memory");
                     }
                     commit_to_pair(empty + stage * 8);
-                    if (block == blocks - 1) commit_to_pair(acc_full + (round & 1) * 8);
+                    if (block == end - 1) commit_to_pair(acc_full + (round & 1) * 8);
                 }
                 __syncwarp();
                 if (++stage == a.stages) {
@@ -563,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         }
     } else if (warp >= 4) {  // ---- outputs: thread = row of the accumulator
         grid_dependency_wait();
-        const int tiles = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles;
+        const int items = (GROUPED ? *a.tile_count : a.lane_tiles) * a.row_tiles * splits;
         const int quarter = warp & 3, part = (warp - 4) >> 2, thread = threadIdx.x - 128, row = quarter * 32 + lane;
         // what a tile's outputs take besides its sums; fetched a tile ahead
         struct Extra {
@@ -591,12 +605,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
         int round = 0;
         Tile tile = {}, next = {};
         Extra extra = {};
-        if (pair < tiles) {
-            tile = tile_at<MODE>(a, pair, rank);
-            if (pair + pairs < tiles) next = tile_at<MODE>(a, pair + pairs, rank);
+        if (pair < items) {
+            tile = tile_of(pair);
+            if (pair + pairs < items) next = tile_of(pair + pairs);
             extra = fetch(tile);
         }
-        for (int index = pair; index < tiles; index += pairs, round++) {
+        for (int index = pair; index < items; index += pairs, round++) {
             LaneInfo &info = control.lanes[round & 1];  // (what stood there two tiles before is out: all threads have passed the last tile's barrier)
             info.scale[thread] = extra.scale;
             info.to[thread] = extra.to;
@@ -604,12 +618,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
             if (!all_of<1, 32 * OUTPUT_WARPS>(wait_barrier(acc_full + (round & 1) * 8, static_cast<uint32_t>((round / 2) & 1), a.error_flag))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             Tile after = {};
-            if (index + 2 * pairs < tiles) after = tile_at<MODE>(a, index + 2 * pairs, rank);
-            if (index + pairs < tiles) extra = fetch(next);
+            if (index + 2 * pairs < items) after = tile_of(index + 2 * pairs);
+            if (index + pairs < items) extra = fetch(next);
             const uint32_t width = width_of(tile.count), accumulator = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + ((round & 1) != 0 ? columns - width : 0u);
             const int channel = tile.row0 + row;
             const bool in_range = row < a.rows && channel < a.n;
-            if (quarter * 32 < a.rows) {
+            int *const partials = SPLIT ? a.partials + static_cast<size_t>(index / splits * 2 + rank) * MATRICES * a.tile_lanes * ROWS + row : nullptr;
+            bool writes = true;
+            if (SPLIT) {
+                if (quarter * 32 < a.rows)
+                    for (int column = part * 16; column < tile.count; column += 32) {
+#pragma unroll
+                        for (int matrix = 0; matrix < MATRICES; matrix++) {
+                            int sums[16];
+                            load_sums(accumulator + matrix * (width / 2) + static_cast<uint32_t>(column), sums);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            int *const to = partials + static_cast<size_t>(matrix * a.tile_lanes + column) * ROWS;
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                atomicAdd(to + i * ROWS, sums[i]);  // (what lies behind the tile's rows and lanes is added too, and not read)
+                        }
+                    }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive_at(leader_acc_empty + (round & 1) * 8);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (thread == 0) {  // for all: a fence covers what the barrier has shown this thread
+                    __threadfence();
+                    control.last = atomicAdd(a.arrived + index / splits * 2 + rank, 1) == splits - 1;
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                writes = control.last != 0;
+            }
+            if (quarter * 32 < a.rows && writes) {
                 const uint16_t *residual = MODE == LINEAR ? a.residual : nullptr;
                 // Wide outputs: thread = eight channels of lanes lane / 4 and lane / 4 + 8.  What is added to them is fetched a step ahead.
                 const bool wide = (MODE == LINEAR || MODE == PAIR) && a.wide;
@@ -635,8 +677,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                 }
                 for (int column = part * 16; column < tile.count; column += 32) {
                     int sums[16], up_sums[16];
-                    load_sums(accumulator + static_cast<uint32_t>(column), sums);
-                    if (TWO) load_sums(accumulator + width / 2 + static_cast<uint32_t>(column), up_sums);
+                    if (SPLIT) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            sums[i] = __ldcg(partials + static_cast<size_t>(column + i) * ROWS);
+                            if (TWO) up_sums[i] = __ldcg(partials + static_cast<size_t>(a.tile_lanes + column + i) * ROWS);
+                        }
+                    } else {
+                        load_sums(accumulator + static_cast<uint32_t>(column), sums);
+                        if (TWO) load_sums(accumulator + width / 2 + static_cast<uint32_t>(column), up_sums);
+                    }
                     float scales[16];
                     int to[16];
 #pragma unroll
@@ -703,9 +753,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
                     }
                 }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) arrive_at(leader_acc_empty + (round & 1) * 8);
+            if (!SPLIT) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive_at(leader_acc_empty + (round & 1) * 8);
+            }
             tile = next;
             next = after;
         }
@@ -727,7 +779,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
 //   Up to eight lanes of few columns every CTA quantises itself while its first weights are on their way, and keeps them: one launch.
 //   More are quantised by a kernel in front, which leaves them in this order (PREPARED), and come with every stage.
 // Warps: 0 copies, 1 issues MMAs, 4-7 (PREPARED: 4-11) write outputs, 4-11 (the experts' down product: 8-11) quantise.
-constexpr int FEW = 8, STREAM_LANES = 128, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
+constexpr int FEW = 8, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
 constexpr uint32_t ATOM = 1024, STREAM_STAGE = ROWS * BLOCK_K;
 constexpr int FEW_ROUTES = 128;          // of the experts' form
 constexpr int STREAM_SMALL_SHARE = 48;   // stages
@@ -1298,12 +1350,12 @@ size_t plan_stages(Int8Args &args) {
     return gemm_control<MODE>() + static_cast<size_t>(args.stages - 1) * stage + last;
 }
 
-template <Mode MODE>
-cudaError_t launch_gemm(Int8Args &args, int most_tiles, cudaStream_t stream) {
+template <Mode MODE, bool SPLIT>
+cudaError_t launch_gemm(Int8Args &args, int most_items, cudaStream_t stream) {
     const size_t bytes = plan_stages<MODE>(args);
-    const cudaError_t status = allow_shared_memory<int8_gemm_kernel<MODE>>(SMEM_LIMIT);
+    const cudaError_t status = allow_shared_memory<int8_gemm_kernel<MODE, SPLIT>>(SMEM_LIMIT);
     if (status != cudaSuccess) return status;
-    return launch_dependent(int8_gemm_kernel<MODE>, dim3(2 * std::min(most_tiles, multiprocessors() / 2)), dim3(THREADS), bytes, 1, stream, args);
+    return launch_dependent(int8_gemm_kernel<MODE, SPLIT>, dim3(2 * std::min(most_items, multiprocessors() / 2)), dim3(THREADS), bytes, 1, stream, args);
 }
 
 // A tile's outputs, however many of the 128 rows it has.
@@ -1323,13 +1375,22 @@ int64_t plan_dense(Int8Args &args, bool pair) {
             const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
             const int tensor = matrices * std::max(2 * lanes, 330), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
             const int64_t sums = static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000, outputs = output_cycles(lanes, pair);
-            const int64_t cost = waves * (2 * matrices * lanes <= 512 ? std::max(sums, outputs) : sums + outputs) + outputs;
+            int64_t cost = waves * (2 * matrices * lanes <= 512 ? std::max(sums, outputs) : sums + outputs) + outputs;
+            // few tiles of many columns: several items to a tile, whose sums meet at some 400 a cycle
+            int splits = 1;
+            if (args.lanes > STREAM_LANES && row_tiles * lane_tiles <= SPLIT_TILES) {
+                const int most = std::min(pairs / (row_tiles * lane_tiles), (blocks + 1) / 2);
+                const int64_t added = static_cast<int64_t>(row_tiles * lane_tiles * most) * 2 * rows * lanes * matrices;
+                const int64_t split_cost = static_cast<int64_t>((blocks + most - 1) / std::max(most, 1)) * std::max({tensor, copies, memory}) + 8500 + 3 * outputs + added / 400;
+                if (most > 1 && split_cost < cost) cost = split_cost, splits = most;
+            }
             if (best != 0 && cost >= best) continue;
             best = cost;
             args.rows = rows;
             args.row_tiles = row_tiles;
             args.tile_lanes = lanes;
             args.lane_tiles = lane_tiles;
+            args.splits = splits;
         }
     }
     return best;
@@ -1398,16 +1459,28 @@ cudaError_t launch_stream(const StreamArgs &args, int tiles, size_t bytes, cudaS
 
 // Lanes of a block of the few-lane kernel's activations.
 int stream_width(int lanes) { return lanes <= FEW ? FEW : (lanes + 15) / 16 * 16; }
-// The activations of a linear in the caller's scratch buffer: whole numbers, as rows or as blocks of 128 columns, then one scale per
-// lane.
+// The scratch buffer of a linear: the activations' whole numbers, as rows or as blocks of 128 columns, one scale per lane, and for many
+// lanes the sums of tiles whose columns are split.
 size_t row_bytes(int lanes, int k) {
     return padded(lanes <= STREAM_LANES ? static_cast<size_t>((k + BLOCK_K - 1) / BLOCK_K) * BLOCK_K * stream_width(lanes) : static_cast<size_t>(lanes) * k);
 }
 struct Int8Rows {
     int8_t *values;
     float *scales;
-    Int8Rows(void *scratch, int lanes, int k)
-        : values(static_cast<int8_t *>(scratch)), scales(reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + row_bytes(lanes, k))) {}
+    int *partials;
+    size_t bytes;
+    Int8Rows(void *scratch, int lanes, int k) {
+        uint8_t *const base = static_cast<uint8_t *>(scratch);
+        values = reinterpret_cast<int8_t *>(base);
+        scales = reinterpret_cast<float *>(base + row_bytes(lanes, k));
+        bytes = row_bytes(lanes, k) + padded(static_cast<size_t>(lanes) * sizeof(float));
+        partials = reinterpret_cast<int *>(base + bytes);
+        if (lanes > STREAM_LANES) bytes += partial_bytes(SPLIT_TILES, std::min(MAX_LANES, (lanes + 31) / 32 * 32), 2);
+    }
+    // sums of split tiles, and how many items of a tile have arrived in each CTA's place
+    static size_t partial_bytes(int tiles, int tile_lanes, int matrices) {
+        return static_cast<size_t>(tiles) * 2 * matrices * tile_lanes * ROWS * sizeof(int) + padded(static_cast<size_t>(tiles) * 2 * sizeof(int));
+    }
 };
 
 // gate alone (up == nullptr) or the pair.
@@ -1438,18 +1511,26 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
     } else {
         plan_dense(args, TWO);
     }
-    const cudaError_t status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream);
+    const int tiles = args.row_tiles * args.lane_tiles;
+    size_t zeroed = 0;
+    if (args.splits > 1) {
+        zeroed = Int8Rows::partial_bytes(tiles, args.tile_lanes, TWO ? 2 : 1);
+        args.partials = rows.partials;
+        args.arrived = rows.partials + static_cast<size_t>(tiles) * 2 * (TWO ? 2 : 1) * args.tile_lanes * ROWS;
+    }
+    const cudaError_t status =
+        launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream, 0, rows.partials, zeroed);
     if (status != cudaSuccess) return status;
     if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.tile_lanes / 2))
         return cudaErrorInvalidValue;
     args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
     args.wide = !to_f32 && n % 8 == 0 && (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) % 16 == 0;
-    return launch_gemm<MODE>(args, args.row_tiles * args.lane_tiles, stream);
+    return args.splits > 1 ? launch_gemm<MODE, true>(args, tiles * args.splits, stream) : launch_gemm<MODE, false>(args, tiles, stream);
 }
 
 }  // namespace
 
-size_t linear_int8_scratch_bytes(int lanes, int k) { return row_bytes(lanes, k) + static_cast<size_t>(lanes) * sizeof(float); }
+size_t linear_int8_scratch_bytes(int lanes, int k) { return Int8Rows(nullptr, lanes, k).bytes; }
 
 cudaError_t launch_linear_int8(const uint16_t *x, const int8_t *w, const float *scales, void *y, const uint16_t *residual, void *scratch, int lanes, int n, int k, int to_f32,
                                int *error_flag, cudaStream_t stream) {
@@ -1585,11 +1666,11 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     if (status != cudaSuccess) return status;
     status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, part.pair_of, nullptr, tokens, top_k, hidden, stream);
     if (status != cudaSuccess) return status;
-    status = launch_gemm<EXPERTS_PAIR>(first, most_tiles * first.row_tiles, stream);
+    status = launch_gemm<EXPERTS_PAIR, false>(first, most_tiles * first.row_tiles, stream);
     if (status != cudaSuccess) return status;
     status = launch_quantise_rows<float, HeldF32, 2>(part.h, part.hq, part.h_scales, nullptr, part.counts + 1, part.pair_of, weights, pairs, 1, inter, stream);
     if (status != cudaSuccess) return status;
-    status = launch_gemm<EXPERTS_DOWN>(second, most_tiles * second.row_tiles, stream);
+    status = launch_gemm<EXPERTS_DOWN, false>(second, most_tiles * second.row_tiles, stream);
     return status != cudaSuccess ? status : sum();
 }
 

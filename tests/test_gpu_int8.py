@@ -45,6 +45,24 @@ def test_pair(lanes, n, k):
     ref.assert_close(y, want, want.abs() * relative)
 
 
+@pytest.mark.parametrize("lanes,n,k", [(129, 24, 9008), (143, 405, 18704), (200, 9, 20000), (300, 64, 131072), (600, 130, 16384), (1030, 1000, 20016)])
+def test_few_tiles_of_many_columns(lanes, n, k):
+    """Sums that several blocks add up: those of a lane alone, in whatever order they come, call after call in one buffer."""
+    g = ref.generator(lanes + n)
+    x, (w, scale), (up, up_scale) = ref.activations(g, lanes, k), ref.weights(g, n, k), ref.weights(g, n, k)
+    residual = ref.activations(g, lanes, n)
+    buffer, intact = ref.scratch(nb.library().nerve_b200_op_linear_int8_scratch_bytes(lanes, k))
+    y, z, plus = ref.linear(x, w, scale, to_f32=True, buffer=buffer), ref.pair(x, w, scale, up, up_scale, buffer=buffer), ref.linear(x, w, scale, residual, buffer=buffer)
+    again = [ref.linear(x, w, scale, to_f32=True, buffer=buffer) for _ in range(20)]
+    assert intact() and all(torch.equal(y, other) for other in again)
+    assert torch.equal(plus, (y + residual.float()).to(torch.bfloat16))
+    want = ref.product(x, w, scale)
+    ref.assert_close(y, want, want.abs() * ref.PRODUCT)
+    for lane in (0, 127, 128, lanes - 1):
+        assert torch.equal(ref.linear(x[lane : lane + 1], w, scale, to_f32=True)[0], y[lane])
+        assert torch.equal(ref.pair(x[lane : lane + 1], w, scale, up, up_scale)[0], z[lane])
+
+
 def test_the_widest_sums_are_exact():
     k = 131072
     x = torch.ones((2, k), device="cuda", dtype=torch.bfloat16)
