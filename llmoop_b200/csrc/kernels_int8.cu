@@ -5,17 +5,19 @@
 // tiles nor the company of a lane shows in its outputs, and the only roundings are those of q, of the scales' products
 // and of the output.
 //
-// int8_gemm_kernel, persistent: a CTA walks output tiles of up to 128 weight rows (MMA M) by up to 256 lanes (MMA N).  One
-// warp copies both operands with TMA (128-byte-swizzled rows of 128 columns) into a ring as deep as shared memory allows,
-// straight on into the next tile; one warp issues the MMAs into one of two accumulators in tensor memory; eight warps
-// write the finished accumulator out while the other one fills.  A tile may have fewer than 128 weight rows: the rest of
-// the MMA's A operand is then whatever lies behind in shared memory, and the rest of the accumulator is never read.  So a
-// matrix is cut into as many row tiles as the chip has multiprocessors, and few lanes need no split of K.
+// Kernels, and what bounds them (B200; us of one launch, or of the call where it says so):
+//   quantise_rows_kernel  rows to whole numbers; DRAM (2048 x 14336 bf16 to bytes: 14 us, 6.2 TB/s)
+//   int8_gemm_kernel      many lanes, experts of many tokens; the tensor pipe at the clock that the power limit leaves, 1.64 GHz
+//                         (2048 x 4096 x 14336: 87 us, 2.8 POP/s; 8192 x 8192 x 8192: 3.0), or the weights' bytes (160 lanes of
+//                         the 28672 x 8192 pair: 88 us a call, 5.4 TB/s), or the outputs where K is short
+//   int8_stream_kernel    up to 128 lanes; the weights' bytes (4 x 128256 x 4096: 83 us, 6.3 TB/s) or the chain of its steps
+//                         (1 x 4096 x 4096: 4.6 us a call)
+//   expert_groups_kernel, experts_sum_kernel  around the experts' products; the chain of its barriers, DRAM
 //
 // The gate/up pair multiplies the same lanes by a tile of each matrix into sums that lie side by side, so that one thread holds both
 // factors of an output.
 //
-// The experts' products are the same kernel over tiles that expert_groups_kernel makes of the routes.
+// The experts' products are the same kernels over tiles that expert_groups_kernel, or few tokens themselves, make of the routes.
 // Waits are bounded; a wait that expires sets the error word, and the CTA still frees its tensor memory.  The unbounded wait
 // for the kernel in front comes before them in every role, so none of them counts that kernel's time.
 //
@@ -41,8 +43,9 @@ constexpr int OUTPUT_WARPS = 8, THREADS = 128 + 32 * OUTPUT_WARPS;
 constexpr size_t SMEM_LIMIT = 226 * 1024, SMEM_HALF = 112 * 1024;
 constexpr unsigned int SPIN_LIMIT = 1u << 22;  // tries of 1.5 us
 
-constexpr int STREAM_LANES = 128;  // the most of the few-lane kernel
-constexpr int SPLIT_TILES = 32;    // the most tiles whose columns are split
+constexpr int FEW = 8, STREAM_LANES = 128;         // lanes of which a CTA may quantise its own copy; the most of the few-lane kernel
+constexpr int SPLIT_TILES = 32, SPLIT_K = 4096;    // the most tiles, of no fewer columns, whose columns are split
+constexpr bool may_split(int lanes, int k) { return lanes > FEW && k >= SPLIT_K; }
 
 enum Mode { LINEAR, PAIR, EXPERTS_PAIR, EXPERTS_DOWN };
 
@@ -162,6 +165,10 @@ __device__ __forceinline__ uint32_t two_bf16(float low, float high) {
 
 // ---- quantisation of activation rows
 
+// Bytes from one quantised row to the next: a block of 128 columns is then one line of the cache, not two (1030
+// lanes of 4096 x 12400: 61 us, 74 with rows of k bytes).
+__host__ __device__ constexpr int pitch_of(int k) { return (k + BLOCK_K - 1) / BLOCK_K * BLOCK_K; }
+
 // Sixteen values of a row, as they are read.
 struct HeldBf16 {
     uint4 words[2];
@@ -222,7 +229,7 @@ struct HeldF32 {
 // significands are whole numbers below 256) unless it is one; ties are x = amax / 2, whose 63.5 a multiplier too large sends to
 // the even 64 as the true one does, and those of an amax of 254 powers of two, whose multiplier is a power of two and exact.
 // (An approximate reciprocal, a step of Newton's and a look at the remainder: the division rounded up takes a kernel of
-// microseconds 0.4 us.)
+// microseconds 0.4 us.)  An f32 quotient (the experts' intermediate rows) may lie nearer to a tie than that and fall to its other side.
 constexpr float UP = 0x1p+90f;
 __device__ __forceinline__ bool is_tiny(uint32_t amax_bits) { return amax_bits < 0x12800000u; }  // 2^-90
 __device__ __forceinline__ bool is_finite(uint32_t amax_bits) { return amax_bits < 0x7f800000u; }
@@ -255,7 +262,7 @@ __device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
 // wider is read again, from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once
 // to the place of each of its top_k routes, where it has one, and leaves there which route that is (a store of its own for every
 // route, which expert_groups_kernel's one CTA would take 8 us for).  With weights the scale is that of the row times its route's weight.
-// Bound by DRAM for large batches, by the chain of loads, barrier and stores for small ones.
+// Bound by DRAM for large batches (2048 x 14336: 14 us, 6.2 TB/s), by the chain of loads, barrier and stores for small ones (2 us).
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.  width > 0: in the order of int8_stream_kernel's stages, blocks of
 // 128 columns of that many rows, sixteen bytes of a row swizzled as TMA would.  zeroed: what the kernel behind wants to find at zero.
 template <typename T, typename Held, int HELD, bool WARP>
@@ -298,7 +305,7 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
         const uint4 packed = quantise(values, multiplier);
         for (int copy = 0; copy < copies; copy++) {
             const int place = places != nullptr ? own_places[copy] : at_row;
-            const size_t to = width > 0 ? (static_cast<size_t>(at >> 7) * width + place) * BLOCK_K + ((((at >> 4) ^ place) & 7) << 4) : static_cast<size_t>(place) * k + at;
+            const size_t to = width > 0 ? (static_cast<size_t>(at >> 7) * width + place) * BLOCK_K + ((((at >> 4) ^ place) & 7) << 4) : static_cast<size_t>(place) * pitch_of(k) + at;
             if (place >= 0) *reinterpret_cast<uint4 *>(q + to) = packed;
         }
     };
@@ -423,6 +430,20 @@ __device__ __forceinline__ void load_sums(uint32_t address, int (&d)[16]) {
                  : "memory");
 }
 
+// Persistent: a pair of CTAs (cta_group::2) walks output tiles of up to 256 weight rows (MMA M, half of them each CTA's) by up to
+// 256 lanes (MMA N, of which each CTA holds half).  The pair's MMA reads both halves of the lanes, so that a multiprocessor
+// copies and holds half of the activations that tiles of its own would take (37 x 1031 x 2032: 9.1 us a call with CTAs of their
+// own, 7.0 in pairs; 2048 x 4096 x 14336: 127 and 126).
+// Warps: 0 copies both operands with TMA (128-byte-swizzled rows of 128 columns) into a ring as deep as shared memory allows,
+// straight on into the next tile; 1 of the first CTA issues the MMAs into one of two accumulators in tensor memory (one behind
+// the other from its front and its back, as wide as the tile's lanes); 4-11 write the finished accumulator out while the other fills.
+// A tile may have fewer than 256 weight rows: the rest of the MMA's A operand is then whatever lies behind in shared memory, and
+// the rest of the accumulator is never read.  So the rows and lanes of a tile are chosen by the time that the whole matrix takes
+// (plan_dense, plan_experts), not by the MMA's shape.
+// bf16 outputs of even widths leave through shared memory, sixteen bytes a thread (2048 x 4096 x 14336 with a residual: 102 us a call, 105 one by one).
+// SPLIT: the columns of a tile are cut into runs, an item each, for matrices of few tiles and many columns.  Their whole-number sums
+// meet by atomic adds, in any order the same number, in a buffer that the quantisation has put at zero; whichever item comes last
+// writes the outputs (143 x 405 x 18704: 15.5 us, 36.6 in one piece; the pair 20 and 68).
 template <Mode MODE, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -775,11 +796,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
 // products only those of a block with its own block count, the outputs add them up.  The tensor pipe takes some 70 cycles for
 // an instruction of 128 rows whatever N up to 128, so that a tile of 28 rows costs a fourth of what one block after the
 // other would.
+// From nine lanes on int8_gemm_kernel takes the same matrices; the lower of the two plans' estimates decides (32 x 4096 x 8192: 10.6
+// us here, 13.5 there; 100 x 1024 x 1040: 8.4 and 6.1; 100 x 64 x 14336: 20.8 and, with its columns split, 9.8; over 440 shapes of 12 to
+// 128 lanes the choice costs 0.7 % of the better one's time on average).
 // Activations, as blocks of 128 columns of `width` swizzled rows:
 //   Up to eight lanes of few columns every CTA quantises itself while its first weights are on their way, and keeps them: one launch.
 //   More are quantised by a kernel in front, which leaves them in this order (PREPARED), and come with every stage.
 // Warps: 0 copies, 1 issues MMAs, 4-7 (PREPARED: 4-11) write outputs, 4-11 (the experts' down product: 8-11) quantise.
-constexpr int FEW = 8, STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
+constexpr int STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
 constexpr uint32_t ATOM = 1024, STREAM_STAGE = ROWS * BLOCK_K;
 constexpr int FEW_ROUTES = 128;          // of the experts' form
 constexpr int STREAM_SMALL_SHARE = 48;   // stages
@@ -1227,7 +1251,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
 
 // ---- experts: routes grouped by expert
 
-// One CTA counts the routes of every expert, gives each a place behind those of the experts before it, and cuts every
+// Bound by the chain of its loads, shared-memory atomics and barriers: 16384 routes of 128 experts take 8 us, 1000 take 4.
+// One CTA (several would have to wait for one another's counts) counts the routes of every expert, gives each a place behind those of the experts before it, and cuts every
 // expert's places into tiles of tile_lanes.  Which of an expert's routes comes first is left to chance: a row's result does
 // not depend on its place.  Routes to no expert (ids outside 0..experts-1) get place -1.  A thread holds GROUP_HELD routes and
 // their ranks among their expert's.
@@ -1288,7 +1313,10 @@ __global__ void __launch_bounds__(GROUP_THREADS) expert_groups_kernel(const int 
     }
 }
 
-// y[token] = the sum of its routes' weighted rows, in their order (+ residual), rounded once.  Four columns to a thread.
+// y[token] = the sum of its routes' weighted rows, in their order (+ residual), rounded once.  Four columns to a thread, eight rows
+// in flight.  Bound by DRAM: 2048 tokens of eight f32 rows of 2048, 28 us, 5.4 TB/s.  (The rows stay f32: rounding them to bf16 would
+// halve this and add eight roundings to every output.  Columns in two to eight chunks, so that their rows would stay in L2, made
+// the experts of 2048 tokens 210 to 247 us instead of 206: shorter products fill the chip worse than the cache saves.)
 __global__ void experts_sum_kernel(const float *parts, const int *ids, const uint16_t *residual, uint16_t *y, int top_k, int experts, int hidden,
                                    int wide) {
     grid_launch_dependents();
@@ -1332,8 +1360,8 @@ EncodeTiled encode_tiled() {  // the driver's entry point, found through the run
     }();
     return found;
 }
-bool encode(CUtensorMap *map, const int8_t *matrix, int64_t rows, int k, int box_rows) {
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(k)};
+bool encode(CUtensorMap *map, const int8_t *matrix, int64_t rows, int k, int pitch, int box_rows) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(pitch)};
     const cuuint32_t box[2] = {BLOCK_K, static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
     const EncodeTiled function = encode_tiled();
     return function != nullptr && function(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(matrix), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1362,9 +1390,13 @@ cudaError_t launch_gemm(Int8Args &args, int most_items, cudaStream_t stream) {
 int64_t output_cycles(int lanes, bool pair) { return lanes * (pair ? 34 : 18); }
 // Tiles of a matrix of n output channels (`pair`: two weight rows each) for that many lanes, by an estimate of the cycles
 // they take, which it returns: of a block of 128 columns the tensor pipe needs half the lanes' number for each of four instructions a matrix
-// (the waits around them 330 at least), the copies arrive at some 56 bytes per cycle and multiprocessor, and the weights,
-// which the first of a row's tiles brings in, at some 23; the outputs hide behind the next tile's sums, but for the last one's
-// and all of a pair's whose two accumulators do not fit tensor memory.
+// (the waits around them 330 at least), the copies arrive at some 56 bytes per cycle and multiprocessor (weights whose rows are no
+// whole lines at two thirds of that), and the weights, which the first of a row's tiles brings in, at some 23; the outputs hide behind
+// the next tile's sums, but for the last one's and all of a pair's whose two accumulators do not fit tensor memory; the first blocks
+// come 200 cycles each later than the others, up to 3000.
+// Columns are split where that comes out lower: to meet costs the sums 8500 cycles and what the atomic adds take, 400 a cycle, and
+// their outputs hide behind nothing (143 x 1024 of 8192 columns: 14.4 us in one piece, 13.2 split; 256 x 4096 of 8192, where one
+// piece is chosen: 17 and 20; over 480 shapes of 143 to 2048 lanes the choice costs 0.6 % of the better one's time on average).
 int64_t plan_dense(Int8Args &args, bool pair) {
     const int pairs = multiprocessors() / 2, blocks = (args.k + BLOCK_K - 1) / BLOCK_K, matrices = pair ? 2 : 1;
     const int padded = (args.lanes + 31) / 32 * 32, least = (padded + MAX_LANES - 1) / MAX_LANES;
@@ -1373,15 +1405,15 @@ int64_t plan_dense(Int8Args &args, bool pair) {
         const int lanes = ((padded + split - 1) / split + 31) / 32 * 32, lane_tiles = (padded + lanes - 1) / lanes;
         for (int rows = ROWS; rows >= 8; rows -= 8) {  // (in steps of sixteen bytes of outputs)
             const int row_tiles = (args.n + 2 * rows - 1) / (2 * rows), waves = (row_tiles * lane_tiles + pairs - 1) / pairs;
-            const int tensor = matrices * std::max(2 * lanes, 330), copies = (matrices * rows + lanes / 2) * BLOCK_K / 56, memory = matrices * rows * BLOCK_K / (23 * lane_tiles);
-            const int64_t sums = static_cast<int64_t>(blocks) * std::max({tensor, copies, memory}) + 1000, outputs = output_cycles(lanes, pair);
-            int64_t cost = waves * (2 * matrices * lanes <= 512 ? std::max(sums, outputs) : sums + outputs) + outputs;
-            // few tiles of many columns: several items to a tile, whose sums meet at some 400 a cycle
+            const int tensor = matrices * std::max(2 * lanes, 330), copies = (matrices * rows * (args.k % BLOCK_K == 0 ? 2 : 3) + lanes) * BLOCK_K / 112,
+                      memory = matrices * rows * BLOCK_K / (23 * lane_tiles), block = std::max({tensor, copies, memory});
+            const int64_t sums = static_cast<int64_t>(blocks) * block + 1000, outputs = output_cycles(lanes, pair);
+            int64_t cost = waves * (2 * matrices * lanes <= 512 ? std::max(sums, outputs) : sums + outputs) + outputs + std::min(3000, 200 * blocks);
             int splits = 1;
-            if (args.lanes > STREAM_LANES && row_tiles * lane_tiles <= SPLIT_TILES) {
+            if (may_split(args.lanes, args.k) && row_tiles * lane_tiles <= SPLIT_TILES) {
                 const int most = std::min(pairs / (row_tiles * lane_tiles), (blocks + 1) / 2);
                 const int64_t added = static_cast<int64_t>(row_tiles * lane_tiles * most) * 2 * rows * lanes * matrices;
-                const int64_t split_cost = static_cast<int64_t>((blocks + most - 1) / std::max(most, 1)) * std::max({tensor, copies, memory}) + 8500 + 3 * outputs + added / 400;
+                const int64_t split_cost = static_cast<int64_t>((blocks + most - 1) / std::max(most, 1)) * block + 8500 + 3 * outputs + added / 400;
                 if (most > 1 && split_cost < cost) cost = split_cost, splits = most;
             }
             if (best != 0 && cost >= best) continue;
@@ -1404,7 +1436,8 @@ size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Tiles of `matrices` matrices of n output channels for the few-lane kernel: as few rows for the busiest CTA as possible, a
 // tile counted as the bytes of four rows more.  Returns an estimate of the cycles they take, as plan_dense does: a stage's four
-// instructions take the tensor pipe 290 cycles or twice their N, and the outputs of a tile, lane by lane, are not hidden by much.
+// instructions take the tensor pipe 290 cycles or twice their N, its copies 340 and 70 a box to issue, and the outputs of a tile, lane by
+// lane, are not hidden by much.
 int64_t plan_stream(StreamArgs &args, int matrices, bool pair) {
     const int count = multiprocessors(), most = std::min(pair ? 64 : 128, args.n);
     int64_t best = 0;
@@ -1424,9 +1457,10 @@ int64_t plan_stream(StreamArgs &args, int matrices, bool pair) {
     while (args.groups * args.width > MAX_LANES) args.groups /= 2;
     args.span_log = args.rows <= 32 ? 5 : args.rows <= 64 ? 6 : 7;
     const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, steps = (blocks + args.groups - 1) / args.groups, weight_rows = args.groups * args.rows * (pair ? 2 : 1);
-    const int tensor = std::max(290, 2 * args.groups * args.width), copies = (weight_rows + args.groups * args.width) * BLOCK_K / 56, memory = weight_rows * BLOCK_K / 23;
+    const int tensor = std::max(290, 2 * args.groups * args.width), copies = (weight_rows + args.groups * args.width) * BLOCK_K / 56, memory = weight_rows * BLOCK_K / 23,
+              issue = 340 + 70 * args.groups * (pair ? 2 : 1);
     const int64_t waves = (static_cast<int64_t>(matrices) * args.row_tiles + count - 1) / count;
-    return waves * (static_cast<int64_t>(steps) * std::max({tensor, copies, memory}) + 900 + args.lanes * (20 + (57 << args.span_log) / 128));
+    return waves * (static_cast<int64_t>(steps) * std::max({tensor, copies, memory, issue}) + 900 + args.lanes * (30 + (57 << args.span_log) / 128));
 }
 // Stages in up to `most` bytes of shared memory, or in all of it where three do not fit into those.  False where three do not
 // fit at all.
@@ -1459,10 +1493,10 @@ cudaError_t launch_stream(const StreamArgs &args, int tiles, size_t bytes, cudaS
 
 // Lanes of a block of the few-lane kernel's activations.
 int stream_width(int lanes) { return lanes <= FEW ? FEW : (lanes + 15) / 16 * 16; }
-// The scratch buffer of a linear: the activations' whole numbers, as rows or as blocks of 128 columns, one scale per lane, and for many
-// lanes the sums of tiles whose columns are split.
+// The scratch buffer of a linear: the activations' whole numbers, as rows or as blocks of 128 columns, one scale per lane, and the sums
+// of tiles whose columns are split, where they may be.
 size_t row_bytes(int lanes, int k) {
-    return padded(lanes <= STREAM_LANES ? static_cast<size_t>((k + BLOCK_K - 1) / BLOCK_K) * BLOCK_K * stream_width(lanes) : static_cast<size_t>(lanes) * k);
+    return padded(lanes <= STREAM_LANES ? static_cast<size_t>((k + BLOCK_K - 1) / BLOCK_K) * BLOCK_K * stream_width(lanes) : static_cast<size_t>(lanes) * pitch_of(k));
 }
 struct Int8Rows {
     int8_t *values;
@@ -1475,7 +1509,7 @@ struct Int8Rows {
         scales = reinterpret_cast<float *>(base + row_bytes(lanes, k));
         bytes = row_bytes(lanes, k) + padded(static_cast<size_t>(lanes) * sizeof(float));
         partials = reinterpret_cast<int *>(base + bytes);
-        if (lanes > STREAM_LANES) bytes += partial_bytes(SPLIT_TILES, std::min(MAX_LANES, (lanes + 31) / 32 * 32), 2);
+        if (may_split(lanes, k)) bytes += partial_bytes(SPLIT_TILES, std::min(MAX_LANES, (lanes + 31) / 32 * 32), 2);
     }
     // sums of split tiles, and how many items of a tile have arrived in each CTA's place
     static size_t partial_bytes(int tiles, int tile_lanes, int matrices) {
@@ -1499,7 +1533,7 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
         few.width = stream_width(lanes);
         size_t bytes;
         if (plan_stream(few, 1, TWO) <= plan_dense(args, TWO) || own) {
-            if (!encode(&few.weights, w, n, k, few.rows) || (TWO && !encode(&few.up, up, n, k, few.rows))) return cudaErrorInvalidValue;
+            if (!encode(&few.weights, w, n, k, k, few.rows) || (TWO && !encode(&few.up, up, n, k, k, few.rows))) return cudaErrorInvalidValue;
             if (own && plan_stages<MODE, false>(few, stream_share(few), &bytes)) return launch_stream<MODE, false>(few, few.row_tiles, bytes, stream);
             const cudaError_t status =
                 launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream, few.width);
@@ -1521,7 +1555,8 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
     const cudaError_t status =
         launch_quantise_rows<uint16_t, HeldBf16, 4>(x, rows.values, rows.scales, nullptr, nullptr, nullptr, nullptr, lanes, 1, k, stream, 0, rows.partials, zeroed);
     if (status != cudaSuccess) return status;
-    if (!encode(&args.weights, w, n, k, args.rows) || (TWO && !encode(&args.up, up, n, k, args.rows)) || !encode(&args.activations, rows.values, lanes, k, args.tile_lanes / 2))
+    if (!encode(&args.weights, w, n, k, k, args.rows) || (TWO && !encode(&args.up, up, n, k, k, args.rows)) ||
+        !encode(&args.activations, rows.values, lanes, k, pitch_of(k), args.tile_lanes / 2))
         return cudaErrorInvalidValue;
     args.scales = scales, args.up_scales = up_scales, args.lane_scales = rows.scales, args.y = y, args.residual = residual;
     args.wide = !to_f32 && n % 8 == 0 && (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) % 16 == 0;
@@ -1568,9 +1603,9 @@ struct ExpertsScratch {
         pair_of = reinterpret_cast<int *>(take(pairs * sizeof(int)));
         x_scales = reinterpret_cast<float *>(take(pairs * sizeof(float)));
         h_scales = reinterpret_cast<float *>(take(pairs * sizeof(float)));
-        hq = reinterpret_cast<int8_t *>(take(pairs * inter));
+        hq = reinterpret_cast<int8_t *>(take(pairs * pitch_of(inter)));
         const size_t shared = used;
-        xq = reinterpret_cast<int8_t *>(take(pairs * hidden));
+        xq = reinterpret_cast<int8_t *>(take(pairs * pitch_of(hidden)));
         h = reinterpret_cast<float *>(take(pairs * inter * sizeof(float)));
         const size_t product_end = used;
         if (tokens > FEW) used = shared;
@@ -1634,8 +1669,8 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
         }
         size_t first_bytes, second_bytes;
         if (plan_stages<EXPERTS_PAIR, false>(first, SMEM_LIMIT, &first_bytes) && plan_stages<EXPERTS_DOWN, false>(second, SMEM_HALF, &second_bytes)) {
-            if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) ||
-                !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows))
+            if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, hidden, first.rows) ||
+                !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, inter, second.rows))
                 return cudaErrorInvalidValue;
             cudaError_t status = launch_stream<EXPERTS_PAIR, false>(first, std::min(experts, pairs) * first.row_tiles, first_bytes, stream);
             if (status != cudaSuccess) return status;
@@ -1648,8 +1683,10 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     second.n = hidden, second.k = inter;
     plan_experts(first, pairs, experts, true);
     plan_experts(second, pairs, experts, false);
-    if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, first.rows) || !encode(&first.activations, part.xq, pairs, hidden, first.tile_lanes / 2) ||
-        !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, second.rows) || !encode(&second.activations, part.hq, pairs, inter, second.tile_lanes / 2))
+    if (!encode(&first.weights, gate_up, static_cast<int64_t>(experts) * 2 * inter, hidden, hidden, first.rows) ||
+        !encode(&first.activations, part.xq, pairs, hidden, pitch_of(hidden), first.tile_lanes / 2) ||
+        !encode(&second.weights, down, static_cast<int64_t>(experts) * hidden, inter, inter, second.rows) ||
+        !encode(&second.activations, part.hq, pairs, inter, pitch_of(inter), second.tile_lanes / 2))
         return cudaErrorInvalidValue;
     first.scales = gate_up_scales, second.scales = down_scales;
     first.lane_scales = part.x_scales, second.lane_scales = part.h_scales;
