@@ -1532,7 +1532,8 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
         few.lanes = lanes, few.n = n, few.k = k, few.to_f32 = to_f32, few.error_flag = error_flag;
         few.width = stream_width(lanes);
         size_t bytes;
-        if (plan_stream(few, 1, TWO) <= plan_dense(args, TWO) || own) {
+        const int64_t cost = plan_stream(few, 1, TWO);
+        if (own || cost <= plan_dense(args, TWO)) {
             if (!encode(&few.weights, w, n, k, k, few.rows) || (TWO && !encode(&few.up, up, n, k, k, few.rows))) return cudaErrorInvalidValue;
             if (own && plan_stages<MODE, false>(few, stream_share(few), &bytes)) return launch_stream<MODE, false>(few, few.row_tiles, bytes, stream);
             const cudaError_t status =

@@ -11,7 +11,9 @@
 // experts in 8 groups: 81 us), so that 32 bits, with a bound on the error, find the few candidates, which alone are scored and ranked
 // in 64; tokens that cannot be decided so (groups closer than the error, infinities) are done by the definition.
 //
-// One warp per token.  (No pointer is __restrict__: loads through those may move in front of the wait
+// One warp per token, of which the chip holds enough to cover the loads.  Bound by the instructions that it issues, some 1050 a token:
+// 16384 tokens of 256 experts, 26 us, of which the logits' bytes are 2.8.  One token of 128 experts takes 2.8 us, a launch and the
+// chain of reductions.  (No pointer is __restrict__: loads through those may move in front of the wait
 // for the kernel that writes the logits.)
 #include <algorithm>
 
