@@ -6,9 +6,10 @@
 // and of the output.
 //
 // Kernels, and what bounds them (B200; us of one launch, or of the call where it says so):
-//   quantise_rows_kernel  rows to whole numbers; DRAM (2048 x 14336 bf16 to bytes: 14 us, 6.2 TB/s)
+//   quantise_rows_kernel  rows to whole numbers; DRAM and the issue of 134 warp instructions for sixteen values a thread (2048 x 14336 bf16
+//                         from DRAM: 16 us, 5.4 TB/s)
 //   int8_gemm_kernel      many lanes, experts of many tokens; the tensor pipe at the clock that the power limit leaves, 1.64 GHz
-//                         (2048 x 4096 x 14336: 87 us, 2.8 POP/s; 8192 x 8192 x 8192: 3.0), or the weights' bytes (160 lanes of
+//                         (2048 x 4096 x 14336: 85 us, 2.8 POP/s; 8192 x 8192 x 8192: 3.0), or the weights' bytes (160 lanes of
 //                         the 28672 x 8192 pair: 88 us a call, 5.4 TB/s), or the outputs where K is short
 //   int8_stream_kernel    up to 128 lanes; the weights' bytes (4 x 128256 x 4096: 83 us, 6.3 TB/s) or the chain of its steps
 //                         (1 x 4096 x 4096: 4.6 us a call)
@@ -262,7 +263,7 @@ __device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
 // wider is read again, from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once
 // to the place of each of its top_k routes, where it has one, and leaves there which route that is (a store of its own for every
 // route, which expert_groups_kernel's one CTA would take 8 us for).  With weights the scale is that of the row times its route's weight.
-// Bound by DRAM for large batches (2048 x 14336: 14 us, 6.2 TB/s), by the chain of loads, barrier and stores for small ones (2 us).
+// Bound by DRAM and its instructions for large batches (2048 x 14336: 16 us, 5.4 TB/s), by the chain of loads, barrier and stores for small ones (2 us).
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.  width > 0: in the order of int8_stream_kernel's stages, blocks of
 // 128 columns of that many rows, sixteen bytes of a row swizzled as TMA would.  zeroed: what the kernel behind wants to find at zero.
 template <typename T, typename Held, int HELD, bool WARP>
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
     if (!WARP) {
         if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = amax;
         __syncthreads();
-        for (int warp = 0; warp < static_cast<int>(blockDim.x >> 5); warp++) amax = max(amax, warps[warp]);
+        amax = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? warps[threadIdx.x & 31] : 0u);
     }
     const float multiplier = row_multiplier(amax);
     const int copies = places != nullptr ? top_k : 1;
@@ -327,7 +328,8 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 
 // Rows of up to 1024 columns of which there are more than the chip has warps to wait with are a warp's each (16384 rows of 768
 // f32 values: 20 us with a CTA each, 12 with a warp).  Otherwise as many threads as sixteen columns each ask for up to 256, then
-// more columns each.
+// more columns each; twice as many columns each where rows fill the chip, whose time is then the instructions around a thread's first
+// load (2048 x 4096 x 14336: 97.9 us a call, 100.1 with half as many; 300 x 14336, where threads are few: 12.7 and 11.5).
 template <typename T, typename Held, int MOST>
 cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
                                  int k, cudaStream_t stream, int width = 0, void *zeroed = nullptr, size_t zeroed_bytes = 0) {
@@ -338,8 +340,9 @@ cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int
                                 weights, rows, top_k, k, wide, width, static_cast<uint4 *>(zeroed), static_cast<int>(zeroed_bytes / sizeof(uint4)));
     };
     if (parts <= 64 && rows >= 1024) return with(quantise_rows_kernel<T, Held, 2, true>, 2, 8);
-    if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1, false>, 1, 0);
-    if (parts <= 1024 || MOST == 2) return with(quantise_rows_kernel<T, Held, 2, false>, 2, 0);
+    const bool many = rows >= 512;
+    if (parts <= 256 && (!many || parts <= 64)) return with(quantise_rows_kernel<T, Held, 1, false>, 1, 0);
+    if (parts <= (many ? 256 : 1024) || MOST == 2) return with(quantise_rows_kernel<T, Held, 2, false>, 2, 0);
     return with(quantise_rows_kernel<T, Held, MOST, false>, MOST, 0);
 }
 
