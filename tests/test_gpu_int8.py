@@ -64,6 +64,34 @@ def test_few_tiles_of_many_columns(lanes, n, k):
         assert torch.equal(ref.pair(x[lane : lane + 1], w, scale, up, up_scale)[0], z[lane])
 
 
+@pytest.mark.parametrize("lanes", [20, 200])
+def test_few_tiles_of_many_columns_in_a_graph(lanes):
+    """Replays on new rows, one of them of zeros and one with a NaN, in a buffer that holds anything before the first call."""
+    n, k = 70, 12304
+    g = ref.generator(lanes)
+    w, scale = ref.weights(g, n, k)
+    x, y = ref.activations(g, lanes, k), torch.empty((lanes, n), dtype=torch.bfloat16, device="cuda")
+    size = nb.library().nerve_b200_op_linear_int8_scratch_bytes(lanes, k)
+    buffer = torch.randint(0, 256, (size,), dtype=torch.uint8, device="cuda")
+    ref.linear(x, w, scale, x[:, :n].contiguous(), y=y, buffer=buffer)
+    torch.cuda.synchronize()
+    residual = ref.activations(g, lanes, n)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ref.linear(x, w, scale, residual, y=y, buffer=buffer)
+        ref.linear(x, w, scale, y, y=y, buffer=buffer)  # onto its own outputs
+    for round in range(3):
+        x.copy_(ref.activations(g, lanes, k))
+        x[round] = 0
+        x[lanes - 1 - round, 5] = math.nan
+        graph.replay()
+        first = ref.linear(x, w, scale, residual)
+        want = ref.linear(x, w, scale, first)
+        assert torch.equal(y.nan_to_num(7e4), want.nan_to_num(7e4))
+        assert bool(y[lanes - 1 - round].isnan().all()) and torch.equal(y[round], residual[round])
+        torch.cuda.synchronize()
+
+
 def test_the_widest_sums_are_exact():
     k = 131072
     x = torch.ones((2, k), device="cuda", dtype=torch.bfloat16)
