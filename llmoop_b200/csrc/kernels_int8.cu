@@ -259,6 +259,86 @@ __device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
+// ---- the experts' routes: places in the order of the experts, tiles of them
+
+// Routes by number, ids [pairs], and what is made of them: tiles {expert, first place, places}, counts {tiles, places}.
+struct Grouping {
+    const int *ids;
+    int pairs, experts, tile_lanes;
+    int4 *tiles;
+    int *counts;
+    __device__ __forceinline__ bool routed(int id) const { return static_cast<uint32_t>(id) < static_cast<uint32_t>(experts); }
+};
+// The most routes that every CTA of the rows' quantisation looks through, with that many threads at least: a launch less than with
+// expert_groups_kernel in front (14 tokens of 6 of 29 experts 14.4 us and 16.6, 24 of 8 of 128 experts 71.8 and 73.4, 250 of 2 of 8
+// 20.1 and 22.1, but 64 of 8 of 128 94.3 and 92.0; 120 of 8 of 16 with twice as many allowed 23.1 and 20.8).
+constexpr int FEW_GROUPED = 512, GROUPING_THREADS = 128;
+
+// The routes of the table, some a thread; those to no expert behind all others.
+constexpr int ROUTES_HELD = FEW_GROUPED / GROUPING_THREADS;
+__device__ __forceinline__ void load_routes(const Grouping &g, int (&ids)[ROUTES_HELD]) {
+#pragma unroll
+    for (int i = 0; i < ROUTES_HELD; i++) {
+        const int pair = threadIdx.x + i * blockDim.x;
+        ids[i] = pair < g.pairs ? g.ids[pair] : -1;
+        if (!g.routed(ids[i])) ids[i] = g.experts;
+    }
+}
+
+// By a CTA: counts of every expert, then GROUPING_THREADS threads, of which each has a run of experts.
+__device__ __forceinline__ void make_tiles(const Grouping &g) {
+    __shared__ int count[EXPERTS_INT8_MAX + 1], warp_places[GROUPING_THREADS / 32], warp_tiles[GROUPING_THREADS / 32];
+    int ids[ROUTES_HELD];
+    load_routes(g, ids);
+    const int thread = threadIdx.x;
+    for (int expert = thread; expert < g.experts; expert += blockDim.x) count[expert] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROUTES_HELD; i++) atomicAdd(&count[ids[i]], 1);
+    __syncthreads();
+    const int run = (g.experts + GROUPING_THREADS - 1) / GROUPING_THREADS, first = min(thread * run, g.experts), last = thread < GROUPING_THREADS ? min(first + run, g.experts) : first;
+    int places = 0, tiles = 0;
+    for (int expert = first; expert < last; expert++) places += count[expert], tiles += (count[expert] + g.tile_lanes - 1) / g.tile_lanes;
+    const int own_places = places, own_tiles = tiles;
+    for (int offset = 1; offset < 32; offset *= 2) {
+        const int other_places = __shfl_up_sync(0xffffffffu, places, offset), other_tiles = __shfl_up_sync(0xffffffffu, tiles, offset);
+        if ((thread & 31) >= offset) places += other_places, tiles += other_tiles;
+    }
+    if (thread < GROUPING_THREADS && (thread & 31) == 31) warp_places[thread >> 5] = places, warp_tiles[thread >> 5] = tiles;
+    __syncthreads();
+    if (thread >= GROUPING_THREADS) return;
+    for (int warp = 0; warp < thread >> 5; warp++) places += warp_places[warp], tiles += warp_tiles[warp];
+    if (thread == GROUPING_THREADS - 1) g.counts[0] = tiles, g.counts[1] = places;
+    places -= own_places, tiles -= own_tiles;
+    for (int expert = first; expert < last; expert++)
+        for (int left = count[expert]; left > 0; left -= g.tile_lanes) {
+            const int lanes = min(left, g.tile_lanes);
+            g.tiles[tiles++] = make_int4(expert, places, lanes, 0);
+            places += lanes;
+        }
+}
+
+// By a CTA: the places of routes first ... first + count - 1, -1 for those to no expert; there behind the CTA's next barrier.
+__device__ __forceinline__ void find_places(const Grouping &g, int first, int count, int *places) {
+    int ids[ROUTES_HELD];
+    load_routes(g, ids);
+    __shared__ int own[ROUTING_MAX_TOP_K];
+    for (int j = threadIdx.x; j < count; j += blockDim.x) {
+        own[j] = g.ids[first + j];
+        places[j] = g.routed(own[j]) ? 0 : -1;
+    }
+    __syncthreads();
+    for (int j = 0; j < count; j++) {
+        const int id = own[j];
+        if (!g.routed(id)) continue;
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i < ROUTES_HELD; i++) before += ids[i] < id + (static_cast<int>(threadIdx.x + i * blockDim.x) < first + j ? 1 : 0);
+        before = __reduce_add_sync(0xffffffffu, before);
+        if ((threadIdx.x & 31) == 0 && before != 0) atomicAdd(&places[j], before);
+    }
+}
+
 // A row of x is one CTA's, or one warp's (WARP), whose threads hold it in registers, HELD times sixteen values each; what is
 // wider is read again, from the caches.  Without places the row goes to its own number; with them (the experts' inputs) once
 // to the place of each of its top_k routes, where it has one, and leaves there which route that is (a store of its own for every
@@ -266,15 +346,21 @@ __device__ __forceinline__ uint4 quantise(const Held &held, float multiplier) {
 // Bound by DRAM and its instructions for large batches (2048 x 14336: 16 us, 5.4 TB/s), by the chain of loads, barrier and stores for small ones (2 us).
 // wide: x rows start on 16-byte boundaries.  k is a multiple of 16.  width > 0: in the order of int8_stream_kernel's stages, blocks of
 // 128 columns of that many rows, sixteen bytes of a row swizzled as TMA would.  zeroed: what the kernel behind wants to find at zero.
-template <typename T, typename Held, int HELD, bool WARP>
+// GROUPS: places are not there yet.  Every CTA finds those of its own row's routes, as many as routes lie in front of them in the order
+// of experts, then of numbers; the first CTA has no row and cuts the experts' places into tiles.
+template <typename T, typename Held, int HELD, bool WARP, bool GROUPS>
 __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *q, float *scales, const int *places,
                                                             const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
-                                                            int k, int wide, int width, uint4 *zeroed, int zeroed_count) {
+                                                            int k, int wide, int width, uint4 *zeroed, int zeroed_count, Grouping groups) {
     __shared__ uint32_t warps[16];
     grid_launch_dependents();
     grid_dependency_wait();
+    if (GROUPS && blockIdx.x == 0) {
+        make_tiles(groups);
+        return;
+    }
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < zeroed_count; i += gridDim.x * blockDim.x) zeroed[i] = make_uint4(0, 0, 0, 0);
-    const int at_row = WARP ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
+    const int at_row = WARP ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x) - (GROUPS ? 1 : 0);
     if (row_count != nullptr) rows = *row_count;
     if (at_row >= rows) return;
     const T *row = x + static_cast<size_t>(at_row) * k;
@@ -283,6 +369,8 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 #pragma unroll
     for (int i = 0; i < HELD; i++)
         if (first + i * step < k) held[i].load(row, first + i * step, wide);
+    __shared__ int found[GROUPS ? ROUTING_MAX_TOP_K : 1];
+    if constexpr (GROUPS) find_places(groups, at_row * top_k, top_k, found);
     uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < HELD; i++)
@@ -299,13 +387,14 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
         amax = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? warps[threadIdx.x & 31] : 0u);
     }
     const float multiplier = row_multiplier(amax);
-    const int copies = places != nullptr ? top_k : 1;
-    const int *own_places = places + (places != nullptr ? static_cast<size_t>(at_row) * top_k : 0);
+    const bool placed = GROUPS || places != nullptr;
+    const int copies = placed ? top_k : 1;
+    const int *const own_places = GROUPS ? found : places + (places != nullptr ? static_cast<size_t>(at_row) * top_k : 0);
     auto store = [&](int at, Held &values) {
         if (is_tiny(amax)) values.scale_up();
         const uint4 packed = quantise(values, multiplier);
         for (int copy = 0; copy < copies; copy++) {
-            const int place = places != nullptr ? own_places[copy] : at_row;
+            const int place = placed ? own_places[copy] : at_row;
             const size_t to = width > 0 ? (static_cast<size_t>(at >> 7) * width + place) * BLOCK_K + ((((at >> 4) ^ place) & 7) << 4) : static_cast<size_t>(place) * pitch_of(k) + at;
             if (place >= 0) *reinterpret_cast<uint4 *>(q + to) = packed;
         }
@@ -319,10 +408,10 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
         store(at, more);
     }
     for (int copy = first / 16; copy < copies; copy += step / 16) {
-        const int place = places != nullptr ? own_places[copy] : at_row;
+        const int place = placed ? own_places[copy] : at_row;
         if (place < 0) continue;
         scales[place] = weights != nullptr ? __fmul_rn(row_scale(amax), weights[pair_of[place]]) : row_scale(amax);
-        if (places != nullptr) pair_of[place] = at_row * top_k + copy;
+        if (placed) pair_of[place] = at_row * top_k + copy;
     }
 }
 
@@ -332,18 +421,26 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 // load (2048 x 4096 x 14336: 97.9 us a call, 100.1 with half as many; 300 x 14336, where threads are few: 12.7 and 11.5).
 template <typename T, typename Held, int MOST>
 cudaError_t launch_quantise_rows(const T *x, int8_t *q, float *scales, const int *places, const int *row_count, int *pair_of, const float *weights, int rows, int top_k,
-                                 int k, cudaStream_t stream, int width = 0, void *zeroed = nullptr, size_t zeroed_bytes = 0) {
+                                 int k, cudaStream_t stream, int width = 0, void *zeroed = nullptr, size_t zeroed_bytes = 0, const Grouping &groups = {}) {
     const int parts = k / 16, wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    const bool grouping = groups.ids != nullptr;
     auto with = [&](auto kernel, int held, int warp_rows) {
-        const int threads = warp_rows != 0 ? 32 * warp_rows : std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
-        return launch_dependent(kernel, dim3(warp_rows != 0 ? (rows + warp_rows - 1) / warp_rows : rows), dim3(threads), 0, 1, stream, x, q, scales, places, row_count, pair_of,
-                                weights, rows, top_k, k, wide, width, static_cast<uint4 *>(zeroed), static_cast<int>(zeroed_bytes / sizeof(uint4)));
+        int threads = warp_rows != 0 ? 32 * warp_rows : std::min(512, ((parts + held - 1) / held + 31) / 32 * 32);
+        if (grouping) threads = std::max(threads, GROUPING_THREADS);
+        return launch_dependent(kernel, dim3(warp_rows != 0 ? (rows + warp_rows - 1) / warp_rows : rows + grouping), dim3(threads), 0, 1, stream, x, q, scales, places, row_count,
+                                pair_of, weights, rows, top_k, k, wide, width, static_cast<uint4 *>(zeroed), static_cast<int>(zeroed_bytes / sizeof(uint4)), groups);
     };
-    if (parts <= 64 && rows >= 1024) return with(quantise_rows_kernel<T, Held, 2, true>, 2, 8);
+    if constexpr (MOST == 4)
+        if (grouping) {
+            if (parts <= 256) return with(quantise_rows_kernel<T, Held, 1, false, true>, 1, 0);
+            if (parts <= 1024) return with(quantise_rows_kernel<T, Held, 2, false, true>, 2, 0);
+            return with(quantise_rows_kernel<T, Held, 4, false, true>, 4, 0);
+        }
+    if (parts <= 64 && rows >= 1024) return with(quantise_rows_kernel<T, Held, 2, true, false>, 2, 8);
     const bool many = rows >= 512;
-    if (parts <= 256 && (!many || parts <= 64)) return with(quantise_rows_kernel<T, Held, 1, false>, 1, 0);
-    if (parts <= (many ? 256 : 1024) || MOST == 2) return with(quantise_rows_kernel<T, Held, 2, false>, 2, 0);
-    return with(quantise_rows_kernel<T, Held, MOST, false>, MOST, 0);
+    if (parts <= 256 && (!many || parts <= 64)) return with(quantise_rows_kernel<T, Held, 1, false, false>, 1, 0);
+    if (parts <= (many ? 256 : 1024) || MOST == 2) return with(quantise_rows_kernel<T, Held, 2, false, false>, 2, 0);
+    return with(quantise_rows_kernel<T, Held, MOST, false, false>, MOST, 0);
 }
 
 // ---- the product
@@ -1254,7 +1351,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
 
 // ---- experts: routes grouped by expert
 
-// Bound by the chain of its loads, shared-memory atomics and barriers: 16384 routes of 128 experts take 8 us, 1000 take 4.
+// For tables of more than FEW_GROUPED routes.  Bound by the chain of its loads, shared-memory atomics and barriers: 16384 routes of
+// 128 experts take 8 us, 1000 take 4.
 // One CTA (several would have to wait for one another's counts) counts the routes of every expert, gives each a place behind those of the experts before it, and cuts every
 // expert's places into tiles of tile_lanes.  Which of an expert's routes comes first is left to chance: a row's result does
 // not depend on its place.  Routes to no expert (ids outside 0..experts-1) get place -1.  A thread holds GROUP_HELD routes and
@@ -1702,10 +1800,15 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
         args->error_flag = error_flag;
     }
     const int most_tiles = pairs / first.tile_lanes + std::min(experts, pairs);
-    cudaError_t status = launch_dependent(expert_groups_kernel, dim3(1), dim3(GROUP_THREADS), 0, 1, stream, ids, pairs, experts, first.tile_lanes, part.tiles, part.counts,
-                                          part.place_of);
-    if (status != cudaSuccess) return status;
-    status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, part.pair_of, nullptr, tokens, top_k, hidden, stream);
+    cudaError_t status;
+    if (pairs <= FEW_GROUPED) {
+        status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, nullptr, nullptr, part.pair_of, nullptr, tokens, top_k, hidden, stream, 0, nullptr, 0,
+                                                             Grouping{ids, pairs, experts, first.tile_lanes, part.tiles, part.counts});
+    } else {
+        status = launch_dependent(expert_groups_kernel, dim3(1), dim3(GROUP_THREADS), 0, 1, stream, ids, pairs, experts, first.tile_lanes, part.tiles, part.counts, part.place_of);
+        if (status != cudaSuccess) return status;
+        status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, part.place_of, nullptr, part.pair_of, nullptr, tokens, top_k, hidden, stream);
+    }
     if (status != cudaSuccess) return status;
     status = launch_gemm<EXPERTS_PAIR, false>(first, most_tiles * first.row_tiles, stream);
     if (status != cudaSuccess) return status;

@@ -385,6 +385,7 @@ def _routes(g, tokens, top_k, count):
 @pytest.mark.parametrize("tokens,top_k,count,hidden,inter", [
     (1, 1, 1, 16, 16), (1, 2, 4, 64, 32), (3, 3, 8, 80, 48), (1, 8, 128, 2048, 768), (24, 8, 128, 2048, 768), (37, 2, 5, 1008, 336), (131, 6, 60, 256, 144),
     (8, 16, 128, 4096, 256), (7, 12, 16, 1024, 512), (300, 4, 8, 512, 128), (70, 1, 2, 128, 1040), (513, 2, 3, 272, 80), (65, 5, 1024, 64, 32),
+    (64, 8, 16, 128, 48), (171, 3, 7, 96, 64), (9, 56, 64, 48, 32), (64, 8, 1024, 64, 48), (12, 1, 1, 4112, 80), (9, 40, 1024, 16400, 16),
 ])
 @pytest.mark.parametrize("with_residual", [False, True])
 def test_experts(tokens, top_k, count, hidden, inter, with_residual):
@@ -395,9 +396,10 @@ def test_experts(tokens, top_k, count, hidden, inter, with_residual):
     ref.assert_close(y, *ref.experts_reference(x, ids, weights, *layer, residual))
 
 
-def test_experts_empty_doubled_and_crowded_routes():
+@pytest.mark.parametrize("tokens", [300, 100])  # routes grouped by a launch of their own, or by the rows'
+def test_experts_empty_doubled_and_crowded_routes(tokens):
     g = ref.generator(8)
-    x, layer, (ids, weights) = ref.activations(g, 300, 256), _layer(g, 6, 256, 64), _routes(g, 300, 3, 6)
+    x, layer, (ids, weights) = ref.activations(g, tokens, 256), _layer(g, 6, 256, 64), _routes(g, tokens, 3, 6)
     ids[:40] = 2  # one expert three times
     ids[40:60] = -1  # tokens without a route
     ids[60:70, 1] = 6  # no such expert
@@ -408,7 +410,7 @@ def test_experts_empty_doubled_and_crowded_routes():
     want, error = ref.experts_reference(x, ids, weights, *layer)
     ref.assert_close(y, want, error)
     assert bool((y[40:60] == 0).all())
-    residual = ref.activations(g, 300, 256)
+    residual = ref.activations(g, tokens, 256)
     kept = residual.clone()
     ref.experts(x, ids, weights, *layer, residual, y=residual)  # in place
     ref.assert_close(residual, want + kept.double(), error + (want + kept.double()).abs() * ref.F32)
