@@ -220,7 +220,8 @@ struct Candidates {
 
 // A token whose candidates are found in 32 bits, with a bound on the error, and ranked in 64; false where that is not certain to
 // choose what the definition does.  Without a bias experts are in the order of their logits, which needs no arithmetic; groups of
-// ranks closer than the error are not decided here.  Thread l holds the `per` experts from l * per on, where that makes every group a
+// ranks closer than the error are decided here where a group is a run of threads that holds sigmoids (20 of 16384 tokens of 256 experts
+// in 8 groups; by the definition they took 5 of 27 us, the last of them alone on the chip).  Thread l holds the `per` experts from l * per on, where that makes every group a
 // run of threads and leaves few of them idle; else those 32 apart.
 template <typename T, int PER_THREAD>
 __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *bias, int *ids, float *weights, int token, const Plan &plan, Candidates &found) {
@@ -290,10 +291,21 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
                 next = max(next, min(best, value));
                 best = max(best, value);
             }
-            for (int other = 0; other < threads; other++) {
-                const uint32_t b = __shfl_sync(0xffffffffu, best, first + other), n = __shfl_sync(0xffffffffu, next, first + other);
-                group_next = max(max(group_next, n), min(group_best, b));
-                group_best = max(group_best, b);
+            if ((threads & (threads - 1)) == 0) {
+                group_best = best, group_next = next;
+#pragma unroll
+                for (int offset = 1; offset < 32; offset *= 2) {
+                    if (offset >= threads) break;
+                    const uint32_t b = __shfl_xor_sync(0xffffffffu, group_best, offset), n = __shfl_xor_sync(0xffffffffu, group_next, offset);
+                    group_next = max(max(group_next, n), min(group_best, b));
+                    group_best = max(group_best, b);
+                }
+            } else {
+                for (int other = 0; other < threads; other++) {
+                    const uint32_t b = __shfl_sync(0xffffffffu, best, first + other), n = __shfl_sync(0xffffffffu, next, first + other);
+                    group_next = max(max(group_next, n), min(group_best, b));
+                    group_best = max(group_best, b);
+                }
             }
         } else {
             for (int group = 0; group < routing.groups; group++) {
@@ -314,16 +326,60 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         const bool open = own_group < routing.groups && group_best != 0;
         float rank = open ? value_of(group_best) : -infinity;
         if (routing.group_scores > 1 && open && group_next != 0) rank += value_of(group_next);
+        // the groups in front of this thread's: each of a group's threads compares some
+        const int team = max(threads, 1), team_first = own_group * team;
         int before = 0;
-        for (int group = 0; group < routing.groups; group++) {
-            const float other = __shfl_sync(0xffffffffu, rank, group * max(threads, 1));
-            before += other > rank || (other == rank && group < own_group);
+        for (int from = 0; from < routing.groups; from += team) {
+            const int group = from + lane - team_first;
+            const float other = __shfl_sync(0xffffffffu, rank, min(group, routing.groups - 1) * team);
+            const uint32_t in_front = __ballot_sync(0xffffffffu, group < routing.groups && (other > rank || (other == rank && group < own_group)));
+            before += __popc((in_front >> team_first) & ((1u << team) - 1u));
         }
-        const bool kept = open && before < routing.chosen_groups;
+        bool kept = open && before < routing.chosen_groups;
         const uint32_t first_left = __reduce_max_sync(0xffffffffu, open && !kept ? key_of(rank) : 0u), last_kept = __reduce_min_sync(0xffffffffu, kept ? key_of(rank) : 0xffffffffu);
         if (first_left != 0) {  // (logits as close as 1e-12 may be one score in 64 bits)
             const float in = value_of(last_kept), out = value_of(first_left);
-            if (!(in - out > (scored ? margin(in) : 1e-12f))) return false;
+            if (!(in - out > (scored ? margin(in) : 1e-12f))) {
+                if (!scored || !routing.sigmoid || threads == 0 || !(fmaxf(fabsf(in), fabsf(out)) < 1e30f)) return false;
+                // those in doubt are ranked in 64 bits; a group further than the error above the best that was left, or below the
+                // last that was kept, is not
+                const float error = 2.0f * margin(fmaxf(fabsf(in), fabsf(out)));
+                const bool sure = open && rank > out + error, doubt = open && !sure && rank >= in - error;
+                const int places = routing.chosen_groups - __popc(__ballot_sync(0xffffffffu, sure && lane == team_first));
+                const uint32_t least = routing.group_scores > 1 ? group_next : group_best;  // candidates for the group's largest: what is not further below
+                uint32_t some = 0;
+                if (doubt) {
+                    const uint32_t from = least != 0 ? key_of(value_of(least) - error) : 1u;
+#pragma unroll
+                    for (int j = 0; j < PER_THREAD; j++) some |= value_at(j) >= from ? 1u << j : 0u;
+                }
+                double exact_best = -static_cast<double>(infinity), exact_next = exact_best;
+                while (__any_sync(0xffffffffu, some != 0)) {
+                    if (some == 0) continue;
+                    const int expert = base + __ffs(some) - 1;
+                    some &= some - 1;
+                    double value = 1.0 / (1.0 + exp(-static_cast<double>(logit_of(row, expert))));
+                    if (bias != nullptr) value += static_cast<double>(bias[expert]);
+                    exact_next = fmax(exact_next, fmin(exact_best, value));
+                    exact_best = fmax(exact_best, value);
+                }
+                double best_of_all = -static_cast<double>(infinity), next_of_all = best_of_all;
+                for (int other = 0; other < threads; other++) {
+                    const int from = min(team_first + other, 31);
+                    const double b = __shfl_sync(0xffffffffu, exact_best, from), n = __shfl_sync(0xffffffffu, exact_next, from);
+                    next_of_all = fmax(fmax(next_of_all, n), fmin(best_of_all, b));
+                    best_of_all = fmax(best_of_all, b);
+                }
+                double exact = best_of_all;
+                if (routing.group_scores > 1 && next_of_all > -static_cast<double>(infinity)) exact += next_of_all;
+                const uint32_t doubtful = __ballot_sync(0xffffffffu, doubt);
+                int ahead = 0;
+                for (int group = 0; group < routing.groups; group++) {
+                    const double other = __shfl_sync(0xffffffffu, exact, group * team);
+                    ahead += ((doubtful >> (group * team)) & 1u) && (other > exact || (other == exact && group < own_group));
+                }
+                kept = sure || (doubt && ahead < places);
+            }
         }
         if (threads > 0) {
 #pragma unroll
@@ -347,21 +403,28 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
     }
     if (limit == 0) limit = 1;  // all that are open
     else if (bias != nullptr) limit = key_of(value_of(limit) - margin(value_of(limit)));
-    int count = 0;
-    uint32_t left = 0;  // the largest that is no candidate
+    uint32_t left = 0, own = 0;  // the largest that is no candidate; bit j: one is
 #pragma unroll
     for (int j = 0; j < PER_THREAD; j++) {
         const bool candidate = key[j] >= limit;
         left = max(left, candidate ? 0u : key[j]);
-        const uint32_t all = __ballot_sync(0xffffffffu, candidate);
-        const int place = count + __popc(all & ((1u << lane) - 1u));
-        if (candidate && place < 32) {
-            found.expert[place] = static_cast<uint32_t>(base + j * step);
-            found.logit[place] = logit[j];
-        }
-        count += __popc(all);
+        own |= candidate ? 1u << j : 0u;
+    }
+    int count = 0, place = 0;  // of all, and of the threads before
+    const int own_count = __popc(own);
+#pragma unroll
+    for (int bit = 0; (1 << bit) <= PER_THREAD; bit++) {
+        const uint32_t set = __ballot_sync(0xffffffffu, (own_count >> bit) & 1);
+        count += __popc(set) << bit;
+        place += __popc(set & ((1u << lane) - 1u)) << bit;
     }
     if (count > 31) return false;
+#pragma unroll
+    for (int j = 0; j < PER_THREAD; j++)
+        if ((own >> j) & 1u) {
+            found.expert[place] = static_cast<uint32_t>(base + j * step);
+            found.logit[place++] = logit[j];
+        }
     left = bias == nullptr ? __reduce_max_sync(0xffffffffu, left) : 0u;  // (with a bias the margin keeps it apart)
     __syncwarp();
     // one candidate to a thread: its score in 64 bits, and the number of those in front of it; to the next thread the logit that is left
@@ -388,7 +451,7 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
     const double left_score = __shfl_sync(0xffffffffu, own_score, count);
     if (left != 0 && __any_sync(0xffffffffu, lane < count && own_score <= left_score)) return false;
     __syncwarp();
-    int place = 0;
+    place = 0;
     for (int other = 0; other < count; other++) {
         const double theirs = found.choice[other];
         place += theirs > choice || (theirs == choice && found.expert[other] < my_expert);

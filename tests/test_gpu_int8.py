@@ -362,6 +362,27 @@ def test_route_scores_that_meet_in_64_bits(middle, spread, groups, sigmoid):
     assert bool(((weights.double() - want).abs() <= want.abs() * (ref.F32 + 2.0 ** -40) + 1e-44).all())
 
 
+@pytest.mark.parametrize("apart", [0.0, 1e-9, 1e-7, 2e-6, 2e-5, 2e-4])
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("count,groups,chosen,group_scores", [(256, 8, 4, 2), (64, 8, 3, 1), (96, 3, 1, 2), (120, 5, 2, 2), (24, 12, 5, 2), (488, 4, 2, 2), (1024, 32, 7, 2), (70, 7, 3, 2)])
+def test_route_groups_next_to_one_another(count, groups, chosen, group_scores, sigmoid, apart):
+    """Groups of the same logits in other orders, told apart by the bias; some experts and whole groups closed."""
+    g = ref.generator(count + groups)
+    r, size = nb.Routing(experts=count, top_k=min(6, chosen * (count // groups)), sigmoid=sigmoid, groups=groups, chosen_groups=chosen, group_scores=group_scores, scale=1.5), count // groups
+    one = (torch.randn((48, 1, size), generator=g, device="cuda") * 3).repeat(1, groups, 1)
+    order = torch.rand((48, groups, size), generator=g, device="cuda").argsort(dim=2)
+    logits = one.gather(2, order).view(48, count).contiguous()
+    logits[20:30].masked_fill_(torch.rand((10, count), generator=g, device="cuda") < 0.5, -math.inf)
+    logits[30:36, : 2 * size] = -math.inf
+    logits[36:40] += torch.randn((4, groups, 1), generator=g, device="cuda").repeat(1, 1, size).view(4, count)  # some further away
+    bias = torch.randn(count, generator=g, device="cuda") * apart
+    for some in (bias, bias + 0.25, bias - 3.0, None):
+        ids, weights = ref.route(logits, some, r)
+        want_ids, want = _route_reference(logits, some, r)
+        assert torch.equal(ids, want_ids)
+        assert bool(((weights.double() - want).abs() <= want.abs() * (ref.F32 + 2.0 ** -40) + 1e-44).all())
+
+
 def test_route_leaves_what_lies_behind():
     logits = torch.randn((5, 16), device="cuda")
     ids, weights = torch.full((6, 4), 9, dtype=torch.int32, device="cuda"), torch.full((6, 4), 9.0, device="cuda")
