@@ -220,8 +220,8 @@ struct Candidates {
 
 // A token whose candidates are found in 32 bits, with a bound on the error, and ranked in 64; false where that is not certain to
 // choose what the definition does.  Without a bias experts are in the order of their logits, which needs no arithmetic; groups of
-// ranks closer than the error are decided here where a group is a run of threads that holds sigmoids (20 of 16384 tokens of 256 experts
-// in 8 groups; by the definition they took 5 of 27 us, the last of them alone on the chip).  Thread l holds the `per` experts from l * per on, where that makes every group a
+// ranks closer than the error are decided here where a group is a run of threads (20 of 16384 tokens of 256 experts in 8 groups by
+// sigmoids; by the definition they took 5 of 27 us, the last of them alone on the chip).  Thread l holds the `per` experts from l * per on, where that makes every group a
 // run of threads and leaves few of them idle; else those 32 apart.
 template <typename T, int PER_THREAD>
 __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *bias, int *ids, float *weights, int token, const Plan &plan, Candidates &found) {
@@ -340,7 +340,7 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         if (first_left != 0) {  // (logits as close as 1e-12 may be one score in 64 bits)
             const float in = value_of(last_kept), out = value_of(first_left);
             if (!(in - out > (scored ? margin(in) : 1e-12f))) {
-                if (!scored || !routing.sigmoid || threads == 0 || !(fmaxf(fabsf(in), fabsf(out)) < 1e30f)) return false;
+                if (!scored || threads == 0 || !(fmaxf(fabsf(in), fabsf(out)) < 1e30f)) return false;
                 // those in doubt are ranked in 64 bits; a group further than the error above the best that was left, or below the
                 // last that was kept, is not
                 const float error = 2.0f * margin(fmaxf(fabsf(in), fabsf(out)));
@@ -353,12 +353,23 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
 #pragma unroll
                     for (int j = 0; j < PER_THREAD; j++) some |= value_at(j) >= from ? 1u << j : 0u;
                 }
+                double all = 0.0;  // the softmax's terms
+                if (!routing.sigmoid) {
+#pragma unroll 1
+                    for (int j = 0; j < per; j++) {
+                        const float at = base + j < experts ? logit_of(row, base + j) : -infinity;
+                        if (at > -infinity) all += exp(static_cast<double>(at) - static_cast<double>(top));
+                    }
+#pragma unroll
+                    for (int offset = 16; offset > 0; offset >>= 1) all += __shfl_xor_sync(0xffffffffu, all, offset);
+                }
                 double exact_best = -static_cast<double>(infinity), exact_next = exact_best;
                 while (__any_sync(0xffffffffu, some != 0)) {
                     if (some == 0) continue;
                     const int expert = base + __ffs(some) - 1;
                     some &= some - 1;
-                    double value = 1.0 / (1.0 + exp(-static_cast<double>(logit_of(row, expert))));
+                    const double at = static_cast<double>(logit_of(row, expert)), power = exp(routing.sigmoid ? -at : at - static_cast<double>(top));
+                    double value = (routing.sigmoid ? 1.0 : power) / (routing.sigmoid ? 1.0 + power : all);
                     if (bias != nullptr) value += static_cast<double>(bias[expert]);
                     exact_next = fmax(exact_next, fmin(exact_best, value));
                     exact_best = fmax(exact_best, value);
