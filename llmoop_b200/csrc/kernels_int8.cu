@@ -907,7 +907,9 @@ constexpr int STREAM_THREADS = 384, STREAM_MAX_STAGES = 12;
 constexpr uint32_t ATOM = 1024, STREAM_STAGE = ROWS * BLOCK_K;
 constexpr int FEW_ROUTES = 128;          // of the experts' form
 constexpr int STREAM_SMALL_SHARE = 48;   // stages
-constexpr int STREAM_OWN = 16384;        // values of which every CTA quantises its own copy
+// Values of which every CTA quantises its own copy (8 x 4096 lanes of a 4096 x 4096 matrix: 10.3 us so, 6.6 with a launch in front; 4 x 4096
+// of a 14336 x 4096 pair: 21.3 so, 22.5 with one).
+constexpr int STREAM_OWN = 16384;
 
 struct StreamArgs {
     CUtensorMap weights, up;  // boxes of 128 columns x rows weight rows
