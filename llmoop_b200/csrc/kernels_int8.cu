@@ -10,7 +10,7 @@
 //                         from DRAM: 16 us, 5.4 TB/s)
 //   int8_gemm_kernel      many lanes, experts of many tokens; the tensor pipe at the clock that the power limit leaves, 1.64 GHz
 //                         (2048 x 4096 x 14336: 85 us, 2.8 POP/s; 8192 x 8192 x 8192: 3.0), or the weights' bytes (160 lanes of
-//                         the 28672 x 8192 pair: 88 us a call, 5.4 TB/s), or the outputs where K is short
+//                         the 28672 x 8192 pair: 86 us a call, 5.6 TB/s), or the outputs where K is short
 //   int8_stream_kernel    up to 128 lanes; the weights' bytes (4 x 128256 x 4096: 83 us, 6.3 TB/s) or the chain of its steps
 //                         (1 x 4096 x 4096: 4.6 us a call)
 //   expert_groups_kernel, experts_sum_kernel  around the experts' products; the chain of its barriers, DRAM
