@@ -413,7 +413,7 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
         if (own_best == limit) own_best = 0;
     }
     if (limit == 0) limit = 1;  // all that are open
-    else if (bias != nullptr) limit = key_of(value_of(limit) - margin(value_of(limit)));
+    else if (bias != nullptr && value_of(limit) < infinity) limit = key_of(value_of(limit) - margin(value_of(limit)));  // (infinite biases are equals, without an error)
     uint32_t left = 0, own = 0;  // the largest that is no candidate; bit j: one is
 #pragma unroll
     for (int j = 0; j < PER_THREAD; j++) {
