@@ -9,7 +9,9 @@
 // The definition holds all of it in 64 bits: experts next to one another are told apart as it does, not by what the last bit of an
 // exponential made of them.  64-bit exponentials and keys are also what such a kernel spends its time on (16384 tokens of 256
 // experts in 8 groups: 81 us), so that 32 bits, with a bound on the error, find the few candidates, which alone are scored and ranked
-// in 64; tokens that cannot be decided so (groups closer than the error, infinities) are done by the definition.
+// in 64.  Groups closer than the error are ranked in 64 bits where they stand, if each is a run of threads.  Tokens that cannot be
+// decided so are done by the definition: more than 31 candidates (top_k 32 to 64), sigmoids of logits above 20, logits of +inf, scores
+// below 1e-250, and groups next to one another that are no runs of threads, have no scores or hold choices from 1e30 on.
 //
 // One warp per token, of which the chip holds enough to cover the loads.  Bound by the instructions that it issues, some 1080 a token:
 // 16384 tokens of 256 experts in 8 groups, 21.5 us, of which the logits' bytes are 2.8.  One token of 128 experts takes 2.8 us, a launch and the
@@ -179,8 +181,9 @@ __device__ __forceinline__ float fast_inverse(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(out) : "f"(x));
     return out;
 }
-// How far two choices, or sums of two, have to lie apart to be as far apart in truth.
+// How far two choices about `value`, or sums of two choices each of up to that magnitude, have to lie apart to be in that order in truth.
 __device__ __forceinline__ float margin(float value) { return 1.6e-5f * (1.0f + fabsf(value)); }
+constexpr float LARGEST = 3.402823466e+38f;
 
 // PER_THREAD successive values, in sixteen bytes where they lie so.
 template <int PER_THREAD>
@@ -324,8 +327,14 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
             }
         }
         const bool open = own_group < routing.groups && group_best != 0;
-        float rank = open ? value_of(group_best) : -infinity;
-        if (routing.group_scores > 1 && open && group_next != 0) rank += value_of(group_next);
+        float rank = open ? value_of(group_best) : -infinity, largest = fabsf(rank);
+        if (routing.group_scores > 1 && open && group_next != 0) {
+            rank += value_of(group_next);
+            largest = fmaxf(largest, fabsf(value_of(group_next)));
+        }
+        // Where the rank lies in truth: it is off by its summands' errors, which may be more than all of it where biases of both signs
+        // cancel.  (An infinite one lies anywhere.)
+        const float error = scored ? 0.5f * margin(largest) : 0.0f, low = fminf(rank, LARGEST) - error, high = fmaxf(rank, -LARGEST) + error;
         // the groups in front of this thread's: each of a group's threads compares some
         const int team = max(threads, 1), team_first = own_group * team;
         int before = 0;
@@ -336,20 +345,19 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
             before += __popc((in_front >> team_first) & ((1u << team) - 1u));
         }
         bool kept = open && before < routing.chosen_groups;
-        const uint32_t first_left = __reduce_max_sync(0xffffffffu, open && !kept ? key_of(rank) : 0u), last_kept = __reduce_min_sync(0xffffffffu, kept ? key_of(rank) : 0xffffffffu);
+        const uint32_t first_left = __reduce_max_sync(0xffffffffu, open && !kept ? key_of(high) : 0u), last_kept = __reduce_min_sync(0xffffffffu, kept ? key_of(low) : 0xffffffffu);
         if (first_left != 0) {  // (logits as close as 1e-12 may be one score in 64 bits)
             const float in = value_of(last_kept), out = value_of(first_left);
-            if (!(in - out > (scored ? margin(in) : 1e-12f))) {
-                if (!scored || threads == 0 || !(fmaxf(fabsf(in), fabsf(out)) < 1e30f)) return false;
-                // those in doubt are ranked in 64 bits; a group further than the error above the best that was left, or below the
-                // last that was kept, is not
-                const float error = 2.0f * margin(fmaxf(fabsf(in), fabsf(out)));
-                const bool sure = open && rank > out + error, doubt = open && !sure && rank >= in - error;
+            if (!(scored ? in > out : in - out > 1e-12f)) {
+                if (!scored || threads == 0) return false;
+                // those in doubt are ranked in 64 bits; a group that lies above all that were left, or below all that were kept, is not
+                const bool sure = open && low > out, doubt = open && !sure && high >= in;
+                if (__any_sync(0xffffffffu, doubt && !(largest < 1e30f))) return false;
                 const int places = routing.chosen_groups - __popc(__ballot_sync(0xffffffffu, sure && lane == team_first));
                 const uint32_t least = routing.group_scores > 1 ? group_next : group_best;  // candidates for the group's largest: what is not further below
                 uint32_t some = 0;
                 if (doubt) {
-                    const uint32_t from = least != 0 ? key_of(value_of(least) - error) : 1u;
+                    const uint32_t from = least != 0 ? key_of(value_of(least) - margin(value_of(least))) : 1u;
 #pragma unroll
                     for (int j = 0; j < PER_THREAD; j++) some |= value_at(j) >= from ? 1u << j : 0u;
                 }

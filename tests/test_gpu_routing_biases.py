@@ -40,3 +40,37 @@ def test_infinite_biases(groups, top_k, sigmoid):
         bias[[1, r.experts // 3]] = torch.tensor([-math.inf, math.nan], device="cuda")
         for kind in (torch.float32, torch.bfloat16):
             agrees(logits.to(kind), bias, r)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("large", [3e2, 1e4, 1e6, 1e9, 1e15, 1e32])
+@pytest.mark.parametrize("how", [dict(experts=16, top_k=2, groups=8, chosen_groups=3), dict(experts=64, top_k=4, groups=32, chosen_groups=9), dict(experts=256, top_k=6, groups=8, chosen_groups=4),
+                                 dict(experts=70, top_k=3, groups=7, chosen_groups=2), dict(experts=244, top_k=2, groups=4, chosen_groups=1), dict(experts=1022, top_k=3, groups=2, chosen_groups=1)],
+                         ids=lambda how: f"{how['experts']}g{how['groups']}")
+def test_groups_of_large_biases_of_both_signs(how, large, sigmoid):
+    """A group's two largest choices cancel, and what is left of its rank is smaller than what 32 bits lose of either."""
+    r, size = nb.Routing(**how, sigmoid=sigmoid, group_scores=2), how["experts"] // how["groups"]
+    g = ref.generator(r.experts)
+    logits = torch.randn((64, r.experts), generator=g, device="cuda") * torch.logspace(-5, 0.5, 64, device="cuda")[:, None]
+    for normal in (0, 1, r.groups):  # groups whose biases are small
+        for open_ in (2, size):
+            bias = torch.full((r.groups, size), -large, device="cuda")
+            first = torch.rand((r.groups, size), generator=g, device="cuda").argsort(dim=1)
+            bias.scatter_(1, first[:, :1], large)
+            bias[:normal] = 0.0
+            bias.scatter_(1, first[:, open_:], -math.inf)
+            agrees(logits, bias.flatten(), r)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("lowest", [-1e9, float(torch.finfo(torch.float32).min), float(torch.finfo(torch.bfloat16).min)])
+@pytest.mark.parametrize("group_scores", [1, 2])
+@pytest.mark.parametrize("count,groups,chosen", [(128, 1, 1), (256, 8, 4), (64, 32, 5), (244, 4, 2)])
+def test_biases_of_the_lowest_value(count, groups, chosen, group_scores, lowest, sigmoid):
+    """A mask by finite biases: experts, all but one of a group, whole groups, all groups but one, all."""
+    r, size = nb.Routing(experts=count, top_k=min(6, count // groups * chosen), sigmoid=sigmoid, groups=groups, chosen_groups=chosen, group_scores=group_scores), count // groups
+    g = ref.generator(count)
+    logits = torch.randn((16, count), generator=g, device="cuda") * 2
+    for masked in (torch.rand(count, generator=g, device="cuda") < 0.5, torch.arange(count, device="cuda") % size > 0, torch.arange(count, device="cuda") // size < groups // 2,
+                   torch.arange(count, device="cuda") // size != groups - 1, torch.ones(count, dtype=torch.bool, device="cuda")):
+        agrees(logits, (torch.randn(count, generator=g, device="cuda") * 0.1).masked_fill(masked, lowest), r)
