@@ -896,9 +896,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) int8_gem
 // products only those of a block with its own block count, the outputs add them up.  The tensor pipe takes some 70 cycles for
 // an instruction of 128 rows whatever N up to 128, so that a tile of 28 rows costs a fourth of what one block after the
 // other would.
-// From nine lanes on int8_gemm_kernel takes the same matrices; the lower of the two plans' estimates decides (32 x 4096 x 8192: 10.6
-// us here, 13.5 there; 100 x 1024 x 1040: 8.4 and 6.1; 100 x 64 x 14336: 20.8 and, with its columns split, 9.8; over 440 shapes of 12 to
-// 128 lanes the choice costs 0.7 % of the better one's time on average).
+// int8_gemm_kernel takes the same matrices; where the lanes come quantised, the lower of the two plans' estimates decides (32 x 4096 x
+// 8192: 10.6 us here, 13.5 there; 100 x 1024 x 1040: 8.4 and 6.1; 100 x 64 x 14336: 20.8 and, with its columns split, 9.8; over 440 shapes of
+// 12 to 128 lanes the choice costs 0.7 % of the better one's time on average).  For up to eight lanes that is almost always this one; wide pairs
+// whose rows make a wave and a little here go there (4 lanes of a 9863 x 8304 pair: 43.8 us here, 33.9 there; 3 x 9853 x 36048: 160 and 116), and
+// some linears of close estimates (8 x 19981 x 59648: 219 and 186).
 // Activations, as blocks of 128 columns of `width` swizzled rows:
 //   Up to eight lanes of few columns every CTA quantises itself while its first weights are on their way, and keeps them: one launch.
 //   More are quantised by a kernel in front, which leaves them in this order (PREPARED), and come with every stage.
