@@ -279,14 +279,16 @@ int32_t nerve_b200_op_linear_fp8(const void *x_device, const void *w_device, con
  * No counterpart in the reference (its 8-bit weights are FP8 and Q8_0).  x bf16 [lanes][k] is quantised per lane within the
  * call: a = amax / 127, q = x / a to the nearest whole number, ties to even.  w int8 [n][k] (all 256 values), one f32 scale
  * per output channel.  The products are added up exactly in 32-bit integers, so a lane's outputs do not depend on the other
- * lanes of the call, bit for bit; what is rounded is q, (sum * channel scale) * a in f32, and the output, once.  A lane that
- * holds an infinity or a NaN is NaN throughout; a lane of zeros gives zeros (+ residual).
+ * lanes of the call, bit for bit; what is rounded is q, the sum to f32 (above 2^24), a, (sum * channel scale) * a in f32, and the
+ * output, once.  A lane that holds an infinity or a NaN is NaN throughout; a lane of zeros gives zeros (+ residual).
  * k: a multiple of 16, up to 131072.  w and scratch start on 16-byte boundaries, everything else on its type's.  The calls
  * work on the current device, to which all pointers and the stream belong; they are asynchronous, capturable and allocate
  * nothing but, the first on a device, what the INT4 linears' first call sets up; their waits are bounded as described above.
- * scratch holds ..._scratch_bytes(...) device bytes (0 for sizes that the call refuses): lanes * k and, for nine lanes or
- * more of at least 4096 columns, up to 16.8 MB in which split sums meet.  Its contents need not be kept or cleared between
- * calls; calls that may overlap in time, captured graphs among them, need one each.  0 lanes or tokens: nothing is done.
+ * scratch holds ..._scratch_bytes(...) device bytes (0 for sizes that the call refuses).  For a linear that is a byte a value, with
+ * k rounded up to a multiple of 128 and up to 128 lanes to a multiple of 16 (up to eight lanes: of 8), and four bytes a lane, both
+ * rounded up to 256 bytes; for nine lanes or more of at least 4096 columns up to 16.8 MB more, in which split sums meet.  Its
+ * contents need not be kept or cleared between calls; calls that may overlap in time, captured graphs among them, need one
+ * each.  0 lanes or tokens: nothing is done.
  */
 uint64_t nerve_b200_op_linear_int8_scratch_bytes(int32_t lanes, int32_t k);
 /* y[lane][n] = x . W^T (+ residual bf16 [lanes][n], which may be y itself), bf16, or f32 where to_f32 != 0. */

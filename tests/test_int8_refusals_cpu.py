@@ -87,3 +87,14 @@ def test_scratch_sizes():
     assert library.nerve_b200_op_linear_int8_scratch_bytes(-1, 4096) == 0
     assert library.nerve_b200_op_experts_int8_scratch_bytes(2048, 8, 128, 2048, 768) >= 2048 * 8 * (4 * 2048 + 768)
     assert library.nerve_b200_op_experts_int8_scratch_bytes(2048, 0, 128, 2048, 768) == 0
+
+
+def test_scratch_bytes_are_what_the_header_says():
+    up = lambda value, step: (value + step - 1) // step * step  # noqa: E731
+    library = nb.library()
+    for lanes in (1, 2, 8, 9, 16, 17, 100, 128, 129, 1000, 4096):
+        for k in (16, 112, 128, 400, 4080, 4096, 14336, 131072):
+            rows = up(lanes, 8 if lanes <= 8 else 16) if lanes <= 128 else lanes
+            least = up(rows * up(k, 128), 256) + up(4 * lanes, 256)
+            split = 2 * 32 * 2 * min(256, up(lanes, 32)) * 128 * 4 + 256 if lanes > 8 and k >= 4096 else 0
+            assert library.nerve_b200_op_linear_int8_scratch_bytes(lanes, k) == least + split <= least + 16_800_000, (lanes, k)
