@@ -91,7 +91,6 @@ __global__ void __launch_bounds__(THREADS, 1) linear_bf16_gemm_kernel(const __gr
     const uint32_t full = base + static_cast<uint32_t>(a.stages) * stage_bytes, empty = full + 8 * MAX_STAGES, acc_full = empty + 8 * MAX_STAGES, acc_empty = acc_full + 16,
                    tmem_slot = acc_empty + 16;
     const int blocks = a.k / BLOCK_K;
-    grid_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < MAX_STAGES; s++) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + s * 8) : "memory");
@@ -113,6 +112,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_bf16_gemm_kernel(const __gr
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // not before the tensor memory is this CTA's: one of the next kernel's that took it first would wait for this one
+    grid_launch_dependents();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
     tmem = __reduce_or_sync(0xffffffffu, tmem);  // a uniform register
