@@ -50,8 +50,26 @@ __device__ __forceinline__ uint8_t f32_to_e4m3(float value) {
 
 // Programmatic dependent launch: a kernel may start while its predecessor in
 // the stream drains; everything before grid_dependency_wait() must not read
-// data the predecessor writes (weight prefetch is fine).
+// data the predecessor writes (weight prefetch is fine).  Pointers to such data,
+// and to outputs, are not __restrict__ and not read by __ldg: either promises that
+// nobody else writes there while the kernel runs, and lets the compiler move the
+// access in front of the wait.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// By a CTA: a row that does not overlap its copy, four loads of a thread in flight (which may not pass a store that might be to the same place).
+template <typename Word>
+__device__ __forceinline__ void copy_row(Word *to, const Word *from, int words) {
+    constexpr int BATCH = 4;
+    for (int first = threadIdx.x; first < words; first += BATCH * blockDim.x) {
+        Word held[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (first + i * static_cast<int>(blockDim.x) < words) held[i] = from[first + i * blockDim.x];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (first + i * static_cast<int>(blockDim.x) < words) to[first + i * blockDim.x] = held[i];
+    }
+}
 
 }  // namespace nerve

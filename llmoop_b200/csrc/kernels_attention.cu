@@ -412,8 +412,8 @@ struct AttentionF32 {
 // A batch may mix streams: each stream contributes `lanes_per_stream` consecutive lanes, and a CTA never spans two streams.
 template <int HD, int GROUP, int QL>
 __global__ void __launch_bounds__(128)
-attention_f32_kernel(const uint16_t *__restrict__ q, KvLayer kv, LaneTable lanes_meta, int lanes, int lanes_per_stream,
-                     int q_heads, float scale, int split_tokens, int max_splits, float *__restrict__ scratch, const AttentionBlock *__restrict__ ragged) {
+attention_f32_kernel(const uint16_t *q, KvLayer kv, LaneTable lanes_meta, int lanes, int lanes_per_stream,
+                     int q_heads, float scale, int split_tokens, int max_splits, float *scratch, const AttentionBlock *ragged) {
     using Form = AttentionF32<HD, GROUP, QL>;
     constexpr int Q = Form::Q, THREADS = Form::THREADS;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -629,7 +629,7 @@ attention_f32_kernel(const uint16_t *__restrict__ q, KvLayer kv, LaneTable lanes
 // Log-sum-exp merge of the split partials of one (lane, q head) pair by one warp: thread s weighs split s, the weighted
 // partials are added split by split in order, as are the sums.  (Every thread weighing every split for each of its dims, one
 // load after the other: 9 us for 17 splits; this, the first rows requested along with the states, 3.3.)
-__global__ void attention_f32_merge_kernel(const float *__restrict__ scratch, uint16_t *__restrict__ out, KvLayer kv,
+__global__ void attention_f32_merge_kernel(const float *scratch, uint16_t *out, KvLayer kv,
                                            LaneTable lanes_meta, int lanes, int q_heads, int head_width, int split_tokens,
                                            int max_splits) {
     grid_launch_dependents();
@@ -712,7 +712,7 @@ cudaError_t launch_f32_of_width(const AttentionArgs &args, cudaStream_t stream) 
 // 16-byte words, else 0.  The rows of a token are requested together, and the merge halves the dims a thread holds with
 // every exchange.  (Element by element and five exchanges per dim: 7.6 us for a 50-token context; this 2.5.)
 template <int HD>
-__global__ void attention_small_kernel(const uint16_t *__restrict__ q, uint16_t *__restrict__ out, KvLayer kv,
+__global__ void attention_small_kernel(const uint16_t *q, uint16_t *out, KvLayer kv,
                                        LaneTable lanes_meta, int lanes, int q_heads, float scale) {
     constexpr int WIDTH = HD > 0 ? HD : 32;
     grid_launch_dependents();
@@ -797,7 +797,7 @@ __global__ void attention_small_kernel(const uint16_t *__restrict__ q, uint16_t 
 }
 
 // Log-sum-exp merge of the split partials; one warp per (lane, q head).
-__global__ void attention_merge_kernel(const float *__restrict__ scratch, uint16_t *__restrict__ out, KvLayer kv,
+__global__ void attention_merge_kernel(const float *scratch, uint16_t *out, KvLayer kv,
                                        LaneTable lanes_meta, int lanes, int q_heads, int head_width, int split_tokens,
                                        int max_splits) {
     grid_launch_dependents();
@@ -1106,8 +1106,7 @@ __device__ __forceinline__ void argmax_block_reduce(float &best, uint32_t &token
     }
 }
 
-__global__ void argmax_partial_kernel(const float *__restrict__ logits, float *__restrict__ partial_logit,
-                                      uint32_t *__restrict__ partial_token, int vocab) {
+__global__ void argmax_partial_kernel(const float *logits, float *partial_logit, uint32_t *partial_token, int vocab) {
     grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float shared_logit[32];
@@ -1133,8 +1132,7 @@ __global__ void argmax_partial_kernel(const float *__restrict__ logits, float *_
     }
 }
 
-__global__ void argmax_final_kernel(const float *__restrict__ partial_logit, const uint32_t *__restrict__ partial_token,
-                                    uint32_t *__restrict__ records) {
+__global__ void argmax_final_kernel(const float *partial_logit, const uint32_t *partial_token, uint32_t *records) {
     grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float shared_logit[32];

@@ -14,15 +14,13 @@ __device__ __forceinline__ unsigned long long global_time() {
     return now;
 }
 
-__global__ void gather_rows_kernel(const uint32_t *__restrict__ src, const int32_t *__restrict__ index,
-                                   uint32_t *__restrict__ dst, int words) {
+__global__ void gather_rows_kernel(const uint32_t *src, const int32_t *index, uint32_t *dst, int words) {
     grid_launch_dependents();
     grid_dependency_wait();
     int row = blockIdx.x;
     int source = index[row];
     if (source < 0) return;
-    for (int word = threadIdx.x; word < words; word += blockDim.x)
-        dst[static_cast<size_t>(row) * words + word] = src[static_cast<size_t>(source) * words + word];
+    copy_row(dst + static_cast<size_t>(row) * words, src + static_cast<size_t>(source) * words, words);
 }
 
 cudaError_t launch_gather_rows(const uint16_t *src, const int32_t *index, uint16_t *dst, int rows, int width,
@@ -36,8 +34,8 @@ cudaError_t launch_gather_rows(const uint16_t *src, const int32_t *index, uint16
 // the host's words, too: the blocks do not wait for one another.
 // (A copy at either end of the graph took its time and one at its border to the kernels, which no early start of the next
 // kernel hides: a cycle of two layers of hidden 64 with one draft took 76 us with them and takes 70.)
-__global__ void begin_cycle_kernel(const uint32_t *host_state, uint32_t *state, int state_words, const uint32_t *__restrict__ pending, const int32_t *slots,
-                                   uint32_t *__restrict__ gathered, int rows, uint32_t *__restrict__ backup, int words, unsigned long long *marks) {
+__global__ void begin_cycle_kernel(const uint32_t *host_state, uint32_t *state, int state_words, const uint32_t *pending, const int32_t *slots,
+                                   uint32_t *gathered, int rows, uint32_t *backup, int words, unsigned long long *marks) {
     grid_launch_dependents();
     grid_dependency_wait();
     const int block = blockIdx.x;
@@ -47,7 +45,7 @@ __global__ void begin_cycle_kernel(const uint32_t *host_state, uint32_t *state, 
     if (source < 0) return;
     const uint32_t *from = pending + static_cast<size_t>(source) * words;
     uint32_t *to = block < rows ? gathered + static_cast<size_t>(block) * words : backup + static_cast<size_t>(source) * words;
-    for (int word = threadIdx.x; word < words; word += blockDim.x) to[word] = from[word];
+    copy_row(to, from, words);
 }
 cudaError_t launch_begin_cycle(const uint32_t *host_state, uint32_t *state, int state_words, const uint16_t *pending, const int32_t *host_slots, uint16_t *gathered, int rows,
                                uint16_t *backup, int max_streams, int hidden, unsigned long long *marks, cudaStream_t stream) {
@@ -70,8 +68,7 @@ cudaError_t launch_finish_cycle(const uint32_t *results, int words, unsigned lon
     return launch_dependent(finish_cycle_kernel, dim3(1), dim3(256), 0, 1, stream, results, words, marks, error_word, host_results);
 }
 
-__global__ void shift_hidden_kernel(const uint32_t *__restrict__ pending, const int32_t *__restrict__ slots,
-                                    const uint32_t *__restrict__ normalized, uint32_t *__restrict__ dst,
+__global__ void shift_hidden_kernel(const uint32_t *pending, const int32_t *slots, const uint32_t *normalized, uint32_t *dst,
                                     int lanes_per_stream, int words, unsigned long long *marks) {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -80,7 +77,7 @@ __global__ void shift_hidden_kernel(const uint32_t *__restrict__ pending, const 
     int s = lane / lanes_per_stream, i = lane % lanes_per_stream;
     const uint32_t *source = i == 0 ? pending + static_cast<size_t>(slots[s]) * words
                                     : normalized + static_cast<size_t>(lane - 1) * words;
-    for (int word = threadIdx.x; word < words; word += blockDim.x) dst[static_cast<size_t>(lane) * words + word] = source[word];
+    copy_row(dst + static_cast<size_t>(lane) * words, source, words);
 }
 
 cudaError_t launch_shift_hidden(const uint16_t *pending, const int32_t *slots, const uint16_t *normalized,
@@ -90,14 +87,13 @@ cudaError_t launch_shift_hidden(const uint16_t *pending, const int32_t *slots, c
 }
 
 // Prefill batches: the lanes of a stream are neighbours, a lane whose neighbour has another slot is its stream's first or last.
-__global__ void shift_hidden_lanes_kernel(const uint32_t *__restrict__ pending, const int32_t *__restrict__ slots, const uint32_t *__restrict__ normalized,
-                                          uint32_t *__restrict__ dst, int words) {
+__global__ void shift_hidden_lanes_kernel(const uint32_t *pending, const int32_t *slots, const uint32_t *normalized, uint32_t *dst, int words) {
     grid_launch_dependents();
     grid_dependency_wait();
     const int lane = blockIdx.x;
     const bool first = lane == 0 || slots[lane - 1] != slots[lane];
     const uint32_t *source = first ? pending + static_cast<size_t>(slots[lane]) * words : normalized + static_cast<size_t>(lane - 1) * words;
-    for (int word = threadIdx.x; word < words; word += blockDim.x) dst[static_cast<size_t>(lane) * words + word] = source[word];
+    copy_row(dst + static_cast<size_t>(lane) * words, source, words);
 }
 cudaError_t launch_shift_hidden_lanes(const uint16_t *pending, const int32_t *slots, const uint16_t *normalized, uint16_t *dst, int lanes, int hidden,
                                       cudaStream_t stream) {
@@ -106,13 +102,12 @@ cudaError_t launch_shift_hidden_lanes(const uint16_t *pending, const int32_t *sl
                             reinterpret_cast<const uint32_t *>(normalized), reinterpret_cast<uint32_t *>(dst), hidden / 2);
 }
 
-__global__ void commit_hidden_kernel(const uint32_t *__restrict__ normalized, const int32_t *__restrict__ slots, uint32_t *__restrict__ pending, int words) {
+__global__ void commit_hidden_kernel(const uint32_t *normalized, const int32_t *slots, uint32_t *pending, int words) {
     grid_launch_dependents();
     grid_dependency_wait();
     const int lane = blockIdx.x;
     if (lane + 1 < static_cast<int>(gridDim.x) && slots[lane + 1] == slots[lane]) return;
-    for (int word = threadIdx.x; word < words; word += blockDim.x)
-        pending[static_cast<size_t>(slots[lane]) * words + word] = normalized[static_cast<size_t>(lane) * words + word];
+    copy_row(pending + static_cast<size_t>(slots[lane]) * words, normalized + static_cast<size_t>(lane) * words, words);
 }
 cudaError_t launch_commit_hidden(const uint16_t *normalized, const int32_t *slots, uint16_t *pending, int lanes, int hidden, cudaStream_t stream) {
     if (lanes <= 0) return cudaSuccess;
@@ -120,9 +115,8 @@ cudaError_t launch_commit_hidden(const uint16_t *normalized, const int32_t *slot
                             reinterpret_cast<uint32_t *>(pending), hidden / 2);
 }
 
-__global__ void draft_select_kernel(const uint32_t *__restrict__ records, const uint32_t *__restrict__ forced, int step,
-                                    int streams, int drafts, uint32_t *__restrict__ next_tokens,
-                                    uint32_t *__restrict__ verify_tokens, unsigned long long *marks) {
+__global__ void draft_select_kernel(const uint32_t *records, const uint32_t *forced, int step, int streams, int drafts, uint32_t *next_tokens,
+                                    uint32_t *verify_tokens, unsigned long long *marks) {
     grid_launch_dependents();
     grid_dependency_wait();
     int s = blockIdx.x * blockDim.x + threadIdx.x;
@@ -143,10 +137,9 @@ cudaError_t launch_draft_select(const uint32_t *records, const uint32_t *forced,
     return launch_dependent(draft_select_kernel, dim3((streams + 63) / 64), dim3(64), 0, 1, stream, records, forced, step, streams, drafts, next_tokens, verify_tokens, marks);
 }
 
-__global__ void accept_kernel(const uint32_t *__restrict__ verify_tokens, const uint32_t *__restrict__ target_records,
-                              const uint32_t *__restrict__ stop_tokens, const int32_t *__restrict__ stop_counts,
-                              const int32_t *__restrict__ own_drafts, int max_stop, int drafts, uint32_t *__restrict__ out, const uint32_t *__restrict__ normalized,
-                              uint32_t *__restrict__ pending, const int32_t *__restrict__ slots, int words) {
+__global__ void accept_kernel(const uint32_t *verify_tokens, const uint32_t *target_records, const uint32_t *stop_tokens, const int32_t *stop_counts,
+                              const int32_t *own_drafts, int max_stop, int drafts, uint32_t *out, const uint32_t *normalized, uint32_t *pending,
+                              const int32_t *slots, int words) {
     grid_launch_dependents();
     grid_dependency_wait();
     __shared__ int committed_shared;
@@ -177,13 +170,13 @@ __global__ void accept_kernel(const uint32_t *__restrict__ verify_tokens, const 
         row[1] = static_cast<uint32_t>(committed);
         row[2] = static_cast<uint32_t>(count);
         row[3] = 0u;
-        for (int i = 0; i < width; i++) row[4 + width + i] = target_records[(static_cast<size_t>(s) * width + i) * 4];
         committed_shared = committed;
     }
+    for (int i = threadIdx.x; i < width; i += blockDim.x) row[4 + width + i] = target_records[(static_cast<size_t>(s) * width + i) * 4];
     __syncthreads();
     const uint32_t *source = normalized + (static_cast<size_t>(s) * width + committed_shared - 1) * words;
     uint32_t *destination = pending + static_cast<size_t>(slots[s]) * words;
-    for (int word = threadIdx.x; word < words; word += blockDim.x) destination[word] = source[word];
+    copy_row(destination, source, words);
 }
 
 cudaError_t launch_accept(const uint32_t *verify_tokens, const uint32_t *target_records, const uint32_t *stop_tokens,
@@ -199,7 +192,7 @@ cudaError_t launch_accept(const uint32_t *verify_tokens, const uint32_t *target_
 // payload): the logit bits in the first word, the global token id in the second; a reader accepts a pair once both
 // carry the number of the vote in progress.  Parities alternate per vote: a rank can only be one vote ahead of a
 // peer (it needs the peer's word of vote v before it can finish v), so the slot of vote v + 2 is free by then.
-__global__ void tensor_parallel_argmax_kernel(const uint32_t *__restrict__ records_local, uint32_t first_token, uint32_t *__restrict__ records,
+__global__ void tensor_parallel_argmax_kernel(const uint32_t *records_local, uint32_t first_token, uint32_t *records,
                                               int lanes, const StackTp *__restrict__ tp_pointer, int *error_flag) {
     grid_launch_dependents();
     grid_dependency_wait();

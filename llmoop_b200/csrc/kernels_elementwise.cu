@@ -11,6 +11,20 @@
 
 namespace nerve {
 
+// Words first, first + step ... in front of `count`: store(word, load(word)), BATCH loads of a thread in flight.
+template <int BATCH = 4, typename Load, typename Store>
+__device__ __forceinline__ void in_batches(size_t first, size_t step, size_t count, Load load, Store store) {
+    for (; first < count; first += BATCH * step) {
+        decltype(load(first)) held[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (first + i * step < count) held[i] = load(first + i * step);
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (first + i * step < count) store(first + i * step, held[i]);
+    }
+}
+
 // Bound by the pages' bytes (32 pages of 64 KB in 33 layers: 140 MB moved); four CTAs share a page so that a single
 // stream's page still spreads over the chip.
 constexpr int PAGE_COPY_PARTS = 4;
@@ -37,8 +51,8 @@ cudaError_t launch_copy_pages(const PagePool *pools, int layers, const PageCopy 
 
 // embedding_lookup_bf16.comp.template:31-46: out = bf16(bf16(row) * scale); a
 // token id >= vocab leaves the frame untouched.
-__global__ void embedding_kernel(const uint32_t *__restrict__ table, const uint32_t *__restrict__ tokens,
-                                 uint32_t *__restrict__ out, int width_words, int vocab, float scale) {
+__global__ void embedding_kernel(const uint32_t *__restrict__ table, const uint32_t *tokens,
+                                 uint32_t *out, int width_words, int vocab, float scale) {
     grid_launch_dependents();
     grid_dependency_wait();
     int lane = blockIdx.y;
@@ -61,8 +75,8 @@ cudaError_t launch_embedding(const uint16_t *table, const uint32_t *tokens, uint
 // latency, not bandwidth.  A thread's words (WORDS of them, blockDim apart, or more than that in a loop) and their weights
 // are requested together and stay in registers between the two passes (one lane of 4096: 4.1 -> 1.7 us).
 template <int WORDS>
-__global__ void rms_norm_kernel(const uint32_t *__restrict__ x, const uint32_t *__restrict__ weight,
-                                uint32_t *__restrict__ y, int width_words, float inv_width, float eps, float offset) {
+__global__ void rms_norm_kernel(const uint32_t *x, const uint32_t *__restrict__ weight,
+                                uint32_t *y, int width_words, float inv_width, float eps, float offset) {
     __shared__ float partial[32];
     const uint32_t *row = x + static_cast<size_t>(blockIdx.x) * width_words;
     uint32_t *out = y + static_cast<size_t>(blockIdx.x) * width_words;
@@ -90,7 +104,7 @@ __global__ void rms_norm_kernel(const uint32_t *__restrict__ x, const uint32_t *
         for (int i = 0; i < WORDS; i++)
             if (static_cast<int>(threadIdx.x) + i * step < width_words) square(values[i]);
     } else {
-        for (int word = threadIdx.x; word < width_words; word += step) square(row[word]);
+        in_batches<8>(threadIdx.x, step, width_words, [&](size_t word) { return row[word]; }, [&](size_t, uint32_t value) { square(value); });
     }
     sum = warp_sum(sum);
     if ((threadIdx.x & 31) == 0) partial[threadIdx.x >> 5] = sum;
@@ -105,7 +119,7 @@ __global__ void rms_norm_kernel(const uint32_t *__restrict__ x, const uint32_t *
         for (int i = 0; i < WORDS; i++)
             if (static_cast<int>(threadIdx.x) + i * step < width_words) out[threadIdx.x + i * step] = norm(values[i], weights[i]);
     } else {
-        for (int word = threadIdx.x; word < width_words; word += step) out[word] = norm(row[word], weight[word]);
+        in_batches(threadIdx.x, step, width_words, [&](size_t word) { return make_uint2(row[word], weight[word]); }, [&](size_t word, uint2 v) { out[word] = norm(v.x, v.y); });
     }
 }
 
@@ -119,15 +133,11 @@ cudaError_t launch_rms_norm(const uint16_t *x, const uint16_t *weight, uint16_t 
 }
 
 // add_bf16.comp.template:17-24
-__global__ void add_kernel(const uint32_t *__restrict__ a, const uint32_t *__restrict__ b, uint32_t *__restrict__ y,
-                           size_t words) {
+__global__ void add_kernel(const uint32_t *a, const uint32_t *b, uint32_t *y, size_t words) {
     grid_launch_dependents();
     grid_dependency_wait();
-    for (size_t word = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; word < words;
-         word += static_cast<size_t>(gridDim.x) * blockDim.x) {
-        uint32_t left = a[word], right = b[word];
-        y[word] = pack_bf16(bf16_lo(left) + bf16_lo(right), bf16_hi(left) + bf16_hi(right));
-    }
+    in_batches(blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x, static_cast<size_t>(gridDim.x) * blockDim.x, words, [&](size_t word) { return make_uint2(a[word], b[word]); },
+               [&](size_t word, uint2 v) { y[word] = pack_bf16(bf16_lo(v.x) + bf16_lo(v.y), bf16_hi(v.x) + bf16_hi(v.y)); });
 }
 
 cudaError_t launch_add(const uint16_t *a, const uint16_t *b, uint16_t *y, size_t count, cudaStream_t stream) {
@@ -140,16 +150,16 @@ cudaError_t launch_add(const uint16_t *a, const uint16_t *b, uint16_t *y, size_t
 
 // After the tensor-parallel all-reduce of a row-parallel linear: the reference's linear rounds its f32 sum to bf16
 // and its residual_add rounds again (add_bf16.comp.template:17-24).
-__global__ void round_add_kernel(const float *__restrict__ sums, const uint16_t *__restrict__ residual, uint16_t *__restrict__ out,
-                                 size_t count) {
+__global__ void round_add_kernel(const float *sums, const uint16_t *residual, uint16_t *out, size_t count) {
     grid_launch_dependents();
     grid_dependency_wait();
-    for (size_t index = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; index < count;
-         index += static_cast<size_t>(gridDim.x) * blockDim.x) {
-        float value = round_bf16(sums[index]);
-        if (residual != nullptr) value += bf16_bits_to_f32(residual[index]);
-        out[index] = static_cast<uint16_t>(f32_to_bf16_bits(value));
-    }
+    in_batches(blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x, static_cast<size_t>(gridDim.x) * blockDim.x, count,
+               [&](size_t index) { return make_float2(sums[index], residual != nullptr ? bf16_bits_to_f32(residual[index]) : 0.0f); },
+               [&](size_t index, float2 v) {
+                   float value = round_bf16(v.x);
+                   if (residual != nullptr) value += v.y;
+                   out[index] = static_cast<uint16_t>(f32_to_bf16_bits(value));
+               });
 }
 
 cudaError_t launch_round_add(const float *sums, const uint16_t *residual, uint16_t *out, size_t count, cudaStream_t stream) {
@@ -160,15 +170,11 @@ cudaError_t launch_round_add(const float *sums, const uint16_t *residual, uint16
 }
 
 // silu_multiply_bf16.comp.template:30-52: bf16(bf16(silu(gate)) * up)
-__global__ void silu_multiply_kernel(const uint32_t *__restrict__ gate, const uint32_t *__restrict__ up,
-                                     uint32_t *__restrict__ y, size_t words) {
+__global__ void silu_multiply_kernel(const uint32_t *gate, const uint32_t *up, uint32_t *y, size_t words) {
     grid_launch_dependents();
     grid_dependency_wait();
-    for (size_t word = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; word < words;
-         word += static_cast<size_t>(gridDim.x) * blockDim.x) {
-        uint32_t g = gate[word], u = up[word];
-        y[word] = pack_bf16(rounded_silu(bf16_lo(g)) * bf16_lo(u), rounded_silu(bf16_hi(g)) * bf16_hi(u));
-    }
+    in_batches(blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x, static_cast<size_t>(gridDim.x) * blockDim.x, words, [&](size_t word) { return make_uint2(gate[word], up[word]); },
+               [&](size_t word, uint2 v) { y[word] = pack_bf16(rounded_silu(bf16_lo(v.x)) * bf16_lo(v.y), rounded_silu(bf16_hi(v.x)) * bf16_hi(v.y)); });
 }
 
 cudaError_t launch_silu_multiply(const uint16_t *gate, const uint16_t *up, uint16_t *y, size_t count,
@@ -182,15 +188,15 @@ cudaError_t launch_silu_multiply(const uint16_t *gate, const uint16_t *up, uint1
 
 // concatenate_bf16.comp.template:20-30 (per lane: [a | b])
 template <typename Word>
-__global__ void concat_kernel(const Word *__restrict__ a, const Word *__restrict__ b, Word *__restrict__ y,
-                              int words_a, int words_b) {
+__global__ void concat_kernel(const Word *a, const Word *b, Word *y, int words_a, int words_b) {
     grid_launch_dependents();
     grid_dependency_wait();
     int lane = blockIdx.x;
     int total = words_a + words_b;
-    for (int word = blockIdx.y * blockDim.x + threadIdx.x; word < total; word += gridDim.y * blockDim.x)
-        y[static_cast<size_t>(lane) * total + word] =
-            word < words_a ? a[static_cast<size_t>(lane) * words_a + word] : b[static_cast<size_t>(lane) * words_b + word - words_a];
+    const Word *row_a = a + static_cast<size_t>(lane) * words_a, *row_b = b + static_cast<size_t>(lane) * words_b;
+    Word *row = y + static_cast<size_t>(lane) * total;
+    in_batches(blockIdx.y * blockDim.x + threadIdx.x, gridDim.y * blockDim.x, total, [&](size_t word) { return word < static_cast<size_t>(words_a) ? row_a[word] : row_b[word - words_a]; },
+               [&](size_t word, Word value) { row[word] = value; });
 }
 
 cudaError_t launch_concat(const uint16_t *a, const uint16_t *b, uint16_t *y, int lanes, int width_a, int width_b,
@@ -206,8 +212,8 @@ cudaError_t launch_concat(const uint16_t *a, const uint16_t *b, uint16_t *y, int
 // sequence; parallel_head_norm_rope_2way_bf16.comp.template:166-209 when
 // norm_weight is given (per-head RMSNorm rounded to bf16 first).
 // One CTA per (head, lane); blockDim = head_width/2 rounded up to a warp.
-__global__ void rope_kernel(const uint16_t *__restrict__ x, uint16_t *__restrict__ y, const uint32_t *__restrict__ cos_sin,
-                            uint32_t table_positions, const uint32_t *__restrict__ positions, int heads, int head_width,
+__global__ void rope_kernel(const uint16_t *x, uint16_t *y, const uint32_t *__restrict__ cos_sin,
+                            uint32_t table_positions, const uint32_t *positions, int heads, int head_width,
                             int rotary, int interleaved, const uint16_t *__restrict__ norm_weight, float eps, float offset) {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -265,8 +271,7 @@ cudaError_t launch_rope(const uint16_t *x, uint16_t *y, const uint32_t *cos_sin,
 
 // quantize_fp8_e4m3.comp.template:41-60: per 128-column block scale = absmax/448
 // (1 when the block is all zero), q = e4m3(x / scale).  One warp per block.
-__global__ void quantize_fp8_kernel(const uint32_t *__restrict__ x, uint32_t *__restrict__ q, float *__restrict__ scales,
-                                    int blocks_total) {
+__global__ void quantize_fp8_kernel(const uint32_t *x, uint32_t *q, float *scales, int blocks_total) {
     grid_launch_dependents();
     grid_dependency_wait();
     int block = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -299,8 +304,7 @@ cudaError_t launch_quantize_fp8(const uint16_t *x, uint8_t *q, float *scales, in
 // One warp per token.  A score and its expert make one key (bf16 bits in an order of unsigned numbers, then the smaller
 // expert first), so that a choice is one warp-wide maximum: bound by that chain of top_k steps (128 experts, top 8: 9.7 us
 // with five exchanges of two values per step and one thread for the weights, now 3.6).
-__global__ void moe_topk_kernel(const uint16_t *__restrict__ router_logits, uint32_t *__restrict__ routes, int experts,
-                                int top_k) {
+__global__ void moe_topk_kernel(const uint16_t *router_logits, uint32_t *routes, int experts, int top_k) {
     extern __shared__ uint16_t scores[];  // [experts] in an order of unsigned numbers; 0: chosen, or never to be chosen (-inf, NaN)
     __shared__ int selected[64];
     __shared__ float terms[64];
@@ -356,8 +360,7 @@ cudaError_t launch_moe_topk(const uint16_t *router_logits, uint32_t *routes, int
 // in route (expert-id) order, then * routed scale.
 // A thread adds one word up; its contributions are requested eight at a time (one after the other, four words a thread: 5.8 us
 // for 24 tokens of 2048, now 1.6).
-__global__ void moe_reduce_kernel(const uint32_t *__restrict__ outputs, uint32_t *__restrict__ y, int hidden_words,
-                                  int top_k, float routed_scale) {
+__global__ void moe_reduce_kernel(const uint32_t *outputs, uint32_t *y, int hidden_words, int top_k, float routed_scale) {
     grid_launch_dependents();
     grid_dependency_wait();
     const int token = blockIdx.x, word = blockIdx.y * blockDim.x + threadIdx.x;

@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(FP8_WARPS * 32, 2) linear_silu_multiply_fp8_ke
 // Groups the (token, route) pairs by expert: order[] = pair indices expert by expert, tiles[t] = {expert, first place in
 // order, count <= 8}, tile_count.  One CTA.
 constexpr int GROUP_THREADS = 1024, GROUP_MAX_EXPERTS = 1024;
-__global__ void __launch_bounds__(GROUP_THREADS) moe_group_kernel(const uint32_t *__restrict__ routes, int pairs, int experts, MoeGroups groups) {
+__global__ void __launch_bounds__(GROUP_THREADS) moe_group_kernel(const uint32_t *routes, int pairs, int experts, MoeGroups groups) {
     __shared__ int counts[GROUP_MAX_EXPERTS], places[GROUP_MAX_EXPERTS], tile_places[GROUP_MAX_EXPERTS];
     __shared__ int warp_pairs[32], warp_tiles[32];
     grid_launch_dependents();
@@ -363,9 +363,14 @@ __global__ void __launch_bounds__(GROUP_THREADS) moe_group_kernel(const uint32_t
     for (int t = 0; t < own_tiles; t++) groups.tiles[tile_places[e] + t] = make_int4(e, places[e] + t * TILE_LANES, min(TILE_LANES, own - t * TILE_LANES), 0);
     if (e == GROUP_MAX_EXPERTS - 1) *groups.tile_count = tile_base + tiles_before;
     __syncthreads();
-    for (int pair = threadIdx.x; pair < pairs; pair += GROUP_THREADS) {
-        const int expert = expert_of(pair);
-        if (expert >= 0) groups.order[atomicAdd(&places[expert], 1)] = pair;
+    constexpr int BATCH = 4;  // loads in flight
+    for (int first = threadIdx.x; first < pairs; first += BATCH * GROUP_THREADS) {
+        int held[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) held[i] = first + i * GROUP_THREADS < pairs ? expert_of(first + i * GROUP_THREADS) : -1;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (held[i] >= 0) groups.order[atomicAdd(&places[held[i]], 1)] = first + i * GROUP_THREADS;
     }
 }
 

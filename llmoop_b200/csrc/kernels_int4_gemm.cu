@@ -586,8 +586,8 @@ __global__ void __launch_bounds__(gemm_threads<ROW_TILES>(), ROW_TILES == 1 ? 2 
 // norm's weights are nobody's output and are on their way while the kernel in front still runs (32 x 4096: 4.1 -> 2.7 us).
 constexpr int PREPARE_THREADS = 512;
 template <bool NORM, int HELD>
-__global__ void __launch_bounds__(PREPARE_THREADS) prepare_activations_kernel(const uint16_t *__restrict__ x, const uint16_t *__restrict__ weight, float eps,
-                                                                             float weight_offset, uint8_t *__restrict__ out, float *__restrict__ factors, int lanes,
+__global__ void __launch_bounds__(PREPARE_THREADS) prepare_activations_kernel(const uint16_t *x, const uint16_t *__restrict__ weight, float eps,
+                                                                             float weight_offset, uint8_t *out, float *factors, int lanes,
                                                                              int lane_blocks, int k) {
     constexpr int WARPS = PREPARE_THREADS / 32, REGISTERS = HELD > 0 ? HELD : 1;
     extern __shared__ __align__(16) uint4 normalised[];
@@ -657,10 +657,9 @@ __global__ void __launch_bounds__(PREPARE_THREADS) prepare_activations_kernel(co
     const int exponent = max(static_cast<int>(largest >> 7), 16);
     const float factor = power_of_two(min(268 - exponent, 254));
     if (m < lanes && threadIdx.x == 0) factors[m] = power_of_two(max(exponent - 14, 1));
-    each_piece([&](int i, int p) {
+    auto write = [&](int p, const uint4 &v) {
         uint4 packed = make_uint4(0, 0, 0, 0);
         if (m < lanes) {
-            const uint4 v = HELD > 0 ? held[i] : NORM ? normalised[p] : row[p];
             auto both = [&](uint32_t lo, uint32_t hi) {
                 const __half2 h = __floats2half2_rn(__uint_as_float(lo) * factor, __uint_as_float(hi) * factor);
                 return *reinterpret_cast<const uint32_t *>(&h);
@@ -671,7 +670,21 @@ __global__ void __launch_bounds__(PREPARE_THREADS) prepare_activations_kernel(co
             packed.w = both(v.y & 0xffff0000u, v.w & 0xffff0000u);
         }
         *reinterpret_cast<uint4 *>(out + (static_cast<size_t>(p >> 3) * lane_blocks + (m >> 3)) * 1024 + (m & 7) * 128 + (((p & 7) ^ (m & 7)) * 16)) = packed;
-    });
+    };
+    if (HELD > 0 || NORM) {
+        each_piece([&](int i, int p) { write(p, HELD > 0 ? held[i] : normalised[p]); });
+    } else {
+        constexpr int BATCH = 4;  // loads in flight
+        for (int first = threadIdx.x; first < pieces; first += BATCH * PREPARE_THREADS) {
+            uint4 again[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++)
+                if (m < lanes && first + i * PREPARE_THREADS < pieces) again[i] = row[first + i * PREPARE_THREADS];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++)
+                if (first + i * PREPARE_THREADS < pieces) write(first + i * PREPARE_THREADS, again[i]);
+        }
+    }
 }
 template <bool NORM>
 auto prepare_kernel(int k) {
