@@ -1631,7 +1631,11 @@ cudaError_t launch_dense(const uint16_t *x, const int8_t *w, const float *scales
     Int8Args args = {};
     args.lanes = lanes, args.n = n, args.k = k, args.to_f32 = to_f32, args.error_flag = error_flag;
     if (lanes <= STREAM_LANES) {
-        const bool own = lanes <= FEW && static_cast<int64_t>(lanes) * k <= STREAM_OWN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+        // (no CTA writes onto a row that another one may still have to quantise)
+        const uintptr_t x_at = reinterpret_cast<uintptr_t>(x), y_at = reinterpret_cast<uintptr_t>(y), x_bytes = static_cast<uintptr_t>(lanes) * k * 2,
+                        y_bytes = static_cast<uintptr_t>(lanes) * n * (to_f32 ? 4 : 2);
+        const bool apart = x_at >= y_at + y_bytes || y_at >= x_at + x_bytes;
+        const bool own = lanes <= FEW && static_cast<int64_t>(lanes) * k <= STREAM_OWN && x_at % 16 == 0 && apart;
         StreamArgs few = {};
         few.x = x, few.scales = scales, few.up_scales = up_scales, few.lane_scales = rows.scales, few.y = y, few.residual = residual;
         few.lanes = lanes, few.n = n, few.k = k, few.to_f32 = to_f32, few.error_flag = error_flag;
