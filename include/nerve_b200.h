@@ -288,10 +288,11 @@ int32_t nerve_b200_op_linear_fp8(const void *x_device, const void *w_device, con
  * k rounded up to a multiple of 128 and up to 128 lanes to a multiple of 16 (up to eight lanes: of 8), and four bytes a lane, both
  * rounded up to 256 bytes; for nine lanes or more of at least 4096 columns up to 16.8 MB more, in which split sums meet.  Its
  * contents need not be kept or cleared between calls; calls that may overlap in time, captured graphs among them, need one
- * each.  0 lanes or tokens: nothing is done.
+ * each.  0 lanes or tokens: nothing is done.  y may be or overlap x; beyond that, and where residual says so, y, scratch and the
+ * inputs share no byte (refused where a call can tell).
  */
 uint64_t nerve_b200_op_linear_int8_scratch_bytes(int32_t lanes, int32_t k);
-/* y[lane][n] = x . W^T (+ residual bf16 [lanes][n], which may be y itself), bf16, or f32 where to_f32 != 0. */
+/* y[lane][n] = x . W^T (+ residual bf16 [lanes][n], which may be a bf16 y itself), bf16, or f32 where to_f32 != 0. */
 int32_t nerve_b200_op_linear_int8(const void *x_device, const void *w_device, const void *wscale_device, void *y_device,
                                   const void *residual_device, void *scratch_device, int32_t lanes, int32_t n, int32_t k,
                                   int32_t to_f32, void *stream);

@@ -3,6 +3,7 @@
 #include <cstring>
 #include <mutex>
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/nerve_b200.h"
@@ -200,6 +201,20 @@ void check_size(const char *name, const char *what, int64_t value, int64_t least
     if (value < least || value > most || value % multiple != 0)
         throw std::runtime_error(std::string(name) + ": " + what + " is " + std::to_string(value) + ", must be " + std::to_string(least) + " to " + std::to_string(most) +
                                  (multiple > 1 ? " and a multiple of " + std::to_string(multiple) : ""));
+}
+struct Span {
+    const char *what;
+    const void *pointer;  // NULL: none
+    size_t bytes;
+};
+// What a call writes may share no byte with what its kernels read or write in any order beside it.
+void check_apart(const char *name, const Span &written, std::initializer_list<Span> others) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(written.pointer);
+    for (const Span &other : others) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(other.pointer);
+        if (other.pointer != nullptr && at < first + written.bytes && first < at + other.bytes)
+            throw std::runtime_error(std::string(name) + ": " + written.what + " and " + other.what + " overlap");
+    }
 }
 constexpr int64_t INT8_MAX_LANES = 1 << 20, INT8_MAX_CHANNELS = 1 << 24, EXPERTS_MAX_ROUTES = 1 << 24;
 void check_int8_sizes(const char *name, int32_t lanes, int32_t n, int32_t k) {
@@ -692,6 +707,11 @@ int32_t nerve_b200_op_linear_int8(const void *x, const void *w, const void *wsca
         check_pointer(name, "y", y, to_f32 ? 4 : 2);
         check_pointer(name, "residual", residual, 2, true);
         check_pointer(name, "scratch", scratch, 16);
+        const size_t outputs = static_cast<size_t>(lanes) * n;
+        const Span inputs{"x", x, static_cast<size_t>(lanes) * k * 2}, added{"residual", residual == y && !to_f32 ? nullptr : residual, outputs * 2},
+            out{"y", y, outputs * (to_f32 ? 4 : 2)};
+        check_apart(name, out, {added});  // (y may be x)
+        check_apart(name, {"scratch", scratch, linear_int8_scratch_bytes(lanes, k)}, {inputs, added, out});
     });
     if (checked != NERVE_B200_OK || lanes == 0) return checked;
     return linear_call(name, true, [&](const OperatorDevice *device) {
@@ -713,6 +733,8 @@ int32_t nerve_b200_op_linear_int8_silu_pair(const void *x, const void *gate_w, c
         check_pointer(name, "up_scale", up_scale, 4);
         check_pointer(name, "y", y, 2);
         check_pointer(name, "scratch", scratch, 16);
+        const Span inputs{"x", x, static_cast<size_t>(lanes) * k * 2}, out{"y", y, static_cast<size_t>(lanes) * n * 2};
+        check_apart(name, {"scratch", scratch, linear_int8_scratch_bytes(lanes, k)}, {inputs, out});
     });
     if (checked != NERVE_B200_OK || lanes == 0) return checked;
     return linear_call(name, true, [&](const OperatorDevice *device) {
@@ -774,6 +796,10 @@ int32_t nerve_b200_op_experts_int8(const void *x, const void *ids, const void *w
         check_pointer(name, "y", y, 2);
         check_pointer(name, "residual", residual, 2, true);
         check_pointer(name, "scratch", scratch, 16);
+        const size_t rows = static_cast<size_t>(tokens) * hidden * 2, routes = static_cast<size_t>(tokens) * top_k * 4;
+        const Span inputs{"x", x, rows}, added{"residual", residual == y ? nullptr : residual, rows}, out{"y", y, rows}, chosen{"ids", ids, routes}, factors{"weights", weights, routes};
+        check_apart(name, out, {added, chosen});  // (x and the weights are read before)
+        check_apart(name, {"scratch", scratch, experts_int8_scratch_bytes(tokens, top_k, experts, hidden, inter)}, {inputs, added, out, chosen, factors});
     });
     if (checked != NERVE_B200_OK || tokens == 0) return checked;
     return linear_call(name, true, [&](const OperatorDevice *device) {

@@ -98,3 +98,32 @@ def test_scratch_bytes_are_what_the_header_says():
             least = up(rows * up(k, 128), 256) + up(4 * lanes, 256)
             split = 2 * 32 * 2 * min(256, up(lanes, 32)) * 128 * 4 + 256 if lanes > 8 and k >= 4096 else 0
             assert library.nerve_b200_op_linear_int8_scratch_bytes(lanes, k) == least + split <= least + 16_800_000, (lanes, k)
+
+
+FAR = [A * (16 * i + 16) for i in range(10)]  # addresses 16 MB apart
+
+
+@pytest.mark.parametrize("change,words", [
+    ({"residual": FAR[3], "to_f32": 1}, "y and residual overlap"),  # in place, but not of one size
+    ({"residual": FAR[3] + 4 * 32 * 2 - 2}, "y and residual overlap"), ({"residual": FAR[3] - 64}, "y and residual overlap"),
+    ({"scratch": FAR[0]}, "scratch and x overlap"), ({"scratch": FAR[3] - 512}, "scratch and y overlap"), ({"residual": FAR[5] + 512, "scratch": FAR[5]}, "scratch and residual overlap"),
+])
+def test_linear_onto_its_inputs(change, words):
+    a = {"x": FAR[0], "w": FAR[1], "scale": FAR[2], "y": FAR[3], "residual": None, "scratch": FAR[4], "lanes": 4, "n": 32, "k": 64, "to_f32": 0} | change
+    assert words in refused("nerve_b200_op_linear_int8", *(a[key] for key in ("x", "w", "scale", "y", "residual", "scratch", "lanes", "n", "k", "to_f32")), None)
+
+
+@pytest.mark.parametrize("change,words", [({"scratch": FAR[0] - 16}, "scratch and x overlap"), ({"scratch": FAR[5]}, "scratch and y overlap")])
+def test_pair_onto_its_inputs(change, words):
+    a = {"x": FAR[0], "gate": FAR[1], "gate_scale": FAR[2], "up": FAR[3], "up_scale": FAR[4], "y": FAR[5], "scratch": FAR[6], "lanes": 4, "n": 64, "k": 64} | change
+    assert words in refused("nerve_b200_op_linear_int8_silu_pair", *(a[key] for key in ("x", "gate", "gate_scale", "up", "up_scale", "y", "scratch", "lanes", "n", "k")), None)
+
+
+@pytest.mark.parametrize("change,words", [
+    ({"residual": FAR[7] + 2}, "y and residual overlap"), ({"y": FAR[1]}, "y and ids overlap"), ({"scratch": FAR[0]}, "scratch and x overlap"), ({"scratch": FAR[2]}, "scratch and weights overlap"),
+    ({"scratch": FAR[7]}, "scratch and y overlap"), ({"scratch": FAR[1]}, "scratch and ids overlap"),
+])
+def test_experts_onto_their_inputs(change, words):
+    names = ("x", "ids", "weights", "gate_up", "gate_up_scale", "down", "down_scale", "y", "residual", "scratch")
+    a = dict(zip(names, FAR)) | {"residual": None} | change
+    assert words in refused("nerve_b200_op_experts_int8", *(a[name] for name in names), 4, 2, 8, 64, 32, None)
