@@ -269,10 +269,12 @@ struct Grouping {
     int *counts;
     __device__ __forceinline__ bool routed(int id) const { return static_cast<uint32_t>(id) < static_cast<uint32_t>(experts); }
 };
-// The most routes that every CTA of the rows' quantisation looks through, with that many threads at least: a launch less than with
-// expert_groups_kernel in front (14 tokens of 6 of 29 experts 14.4 us and 16.6, 24 of 8 of 128 experts 71.8 and 73.4, 250 of 2 of 8
-// 20.1 and 22.1, but 64 of 8 of 128 94.3 and 92.0; 120 of 8 of 16 with twice as many allowed 23.1 and 20.8).
-constexpr int FEW_GROUPED = 512, GROUPING_THREADS = 128;
+// The most routes that every CTA of the rows' quantisation looks through, for that many routes a token and with that many threads at
+// least: a launch less than with expert_groups_kernel in front.  Over 54 shapes of up to 512 routes 1.2 us less on average (14 tokens of 6 of
+// 29 experts 20.0 us and 22.0, 24 of 8 of 128 experts 87.4 and 89.0, 250 of 2 of 8 17.4 and 18.7; at worst 1.5 more, 64 of 8 of 128
+// experts 107.0 and 105.4).  A token's routes are looked up one after the other: 32 of 16 of 64 25.9 and 26.6, but 16 of 32 of 128 35.9 and
+// 34.6, 9 of 56 of 64 29.7 and 26.2.  120 of 8 of 16, with twice as many routes allowed, 23.1 and 20.8.
+constexpr int FEW_GROUPED = 512, FEW_GROUPED_TOP_K = 16, GROUPING_THREADS = 128;
 
 // The routes of the table, some a thread; those to no expert behind all others.
 constexpr int ROUTES_HELD = FEW_GROUPED / GROUPING_THREADS;
@@ -322,7 +324,7 @@ __device__ __forceinline__ void make_tiles(const Grouping &g) {
 __device__ __forceinline__ void find_places(const Grouping &g, int first, int count, int *places) {
     int ids[ROUTES_HELD];
     load_routes(g, ids);
-    __shared__ int own[ROUTING_MAX_TOP_K];
+    __shared__ int own[FEW_GROUPED_TOP_K];
     for (int j = threadIdx.x; j < count; j += blockDim.x) {
         own[j] = g.ids[first + j];
         places[j] = g.routed(own[j]) ? 0 : -1;
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(512) quantise_rows_kernel(const T *x, int8_t *
 #pragma unroll
     for (int i = 0; i < HELD; i++)
         if (first + i * step < k) held[i].load(row, first + i * step, wide);
-    __shared__ int found[GROUPS ? ROUTING_MAX_TOP_K : 1];
+    __shared__ int found[GROUPS ? FEW_GROUPED_TOP_K : 1];
     if constexpr (GROUPS) find_places(groups, at_row * top_k, top_k, found);
     uint32_t amax = 0;
 #pragma unroll
@@ -1355,7 +1357,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
 
 // ---- experts: routes grouped by expert
 
-// For tables of more than FEW_GROUPED routes.  Bound by the chain of its loads, shared-memory atomics and barriers: 16384 routes of
+// For tables of more than FEW_GROUPED routes, or FEW_GROUPED_TOP_K a token.  Bound by the chain of its loads, shared-memory atomics and barriers: 16384 routes of
 // 128 experts take 8 us, 1000 take 4.
 // One CTA (several would have to wait for one another's counts) counts the routes of every expert, gives each a place behind those of the experts before it, and cuts every
 // expert's places into tiles of tile_lanes.  Which of an expert's routes comes first is left to chance: a row's result does
@@ -1809,7 +1811,7 @@ cudaError_t launch_experts_int8(const uint16_t *x, const int *ids, const float *
     }
     const int most_tiles = pairs / first.tile_lanes + std::min(experts, pairs);
     cudaError_t status;
-    if (pairs <= FEW_GROUPED) {
+    if (pairs <= FEW_GROUPED && top_k <= FEW_GROUPED_TOP_K) {
         status = launch_quantise_rows<uint16_t, HeldBf16, 4>(x, part.xq, part.x_scales, nullptr, nullptr, part.pair_of, nullptr, tokens, top_k, hidden, stream, 0, nullptr, 0,
                                                              Grouping{ids, pairs, experts, first.tile_lanes, part.tiles, part.counts});
     } else {

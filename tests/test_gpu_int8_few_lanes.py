@@ -33,3 +33,20 @@ def test_pair(lanes, n, k):
     half = n // 2 + 3
     assert torch.equal(ref.pair(x, gate[:half], gate_scale[:half], up[:half], up_scale[:half]), y[:, :half])
     assert torch.equal(ref.pair(x[:1], gate, gate_scale, up, up_scale)[0], y[0])
+
+
+@pytest.mark.parametrize("tokens,top_k", [(32, 16), (30, 17), (9, 56), (16, 32), (33, 16)])
+def test_experts_of_many_routes_a_token(tokens, top_k):
+    """Routes that the rows' quantisation groups itself and those that a launch in front does, at the border between the two."""
+    g = ref.generator(tokens * top_k)
+    (gate_up, gate_up_scale), (down, down_scale) = ref.weights(g, 64, 2 * 96, 256), ref.weights(g, 64, 256, 96)
+    x, layer = ref.activations(g, tokens, 256), (gate_up, gate_up_scale * 3, down, down_scale)
+    ids = torch.rand((tokens, 64), generator=g, device="cuda").argsort(dim=1)[:, :top_k].to(torch.int32).contiguous()
+    weights = torch.rand((tokens, top_k), generator=g, device="cuda").softmax(dim=1).contiguous()
+    ids[3, 2:5] = -1
+    ids[5] = 63
+    y = ref.experts(x, ids, weights, *layer)
+    ref.assert_close(y, *ref.experts_reference(x, ids, weights, *layer))
+    for token in (0, 3, 5, tokens - 1):
+        some = slice(token, token + 1)
+        assert torch.equal(ref.experts(x[some], ids[some], weights[some], *layer)[0], y[token])
