@@ -332,9 +332,10 @@ __device__ __forceinline__ bool route_in_32_bits(const T *logits, const float *b
             rank += value_of(group_next);
             largest = fmaxf(largest, fabsf(value_of(group_next)));
         }
+        if (open) rank = fminf(fmaxf(rank, -LARGEST), LARGEST);  // (two of the lowest values are no closed group's -infinity)
         // Where the rank lies in truth: it is off by its summands' errors, which may be more than all of it where biases of both signs
         // cancel.  (An infinite one lies anywhere.)
-        const float error = scored ? 0.5f * margin(largest) : 0.0f, low = fminf(rank, LARGEST) - error, high = fmaxf(rank, -LARGEST) + error;
+        const float error = scored ? 0.5f * margin(largest) : 0.0f, low = rank - error, high = rank + error;
         // the groups in front of this thread's: each of a group's threads compares some
         const int team = max(threads, 1), team_first = own_group * team;
         int before = 0;

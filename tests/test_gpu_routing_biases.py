@@ -74,3 +74,18 @@ def test_biases_of_the_lowest_value(count, groups, chosen, group_scores, lowest,
     for masked in (torch.rand(count, generator=g, device="cuda") < 0.5, torch.arange(count, device="cuda") % size > 0, torch.arange(count, device="cuda") // size < groups // 2,
                    torch.arange(count, device="cuda") // size != groups - 1, torch.ones(count, dtype=torch.bool, device="cuda")):
         agrees(logits, (torch.randn(count, generator=g, device="cuda") * 0.1).masked_fill(masked, lowest), r)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("count,groups,chosen", [(40, 8, 3), (256, 8, 4), (64, 32, 9), (244, 4, 2)])
+def test_closed_groups_beside_groups_of_the_lowest_biases(count, groups, chosen, sigmoid):
+    """Two choices of the lowest value add up to -infinity in 32 bits; the group stays in front of those without an open expert."""
+    r, size = nb.Routing(experts=count, top_k=min(8, count // groups * chosen), sigmoid=sigmoid, groups=groups, chosen_groups=chosen, group_scores=2), count // groups
+    g = ref.generator(count)
+    lowest = float(torch.finfo(torch.float32).min)
+    logits = torch.randn((groups + 8, count), generator=g, device="cuda")
+    closed = torch.rand((groups + 8, groups), generator=g, device="cuda") < 0.7
+    closed[:groups] = torch.ones((groups, groups), dtype=torch.bool, device="cuda") ^ torch.eye(groups, dtype=torch.bool, device="cuda")  # one group is open, each in turn
+    logits.masked_fill_(closed.repeat_interleave(size, dim=1), -math.inf)
+    for masked in (torch.ones(count, dtype=torch.bool, device="cuda"), torch.rand(count, generator=g, device="cuda") < 0.8, torch.arange(count, device="cuda") // size != groups - 1):
+        agrees(logits, (torch.randn(count, generator=g, device="cuda") * 0.1).masked_fill(masked, lowest), r)
