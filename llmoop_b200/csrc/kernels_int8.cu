@@ -19,8 +19,8 @@
 // factors of an output.
 //
 // The experts' products are the same kernels over tiles that expert_groups_kernel, or few tokens themselves, make of the routes.
-// Waits are bounded; a wait that expires sets the error word, and the CTA still frees its tensor memory.  The unbounded wait
-// for the kernel in front comes before them in every role, so none of them counts that kernel's time.
+// Waits are bounded; a wait that expires sets the error word, and the CTA still frees its tensor memory.  In every role the unbounded
+// wait for the kernel in front comes before the first of them that could last as long, so none counts that kernel's time.
 //
 // No pointer here is __restrict__: what the kernel in front writes may only be read behind the wait for it, and a load through a
 // const __restrict__ pointer, which promises that nobody writes, is free to move in front of that (the routes of a replayed
@@ -1103,8 +1103,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     // not before the tensor memory is this CTA's: one of the next kernel's that took it first would wait for this one.  The experts'
-    // gate/up product also waits for the kernel in front before: the down product, which starts then, may read the routes and the
-    // weights while this one still runs, and waits for its rows alone.
+    // gate/up product also waits for the kernel in front before: the down product, which may start then, reads the routes and the
+    // weights while this one still runs, and waits for its rows alone.  (Its CTAs start where a multiprocessor has their shared memory left or
+    // once this kernel's have gone: beside the 144 CTAs of one token of eight routes of 2048 x 768, which take all of it, on four.)
     if (MODE == EXPERTS_PAIR) grid_dependency_wait();
     grid_launch_dependents();
     uint32_t tmem;
@@ -1135,6 +1136,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) int8_stream_kernel(const __
         for (int tile = first_tile; tile < last_tile && alive; tile++) {
             const int row0 = tile % a.row_tiles * a.rows, expert = GROUPED ? routes.expert[tile / a.row_tiles] : 0;
             for (int step = 0; step < steps; step++) {
+                if (DOWN && issued == a.stages) grid_dependency_wait();  // from here on the MMAs release the stages
                 if (!wait_barrier(empty + stage * 8, parity, a.error_flag)) {
                     for (int s = 0; s < a.stages && s < issued; s++) {  // the copies in flight land before the CTA gives its memory up
                         const int which = (issued - 1 - s) % a.stages;
