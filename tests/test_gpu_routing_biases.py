@@ -89,3 +89,14 @@ def test_closed_groups_beside_groups_of_the_lowest_biases(count, groups, chosen,
     logits.masked_fill_(closed.repeat_interleave(size, dim=1), -math.inf)
     for masked in (torch.ones(count, dtype=torch.bool, device="cuda"), torch.rand(count, generator=g, device="cuda") < 0.8, torch.arange(count, device="cuda") // size != groups - 1):
         agrees(logits, (torch.randn(count, generator=g, device="cuda") * 0.1).masked_fill(masked, lowest), r)
+
+
+@pytest.mark.parametrize("apart", [1e-9, 1e-11])
+@pytest.mark.parametrize("middle", [0.0, 12.0, 19.0])
+def test_candidates_that_a_bias_of_a_billionth_tells_apart(apart, middle):
+    """Scores equal or next to one another in 32 bits, and choices that 64 bits hold apart by more than their exponentials' error."""
+    g = ref.generator(5)
+    logits = middle + torch.randint(0, 3, (64, 128), generator=g, device="cuda") * 2.0 ** -18
+    bias = torch.randn(128, generator=g, device="cuda") * apart
+    for some in (bias, bias + 0.25):
+        agrees(logits, some, nb.Routing(experts=128, top_k=8, sigmoid=True))
