@@ -308,7 +308,10 @@ int32_t nerve_b200_op_linear_int8_silu_pair(const void *x_device, const void *ga
  * where open experts run out; weights f32 [tokens][top_k]: the scores without the bias (0 for -1), over the sum of the
  * chosen ones' where renormalise != 0 (0 where that sum is 0), times scale.  Scores and choices are held in 64 bits.
  * experts 1..1024, top_k 1..64 and no more than chosen_groups' experts, groups 1..32 that divide the experts into runs of
- * at least group_scores. */
+ * at least group_scores.
+ * Time: 16384 tokens of 256 experts and top 8 take 16 us.  Tokens that 32 bits cannot decide take the whole way in 64: with a sigmoid
+ * logit above 20 the same take 43 us, with top 16, 20 and 24 (candidates of close scores fill a warp) 26, 53 and 101, with top 32 or
+ * more 128 and more. */
 typedef struct nerve_b200_routing {
     int32_t experts, top_k;
     int32_t sigmoid; /* 0 = softmax, 1 = sigmoid */

@@ -12,7 +12,7 @@
 //                         (2048 x 4096 x 14336: 85 us, 2.8 POP/s; 8192 x 8192 x 8192: 3.0), or the weights' bytes (160 lanes of
 //                         the 28672 x 8192 pair: 86 us a call, 5.6 TB/s), or the outputs where K is short
 //   int8_stream_kernel    up to 128 lanes; the weights' bytes (4 x 128256 x 4096: 83 us, 6.3 TB/s) or the chain of its steps
-//                         (1 x 4096 x 4096: 4.6 us a call)
+//                         (1 x 4096 x 4096: 6.0 us a call from DRAM, 4.9 from L2)
 //   expert_groups_kernel, experts_sum_kernel  around the experts' products; the chain of its barriers, DRAM
 //
 // The gate/up pair multiplies the same lanes by a tile of each matrix into sums that lie side by side, so that one thread holds both
@@ -1587,8 +1587,8 @@ bool plan_stages(StreamArgs &args, size_t most, size_t *bytes) {
     return true;
 }
 // Where a CTA's share of the weights is small, half of a multiprocessor's shared memory does: a CTA of the next call can
-// start on the other half while this one writes its outputs (one lane of 4096 x 4096: 4.3 us a call, 4.8 with all of it; four of a
-// 14336 x 4096 pair: 24.5 with half, 22 with all of it).
+// start on the other half while this one writes its outputs (one lane of 4096 x 4096 from L2: 5.0 us a call, 5.2 with all of it, from
+// DRAM 6.0 and 5.9; four of a 14336 x 4096 pair: 25.6 with half, 22.0 with all of it).
 size_t stream_share(const StreamArgs &args) {
     const int blocks = (args.k + BLOCK_K - 1) / BLOCK_K, count = multiprocessors(), steps = (args.row_tiles + count - 1) / count * ((blocks + args.groups - 1) / args.groups);
     return steps <= STREAM_SMALL_SHARE ? SMEM_HALF : SMEM_LIMIT;

@@ -10,11 +10,12 @@
 // exponential made of them.  64-bit exponentials and keys are also what such a kernel spends its time on (16384 tokens of 256
 // experts in 8 groups: 81 us), so that 32 bits, with a bound on the error, find the few candidates, which alone are scored and ranked
 // in 64.  Groups closer than the error are ranked in 64 bits where they stand, if each is a run of threads.  Tokens that cannot be
-// decided so are done by the definition: more than 31 candidates (top_k 32 to 64), sigmoids of logits above 20, logits of +inf, scores
+// decided so are done by the definition: more than 31 candidates (top_k 32 to 64, and often from 20 on), sigmoids of logits above 20, logits of +inf, scores
 // below 1e-250, and groups next to one another that are no runs of threads, have no scores or hold choices from 1e30 on.
 //
-// One warp per token, of which the chip holds enough to cover the loads.  Bound by the instructions that it issues, some 1080 a token:
-// 16384 tokens of 256 experts in 8 groups, 21.5 us, of which the logits' bytes are 2.8.  One token of 128 experts takes 2.8 us, a launch and the
+// One warp per token, of which the chip holds enough to cover the loads.  Bound by the instructions that it issues, some 1080 a token, of which
+// some 200 go by the experts and the others are a whole warp's steps for one token (groups, limit, candidates, ranks, weights):
+// 16384 tokens of 256 experts in 8 groups, 23.0 us, of which the logits' bytes are 2.8.  One token of 128 experts takes 2.7 us, a launch and the
 // chain of reductions.  (No pointer is __restrict__: loads through those may move in front of the wait
 // for the kernel that writes the logits.)
 #include <algorithm>
